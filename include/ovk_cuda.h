@@ -499,6 +499,127 @@ OVK_API int32_t ovk_qlinear_global_average_pool(ovk_ctx *ctx, const void *x, int
                                                 int64_t n, int64_t c, int64_t hw, float x_scale,
                                                 int32_t x_zp, float y_scale, int32_t y_zp, void *out);
 
+/* ------------------------------------------- the attention of a decoder layer
+ * What lies between the q | k | v product and the o product of a decoder layer:
+ * rotary positions, the key / value cache in 4 bits, attention over it, and
+ * attention over a whole prompt.  (The reference runs the ONNX graphs of these
+ * blocks node by node; it has no fused counterpart, and no 4-bit cache.)
+ *
+ * Sequences are packed: the tokens of all sequences of a batch lie one after the
+ * other, sequence b in rows cu[b] .. cu[b + 1] - 1 of every [tokens, heads,
+ * head_dim] tensor; cu is an int32 array of batch + 1 row numbers on the DEVICE,
+ * ascending from cu[0] >= 0.  Rows outside every sequence are neither read nor
+ * written.  A sequence may be empty.  Activations are OVK_FLOAT or OVK_FLOAT16
+ * (the two types the products of this library take and give); query head h reads
+ * key head h / (q_heads / kv_heads).
+ *
+ * Lengths and page numbers live on the device and cannot be refused before the
+ * launch: a sequence, position or page outside what the call describes is left
+ * out (its rows are written as zeros, or not stored to the cache), nothing
+ * outside the tensors is touched, and the next ovk_flush returns
+ * OVK_INVALID_ARGUMENT.
+ *
+ * Like every operator these only enqueue on the context's stream.  They keep no
+ * state in the context, so calls on several contexts and replays of captured
+ * graphs do not disturb one another as long as their outputs, caches and
+ * workspaces differ. */
+/* One [tokens, heads, head_dim] tensor; elements of a head are contiguous, the
+ * strides count elements.  A slice of a fused q | k | v product is one of these. */
+typedef struct ovk_heads {
+    void *data;
+    int64_t heads, token_stride, head_stride;
+} ovk_heads;
+typedef struct ovk_rotary_params {
+    int64_t tokens, head_dim;
+    int64_t rotary_dim;   /* the first rotary_dim elements of a head are turned (even), the rest copied */
+    int64_t max_position; /* rows of the tables */
+    int32_t dtype, table_dtype, positions_dtype; /* f32 / f16; f32 / f16; int32 / int64 */
+    int32_t interleaved;  /* 1: pairs (2i, 2i + 1); 0: pairs (i, i + rotary_dim / 2) */
+    int32_t axes;         /* 1 to 4 */
+    int32_t sections[4];  /* pairs per axis, in order; their sum is rotary_dim / 2 */
+} ovk_rotary_params;
+/* Rotary positions with several axes: pair i belongs to the axis whose section
+ * holds it and turns by the angle of that axis's position,
+ *   out[a] = x[a] cos - x[b] sin,  out[b] = x[b] cos + x[a] sin,
+ * cos, sin = tables [max_position, rotary_dim / 2] at [positions[axis][token]][i],
+ * in f32, rounded once.  positions is [axes, tokens].  One axis is the operator
+ * RotaryEmbedding of text decoders; three are time, height and width.  `count`
+ * (1 or 2) tensors are turned in one launch - queries and keys.  out[j] may be
+ * x[j] itself (in place), but not overlap it otherwise.  A token with a position
+ * outside the tables writes zeros (see above). */
+OVK_API int32_t ovk_rotary(ovk_ctx *ctx, const ovk_rotary_params *p, int32_t count,
+                           const ovk_heads *x, const ovk_heads *out, const void *positions,
+                           const void *cos_table, const void *sin_table);
+/* A paged key / value cache in 4 bits.  Token t of a sequence lies in page
+ * block_table[t / page_size] at place t % page_size; a row is one head of one
+ * token, rows are ordered [pages, kv_heads, page_size] (one page per sequence
+ * makes it a plain [batch, kv_heads, capacity] cache).  A row's codes, scales and
+ * zero points are those of a row of ovk_gather_block_quantized's table: head_dim
+ * / 2 bytes, element 2i in the low nibble; head_dim / block_size fp16 scales;
+ * ceil(head_dim / block_size / 2) bytes of zero points, two a byte (both NULL:
+ * implicit 8).  head_dim 64, 128 or 256; block_size 32, 64 or 128.  All pointers
+ * 16-byte aligned; fewer than 2^31 rows. */
+typedef struct ovk_kv4_cache {
+    void *k, *v;
+    void *k_scales, *v_scales;
+    void *k_zero_points, *v_zero_points;
+    int64_t pages, kv_heads, page_size, head_dim, block_size;
+} ovk_kv4_cache;
+/* The sequences of a call: `tokens` packed rows; sequence b brings n = cu[b + 1]
+ * - cu[b] new tokens and has lens[b] tokens once they are in the cache, so its
+ * new token i has position lens[b] - n + i.  block_table is [batch, max_pages]
+ * int32.  All three arrays are on the device. */
+typedef struct ovk_kv4_batch {
+    int64_t tokens, batch, max_pages;
+    const int32_t *cu_tokens, *lens, *block_table;
+} ovk_kv4_batch;
+/* Writes the new tokens' keys and values into the cache.  Per block of
+ * block_size values, with lo = min(0, least) and hi = max(0, greatest):
+ *   scale = fp16((hi - lo) / 15),           zero = rne(-lo / scale)   with zero points
+ *   scale = fp16(max(hi / 7, -lo / 8)),     zero = 8                  without
+ *   code = clamp(rne(x / scale) + zero, 0, 15),
+ * the quotients to their exact rounding (the scale's by way of f32).  A scale
+ * above 65504 becomes 65504; a scale of 0 stores zeros; a NaN stores a zero.  k
+ * and v are [tokens, kv_heads, head_dim] of `dtype`.  Two sequences must not
+ * bring new tokens to the same page and place. */
+OVK_API int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, const ovk_kv4_batch *batch,
+                               const ovk_heads *k, const ovk_heads *v, int32_t dtype);
+/* Causal attention of the new tokens over the cache, their own rows included:
+ *   out = softmax(scale q K^T) V,  K and V = (code - zero) * scale of the rows,
+ * a token at position p reads positions max(0, p - window + 1) .. p (window 0: no
+ * lower limit); one that reads nothing gives zeros.  Scores, softmax and sums are
+ * f32.  q and out are [tokens, q_heads, head_dim] of `dtype`, 16-byte aligned rows.
+ * max_tokens: the most new tokens a sequence brings (1 in decode); a sequence
+ * that brings more is left out as described above.
+ * workspace: partial results of sequences that several CTAs share, 16-byte
+ * aligned, ovk_attention_kv4_workspace() bytes; NULL takes the context's own
+ * workspace, which grows on demand (bring one where the call is captured). */
+OVK_API int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, const ovk_kv4_batch *batch,
+                                  const ovk_heads *q, const ovk_heads *out, int32_t dtype,
+                                  int64_t max_tokens, float scale, int64_t window, void *workspace,
+                                  size_t workspace_bytes);
+/* Bytes of workspace that any call with this cache's shape, this many query heads
+ * and at most this max_tokens needs. */
+OVK_API int32_t ovk_attention_kv4_workspace(ovk_ctx *ctx, const ovk_kv4_cache *cache, int64_t q_heads,
+                                            int64_t max_tokens, int32_t dtype, size_t *bytes);
+/* Attention of packed prompts: out = softmax(scale q k^T) v within each sequence.
+ * cu_q and cu_k give each sequence's query and key rows; where they differ the
+ * queries are the LAST tokens of the keys' sequence (a chunk after earlier ones),
+ * so query i has position p = n_k - n_q + i.  causal: it reads keys up to p;
+ * window > 0: keys from p - window + 1; a row that reads nothing gives zeros.
+ * Scores, softmax and sums are f32.  head_dim 1 to 256.  The f16 tensor-core
+ * kernel takes 16-byte aligned rows (head_dim a multiple of 8); other layouts
+ * and f32 run on the CUDA cores. */
+typedef struct ovk_prompt_params {
+    int64_t q_tokens, k_tokens, batch, head_dim;
+    int32_t dtype, causal;
+    int64_t window;
+    float scale;
+} ovk_prompt_params;
+OVK_API int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p, const ovk_heads *q,
+                                     const ovk_heads *k, const ovk_heads *v, const int32_t *cu_q,
+                                     const int32_t *cu_k, const ovk_heads *out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -138,6 +138,15 @@ int32_t ovk_flush(ovk_ctx *ctx)
             return ovk_fail(ctx, OVK_INVALID_ARGUMENT,
                             "GatherBlockQuantized: an index read on the device fell outside the table "
                             "(its row was written as zeros)");
+        if (st == OVK_DEV_BAD_POSITION)
+            return ovk_fail(ctx, OVK_INVALID_ARGUMENT,
+                            "Rotary: a position read on the device fell outside the tables (its token was written as zeros)");
+        if (st == OVK_DEV_BAD_PAGE)
+            return ovk_fail(ctx, OVK_INVALID_ARGUMENT,
+                            "4-bit cache: a position or page number read on the device fell outside the cache (it was left out)");
+        if (st == OVK_DEV_BAD_SEQUENCE)
+            return ovk_fail(ctx, OVK_INVALID_ARGUMENT,
+                            "Attention: sequence bounds read on the device disagree with the call (the sequence was left out)");
         return ovk_fail(ctx, OVK_TIMEOUT, "a device-side wait gave up (code %d: %s)", st,
                         st == OVK_DEV_TIMEOUT_TMA    ? "bulk copy never arrived"
                         : st == OVK_DEV_TIMEOUT_MMA  ? "tensor core never signalled"

@@ -1,0 +1,197 @@
+// The 4-bit key / value cache: argument checks and the write of new tokens.
+//
+// Bytes bound the write: 2 or 4 bytes are read per value and about 0.6 stored.
+// A thread holds eight values of a row - one 32-bit word of codes - and the
+// block_size / 8 threads of a block find its range with shuffles; keys and values
+// of a row go through the same thread, so its place in the cache is found once.
+//
+// The quotients are rounded exactly without dividing: for an fp16 scale s and an
+// integer n <= 16, (n + 1/2) s has at most 16 significant bits, so the sign of
+// fma(-(n + 1/2), s, x) is the sign of x / s - (n + 1/2), and a first guess
+// n = rint(x * (1 / s)), off by at most one, is set right by the two borders
+// around it.  The scale itself is one f64 quotient a block.
+#include "attention.cuh"
+
+int32_t ovk_check_kv4(ovk_ctx *ctx, const char *op, const ovk_kv4_cache *c)
+{
+    OVK_REQUIRE(ctx, c, "%s: the cache is null", op);
+    OVK_REFUSE(ctx, c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256, "%s: head_dim %lld (64, 128 or 256)", op,
+               (long long)c->head_dim);
+    OVK_REFUSE(ctx, c->block_size != 32 && c->block_size != 64 && c->block_size != 128, "%s: block_size %lld (32, 64 or 128)", op,
+               (long long)c->block_size);
+    OVK_REQUIRE(ctx, c->head_dim % c->block_size == 0, "%s: block_size %lld does not divide head_dim %lld", op,
+                (long long)c->block_size, (long long)c->head_dim);
+    OVK_REQUIRE(ctx, c->pages >= 0 && c->kv_heads >= 1 && c->kv_heads <= OVK_MAX_HEADS && c->page_size >= 1 &&
+                         c->page_size < (int64_t(1) << 31) && c->pages < (int64_t(1) << 31) &&
+                         (c->pages == 0 || c->kv_heads * c->page_size < (int64_t(1) << 31) / c->pages + 1) &&
+                         c->pages * c->kv_heads * c->page_size < (int64_t(1) << 31),
+                "%s: a cache of %lld pages of %lld heads x %lld places (fewer than 2^31 rows)", op, (long long)c->pages,
+                (long long)c->kv_heads, (long long)c->page_size);
+    OVK_REQUIRE(ctx, c->pages == 0 || (c->k && c->v && c->k_scales && c->v_scales), "%s: the cache has no data", op);
+    OVK_REQUIRE(ctx, !c->k_zero_points == !c->v_zero_points, "%s: zero points for keys and values, or for neither", op);
+    OVK_REQUIRE(ctx, aligned_to(c->k, 16) && aligned_to(c->v, 16) && aligned_to(c->k_scales, 16) && aligned_to(c->v_scales, 16) &&
+                         aligned_to(c->k_zero_points, 16) && aligned_to(c->v_zero_points, 16),
+                "%s: the cache's tensors must be 16-byte aligned", op);
+    return OVK_OK;
+}
+
+int32_t ovk_check_kv4_batch(ovk_ctx *ctx, const char *op, const ovk_kv4_batch *b)
+{
+    OVK_REQUIRE(ctx, b, "%s: the batch is null", op);
+    OVK_REQUIRE(ctx, b->tokens >= 0 && b->tokens < (int64_t(1) << 31) && b->batch >= 0 && b->batch < (1 << 24) && b->max_pages >= 0 &&
+                         b->max_pages < (int64_t(1) << 31),
+                "%s: %lld tokens of %lld sequences, %lld pages each", op, (long long)b->tokens, (long long)b->batch,
+                (long long)b->max_pages);
+    OVK_REQUIRE(ctx, b->batch == 0 || (b->cu_tokens && b->lens && (b->block_table || b->max_pages == 0)), "%s: null sequence arrays", op);
+    OVK_REQUIRE(ctx, aligned_to(b->cu_tokens, 4) && aligned_to(b->lens, 4) && aligned_to(b->block_table, 4), "%s: misaligned sequence arrays", op);
+    return OVK_OK;
+}
+
+namespace {
+
+struct AppendArgs {
+    const void *x[2];  // keys, values
+    int64_t token_stride[2], head_stride[2];
+    uint8_t *codes[2];
+    __half *scales[2];
+    uint8_t *zero_points[2];
+    const int32_t *cu, *lens, *table;
+    int64_t items;  // tokens * heads * head_dim / 8
+    int batch, heads, head_dim, block_size, page_size, pages;
+    int64_t max_pages;
+    int *status;
+};
+
+// round-to-nearest-even of x / s for an fp16 value s > 0, clamped to +-16; inv is about 1 / s
+__device__ __forceinline__ int quotient(float x, float s, float inv)
+{
+    const float guess = fminf(fmaxf(rintf(x * inv), -16.0f), 16.0f);
+    const float above = fmaf(-(guess + 0.5f), s, x);  // > 0: x / s lies above the upper border
+    const float below = fmaf(-(guess - 0.5f), s, x);  // < 0: below the lower one
+    const int n = int(guess);
+    const bool odd = n & 1;
+    return n + (above > 0.0f || (above == 0.0f && odd) ? 1 : 0) - (below < 0.0f || (below == 0.0f && odd) ? 1 : 0);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
+{
+    const int64_t item = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int words = a.head_dim / 8;  // a power of two up to 32: a row lies inside a warp
+    const int64_t at = item / words;
+    const int word = int(item - at * words);
+    const int token = int(at / a.heads), head = int(at - int64_t(token) * a.heads);
+    int64_t row = -1;
+    if (item < a.items) {
+        const int b = sequence_of(a.cu, a.batch, token);
+        if (b >= 0) {
+            const int64_t position = int64_t(a.lens[b]) - (int64_t(a.cu[b + 1]) - token);
+            const int64_t page = position < 0 ? a.max_pages : position / a.page_size;
+            const int where = page < a.max_pages ? a.table[int64_t(b) * a.max_pages + page] : -1;
+            if (where >= 0 && where < a.pages)
+                row = (int64_t(where) * a.heads + head) * a.page_size + (position - page * a.page_size);
+            else if (word == 0)
+                atomicExch(a.status, OVK_DEV_BAD_PAGE);
+        }
+    }
+    const int lanes = a.block_size / 8, blocks = a.head_dim / a.block_size;
+    const int block = word / lanes;
+    float x[2][8];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        if (row >= 0) {
+            load_row<T, 8, VEC>(static_cast<const T *>(a.x[j]) + token * a.token_stride[j] + head * a.head_stride[j] + 8 * word, x[j]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                x[j][e] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        float lo = 0.0f, hi = 0.0f;  // fminf and fmaxf drop a NaN
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            lo = fminf(lo, x[j][e]), hi = fmaxf(hi, x[j][e]);
+        for (int o = 1; o < lanes; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const double step = a.zero_points[j] ? (double(hi) - double(lo)) / 15.0 : fmax(double(hi) / 7.0, -double(lo) / 8.0);
+        const __half scale = __float2half_rn(fminf(float(step), 65504.0f));
+        const float s = __half2float(scale);
+        const float inv = s > 0.0f ? 1.0f / s : 0.0f;  // a scale is at least 2^-24: finite
+        int zero = 8;
+        if (a.zero_points[j])
+            zero = s > 0.0f ? max(0, min(15, quotient(-lo, s, inv))) : 0;
+        uint32_t codes = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float v = x[j][e] == x[j][e] ? x[j][e] : 0.0f;
+            const int q = s > 0.0f ? quotient(v, s, inv) : 0;
+            codes |= uint32_t(max(0, min(15, q + zero))) << (4 * e);
+        }
+        // the block to the right shares this block's byte of zero points
+        const int next = __shfl_down_sync(0xffffffffu, zero, lanes);
+        if (row >= 0) {
+            reinterpret_cast<uint32_t *>(a.codes[j])[row * words + word] = codes;
+            if (word % lanes == 0) {
+                a.scales[j][row * blocks + block] = scale;
+                if (a.zero_points[j] && block % 2 == 0)
+                    a.zero_points[j][row * ((blocks + 1) / 2) + block / 2] = uint8_t(zero | (block + 1 < blocks ? next << 4 : 0));
+            }
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, const ovk_kv4_batch *batch, const ovk_heads *k,
+                                  const ovk_heads *v, int32_t dtype)
+{
+    const char *op = "KV4Append";
+    int32_t rc = ovk_check_kv4(ctx, op, cache);
+    if (rc == OVK_OK)
+        rc = ovk_check_kv4_batch(ctx, op, batch);
+    if (rc != OVK_OK)
+        return rc;
+    OVK_REFUSE(ctx, !ovk_is_activation(dtype), "%s: dtype %d (f32 or f16)", op, dtype);
+    const size_t elem = ovk_elem_bytes(dtype);
+    rc = ovk_check_heads(ctx, op, "k", k, batch->tokens, cache->head_dim, elem, false);
+    if (rc == OVK_OK)
+        rc = ovk_check_heads(ctx, op, "v", v, batch->tokens, cache->head_dim, elem, false);
+    if (rc != OVK_OK)
+        return rc;
+    OVK_REQUIRE(ctx, k->heads == cache->kv_heads && v->heads == cache->kv_heads, "%s: %lld and %lld heads for a cache of %lld", op,
+                (long long)k->heads, (long long)v->heads, (long long)cache->kv_heads);
+    const int64_t items = batch->tokens * cache->kv_heads * (cache->head_dim / 8);
+    OVK_REQUIRE(ctx, ceil_div64(items, 256) < (int64_t(1) << 31), "%s: %lld tokens of %lld heads are too many for one call", op,
+                (long long)batch->tokens, (long long)cache->kv_heads);
+    OVK_REQUIRE(ctx, ctx, "%s: null context", op);
+    if (items == 0 || batch->batch == 0)
+        return OVK_OK;
+    DeviceGuard guard(ctx->device);
+    AppendArgs a = {};
+    a.x[0] = k->data, a.x[1] = v->data;
+    a.token_stride[0] = k->token_stride, a.token_stride[1] = v->token_stride;
+    a.head_stride[0] = k->head_stride, a.head_stride[1] = v->head_stride;
+    a.codes[0] = static_cast<uint8_t *>(cache->k), a.codes[1] = static_cast<uint8_t *>(cache->v);
+    a.scales[0] = static_cast<__half *>(cache->k_scales), a.scales[1] = static_cast<__half *>(cache->v_scales);
+    a.zero_points[0] = static_cast<uint8_t *>(cache->k_zero_points), a.zero_points[1] = static_cast<uint8_t *>(cache->v_zero_points);
+    a.cu = batch->cu_tokens, a.lens = batch->lens, a.table = batch->block_table;
+    a.items = items;
+    a.batch = int(batch->batch), a.heads = int(cache->kv_heads), a.head_dim = int(cache->head_dim), a.block_size = int(cache->block_size);
+    a.page_size = int(cache->page_size), a.pages = int(cache->pages), a.max_pages = batch->max_pages;
+    a.status = ctx->dev_status;
+    const unsigned grid = unsigned(ceil_div64(items, 256));
+    const bool vec = ovk_rows_aligned(k, elem) && ovk_rows_aligned(v, elem);
+    if (dtype == OVK_FLOAT) {
+        if (vec) kv4_append_kernel<float, true><<<grid, 256, 0, ctx->stream>>>(a);
+        else kv4_append_kernel<float, false><<<grid, 256, 0, ctx->stream>>>(a);
+    } else {
+        if (vec) kv4_append_kernel<__half, true><<<grid, 256, 0, ctx->stream>>>(a);
+        else kv4_append_kernel<__half, false><<<grid, 256, 0, ctx->stream>>>(a);
+    }
+    OVK_LAUNCHED(ctx, vec ? "kv4_append" : "kv4_append_scalar");
+    return OVK_OK;
+}

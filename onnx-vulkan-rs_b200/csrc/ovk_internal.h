@@ -25,6 +25,9 @@ enum : int {
     OVK_DEV_TIMEOUT_PEER = 5,  // a flag another GPU writes never reached the expected value
     OVK_DEV_TIMEOUT_SELFTEST = 6,  // ovk_selftest_device_timeout: the wait that is meant to run out
     OVK_DEV_TIMEOUT_GRID = 7,      // a block gave up waiting for the other blocks of its own launch
+    OVK_DEV_BAD_POSITION = 8,      // a rotary position read on the device fell outside the tables
+    OVK_DEV_BAD_PAGE = 9,          // a cache position or page number read on the device fell outside the cache
+    OVK_DEV_BAD_SEQUENCE = 10,     // sequence bounds read on the device disagree with the call
 };
 
 struct ovk_ctx {

@@ -38,6 +38,32 @@ class ConvParams(C.Structure):
                 ("pads", C.c_int64 * 4), ("strides", C.c_int64 * 2), ("dilations", C.c_int64 * 2)]
 
 
+class Heads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("heads", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("head_dim", C.c_int64), ("rotary_dim", C.c_int64), ("max_position", C.c_int64),
+                ("dtype", C.c_int32), ("table_dtype", C.c_int32), ("positions_dtype", C.c_int32), ("interleaved", C.c_int32),
+                ("axes", C.c_int32), ("sections", C.c_int32 * 4)]
+
+
+class KV4CacheParams(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("k_zero_points", C.c_void_p), ("v_zero_points", C.c_void_p), ("pages", C.c_int64), ("kv_heads", C.c_int64),
+                ("page_size", C.c_int64), ("head_dim", C.c_int64), ("block_size", C.c_int64)]
+
+
+class KV4Batch(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("batch", C.c_int64), ("max_pages", C.c_int64), ("cu_tokens", C.c_void_p),
+                ("lens", C.c_void_p), ("block_table", C.c_void_p)]
+
+
+class PromptParams(C.Structure):
+    _fields_ = [("q_tokens", C.c_int64), ("k_tokens", C.c_int64), ("batch", C.c_int64), ("head_dim", C.c_int64),
+                ("dtype", C.c_int32), ("causal", C.c_int32), ("window", C.c_int64), ("scale", C.c_float)]
+
+
 _lib = None
 
 # name -> (restype, argtypes); every symbol ovk_cuda.h declares
@@ -111,6 +137,13 @@ SIGNATURES = {
                              C.POINTER(_I64), _P, C.POINTER(_I64), C.POINTER(_I64)]),
     "ovk_quantize_linear": (_I32, [_P, _P, _I64, _I64, _I64, _P, _P, _I32, _P]),
     "ovk_dequantize_linear": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "ovk_rotary": (_I32, [_P, C.POINTER(RotaryParams), _I32, C.POINTER(Heads), C.POINTER(Heads), _P, _P, _P]),
+    "ovk_kv4_append": (_I32, [_P, C.POINTER(KV4CacheParams), C.POINTER(KV4Batch), C.POINTER(Heads), C.POINTER(Heads), _I32]),
+    "ovk_attention_kv4": (_I32, [_P, C.POINTER(KV4CacheParams), C.POINTER(KV4Batch), C.POINTER(Heads), C.POINTER(Heads), _I32, _I64,
+                                 C.c_float, _I64, _P, _SZ]),
+    "ovk_attention_kv4_workspace": (_I32, [_P, C.POINTER(KV4CacheParams), _I64, _I64, _I32, C.POINTER(_SZ)]),
+    "ovk_attention_prompt": (_I32, [_P, C.POINTER(PromptParams), C.POINTER(Heads), C.POINTER(Heads), C.POINTER(Heads), _P, _P,
+                                    C.POINTER(Heads)]),
     "ovk_qlinear_global_average_pool": (_I32, [_P, _P, _I32, _I64, _I64, _I64, C.c_float, _I32, C.c_float, _I32, _P]),
 }
 
@@ -166,6 +199,8 @@ class Context:
             raise OvkError(rc, lib().ovk_last_error(None).decode())
         self.h = h
         self.device = device
+        self._stream = lib().ovk_stream(h)
+        self._kv4_workspace = {}  # (cache shape, query heads, most new tokens, type) -> bytes
 
     def check(self, rc: int):
         if rc:
@@ -526,6 +561,157 @@ class Context:
         self.check(lib().ovk_argmax(self.h, _ptr(x), _dtype_code(x), outer, c, inner, _ptr(out)))
         return out
 
+    # -------------------------------------------- the attention of a decoder layer
+    def _activation(self, what, t, tokens=None, heads=None, head_dim=None, dtype=None):
+        """A [tokens, heads, head_dim] tensor whose heads are contiguous, as the C struct; a slice of a wider one will do."""
+        import torch
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.device.index == self.device):
+            raise OvkError(INVALID_ARGUMENT, f"{what}: a tensor on cuda:{self.device} is needed")
+        if t.dim() != 3 or t.dtype not in (torch.float32, torch.float16):
+            raise OvkError(INVALID_ARGUMENT, f"{what}: [tokens, heads, head_dim] of float32 or float16 is needed, not "
+                                             f"{tuple(t.shape)} of {t.dtype}")
+        n, h, d = t.shape
+        if (tokens is not None and n != tokens) or (heads is not None and h != heads) or (head_dim is not None and d != head_dim) \
+                or (dtype is not None and t.dtype != dtype):
+            raise OvkError(INVALID_ARGUMENT, f"{what}: {tuple(t.shape)} of {t.dtype} does not fit [{tokens or n}, {heads or h}, "
+                                             f"{head_dim or d}] of {dtype or t.dtype}")
+        st, sh, sd = t.stride()
+        if sd != 1 and d != 1:
+            raise OvkError(INVALID_ARGUMENT, f"{what}: the elements of a head must be contiguous (strides {t.stride()})")
+        return Heads(t.data_ptr(), h, st, sh)
+
+    def _indices(self, what, t, shape, dtypes):
+        import torch
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.device.index == self.device and t.is_contiguous()) \
+                or t.dtype not in dtypes or tuple(t.shape) != tuple(shape):
+            raise OvkError(INVALID_ARGUMENT, f"{what}: a contiguous {list(shape)} tensor of {' or '.join(str(d) for d in dtypes)} on "
+                                             f"cuda:{self.device} is needed")
+        return t.data_ptr()
+
+    def _on_stream(self, used, make):
+        """Runs `make` (allocations) for work on this context's stream.  Where that is not torch's current stream the new
+        tensors come from its pool, and those the call reads are kept until it has passed them."""
+        import torch
+        if (torch.cuda.current_stream(self.device).cuda_stream or 1) == self._stream:
+            return make()
+        stream = torch.cuda.ExternalStream(self._stream, device=torch.device("cuda", self.device))
+        for t in used:
+            if t is not None:
+                t.record_stream(stream)
+        with torch.cuda.stream(stream):
+            return make()
+
+    def rotary(self, q, cos, sin, positions, k=None, sections=None, interleaved=False, out=None, k_out=None):
+        """Rotary positions of q (and k) [tokens, heads, head_dim]: cos and sin are [positions, rotary_dim / 2] tables,
+        positions [tokens] or [axes, tokens], sections the pairs of each axis.  Returns q (and k) turned; out may be q."""
+        import torch
+        n, _, d = q.shape if q.dim() == 3 else (0, 0, 0)
+        x = (Heads * 2)(self._activation("Rotary: q", q))
+        if k is not None:
+            x[1] = self._activation("Rotary: k", k, n, None, d, q.dtype)
+        pairs = cos.shape[-1]
+        axes = 1 if positions.dim() == 1 else positions.shape[0]
+        at = self._indices("Rotary: positions", positions, (n,) if positions.dim() == 1 else (axes, n), (torch.int64, torch.int32))
+        tables = [self._indices(f"Rotary: {c}", t, (cos.shape[0], pairs), (torch.float32, torch.float16)) for c, t in
+                  (("cos", cos), ("sin", sin))]
+        if cos.dtype != sin.dtype:
+            raise OvkError(INVALID_ARGUMENT, "Rotary: tables of two types")
+        sections = [pairs] if sections is None else [int(v) for v in sections]
+        if len(sections) != axes or axes > 4:
+            raise OvkError(INVALID_ARGUMENT, f"Rotary: {len(sections)} sections for {axes} axes (1 to 4)")
+        if out is None or (k is not None and k_out is None):
+            def make():
+                return (torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out,
+                        torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None and k_out is None else k_out)
+            out, k_out = self._on_stream((q, k, cos, sin, positions, out, k_out), make)
+        else:
+            self._on_stream((q, k, cos, sin, positions, out, k_out), lambda: None)
+        y = (Heads * 2)(self._activation("Rotary: out", out, n, q.shape[1], d, q.dtype))
+        if k is not None:
+            y[1] = self._activation("Rotary: k_out", k_out, n, k.shape[1], d, q.dtype)
+        p = RotaryParams(n, d, 2 * pairs, cos.shape[0], FLOAT if q.dtype == torch.float32 else FLOAT16,
+                         FLOAT if cos.dtype == torch.float32 else FLOAT16, INT64 if positions.dtype == torch.int64 else INT32,
+                         int(interleaved), axes, (C.c_int32 * 4)(*sections))
+        self.check(lib().ovk_rotary(self.h, p, 1 if k is None else 2, x, y, at, *tables))
+        return out if k is None else (out, k_out)
+
+    def kv4_cache(self, pages, kv_heads, page_size, head_dim, block_size=32, zero_points=True):
+        """An empty paged 4-bit cache; with pages = batch and a block table of one column, a [batch, kv_heads, capacity] one."""
+        import torch
+        blocks = head_dim // block_size if block_size else 0
+        device = torch.device("cuda", self.device)
+        code = lambda: torch.zeros((pages, kv_heads, page_size, head_dim // 2), dtype=torch.uint8, device=device)  # noqa: E731
+        scale = lambda: torch.zeros((pages, kv_heads, page_size, blocks), dtype=torch.float16, device=device)  # noqa: E731
+        zero = lambda: torch.zeros((pages, kv_heads, page_size, (blocks + 1) // 2), dtype=torch.uint8,  # noqa: E731
+                                   device=device) if zero_points else None
+        return self._on_stream((), lambda: KV4Cache(code(), code(), scale(), scale(), zero(), zero()))
+
+    def _kv4_batch(self, what, cache, tokens, block_table, cu_tokens, lens):
+        import torch
+        if cache.k.device.index != self.device:
+            raise OvkError(INVALID_ARGUMENT, f"{what}: the cache is not on cuda:{self.device}")
+        batch = lens.shape[0] if lens.dim() == 1 else -1
+        i32 = (torch.int32,)
+        pages = block_table.shape[1] if block_table.dim() == 2 else -1
+        return KV4Batch(tokens, batch, pages, self._indices(f"{what}: cu_tokens", cu_tokens, (batch + 1,), i32),
+                        self._indices(f"{what}: lens", lens, (batch,), i32),
+                        self._indices(f"{what}: block_table", block_table, (batch, pages), i32))
+
+    def kv4_append(self, cache: "KV4Cache", k, v, block_table, cu_tokens, lens):
+        """Rounds the new tokens' keys and values [tokens, kv_heads, head_dim] to 4 bits and writes them: sequence b brings rows
+        cu_tokens[b] .. cu_tokens[b + 1] - 1, its last lens[b] .. positions; block_table is [batch, max_pages]."""
+        hk = self._activation("KV4Append: k", k, None, cache.kv_heads, cache.head_dim)
+        hv = self._activation("KV4Append: v", v, k.shape[0], cache.kv_heads, cache.head_dim, k.dtype)
+        b = self._kv4_batch("KV4Append", cache, k.shape[0], block_table, cu_tokens, lens)
+        self._on_stream((k, v, block_table, cu_tokens, lens, *cache.tensors), lambda: None)
+        self.check(lib().ovk_kv4_append(self.h, cache.params, b, hk, hv, _dtype_code(k)))
+
+    def attention_kv4(self, cache: "KV4Cache", q, block_table, cu_tokens, lens, max_tokens=1, scale=None, window=0, out=None):
+        """Causal attention of the new tokens q [tokens, q_heads, head_dim] over the cache, which holds their own rows already.
+        max_tokens: the most new tokens a sequence brings; scale: 1 / sqrt(head_dim) unless given; window: positions a
+        token reads, its own included (0: all before it)."""
+        import torch
+        hq = self._activation("AttentionKV4: q", q, None, None, cache.head_dim)
+        b = self._kv4_batch("AttentionKV4", cache, q.shape[0], block_table, cu_tokens, lens)
+        code = _dtype_code(q)
+        key = (cache.shape, q.shape[1], max_tokens, code)
+        need = self._kv4_workspace.get(key)
+        if need is None:
+            n = _SZ()
+            self.check(lib().ovk_attention_kv4_workspace(self.h, cache.params, q.shape[1], max_tokens, code, C.byref(n)))
+            need = self._kv4_workspace[key] = n.value
+
+        def make():
+            return (torch.empty(need, dtype=torch.uint8, device=q.device),
+                    torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out)
+        space, out = self._on_stream((q, block_table, cu_tokens, lens, out, *cache.tensors), make)
+        ho = self._activation("AttentionKV4: out", out, *q.shape, q.dtype)
+        self.check(lib().ovk_attention_kv4(self.h, cache.params, b, hq, ho, code, max_tokens,
+                                           cache.head_dim ** -0.5 if scale is None else scale, window, space.data_ptr(), need))
+        return out
+
+    def attention_prompt(self, q, k, v, cu_q, max_q=None, cu_k=None, scale=None, causal=True, window=0, out=None):
+        """Attention within packed sequences: q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim], cu_q the
+        sequences' first rows.  With cu_k the keys have rows of their own and the queries are the last tokens of the keys'
+        sequence.  max_q (the longest sequence's queries) is accepted for callers that have it; the lengths are read on
+        the device."""
+        import torch
+        hq = self._activation("AttentionPrompt: q", q)
+        hk = self._activation("AttentionPrompt: k", k, None, None, q.shape[2], q.dtype)
+        hv = self._activation("AttentionPrompt: v", v, k.shape[0], k.shape[1], q.shape[2], q.dtype)
+        batch = cu_q.shape[0] - 1
+        pq = self._indices("AttentionPrompt: cu_q", cu_q, (batch + 1,), (torch.int32,))
+        if batch < 0:
+            raise OvkError(INVALID_ARGUMENT, "AttentionPrompt: cu_q is empty")
+        pk = pq if cu_k is None or cu_k is cu_q else self._indices("AttentionPrompt: cu_k", cu_k, (batch + 1,), (torch.int32,))
+        used = (q, k, v, cu_q, cu_k, out)
+        out = self._on_stream(used, lambda: torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out)
+        ho = self._activation("AttentionPrompt: out", out, *q.shape, q.dtype)
+        p = PromptParams(q.shape[0], k.shape[0], batch, q.shape[2], _dtype_code(q), int(causal), window,
+                         q.shape[2] ** -0.5 if scale is None else scale)
+        self.check(lib().ovk_attention_prompt(self.h, p, hq, hk, hv, pq, pk, ho))
+        return out
+
     # ------------------------------------ the QOperator chain around QLinearConv
     def qlinear_add(self, a, a_scale, a_zp, b, b_scale, b_zp, c_scale, c_zp):
         """interp::qlinear_add (interp.rs:4878); a and b are u8 or i8 tensors that broadcast."""
@@ -590,6 +776,35 @@ class Context:
                                                          math.prod(x.shape[2:]), float(x_scale), int(x_zp),
                                                          float(y_scale), int(y_zp), _ptr(out)))
         return out
+
+
+class KV4Cache:
+    """A paged key / value cache in 4 bits: codes [pages, kv_heads, page_size, head_dim / 2], fp16 scales [..., blocks] and zero
+    points [..., ceil(blocks / 2)] (None: implicit 8), rows as ovk_gather_block_quantized reads them."""
+
+    def __init__(self, k, v, k_scales, v_scales, k_zero_points=None, v_zero_points=None):
+        import torch
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.k_zero_points, self.v_zero_points = k_zero_points, v_zero_points
+        self.tensors = tuple(t for t in (k, v, k_scales, v_scales, k_zero_points, v_zero_points) if t is not None)
+        if (k_zero_points is None) != (v_zero_points is None) or k.dim() != 4 or k_scales.dim() != 4 or k_scales.shape[3] < 1:
+            raise OvkError(INVALID_ARGUMENT, "KV4Cache: four-dimensional tensors, with zero points for both or for neither")
+        pages, heads, size, half = k.shape
+        blocks = k_scales.shape[3]
+        for t, last, dtype in ((k, half, torch.uint8), (v, half, torch.uint8), (k_scales, blocks, torch.float16),
+                               (v_scales, blocks, torch.float16), (k_zero_points, (blocks + 1) // 2, torch.uint8),
+                               (v_zero_points, (blocks + 1) // 2, torch.uint8)):
+            if t is not None and (tuple(t.shape) != (pages, heads, size, last) or t.dtype != dtype or not t.is_cuda
+                                  or t.device != k.device or not t.is_contiguous()):
+                raise OvkError(INVALID_ARGUMENT, f"KV4Cache: contiguous {[pages, heads, size, last]} of {dtype} on one GPU is needed, "
+                                                 f"not {tuple(t.shape)} of {t.dtype} on {t.device}")
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, 2 * half
+        if self.head_dim % blocks:
+            raise OvkError(INVALID_ARGUMENT, f"KV4Cache: {blocks} scales for {self.head_dim} elements")
+        self.block_size = self.head_dim // blocks
+        self.shape = (pages, heads, size, self.head_dim, self.block_size)
+        self.params = KV4CacheParams(*[None if t is None else t.data_ptr() for t in (k, v, k_scales, v_scales, k_zero_points, v_zero_points)],
+                                     pages, heads, size, self.head_dim, self.block_size)
 
 
 class NBitsWeight:
