@@ -91,6 +91,12 @@ __device__ __forceinline__ float exp2_approx(float x)
     return y;
 }
 
+__device__ __forceinline__ uint32_t pack_halves(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 // N consecutive elements of 4 or 2 bytes, in 16-byte accesses where VEC says that the address allows it
 template <typename T, int N, bool VEC> __device__ __forceinline__ void load_row(const T *p, float (&v)[N])
 {
@@ -130,11 +136,8 @@ template <typename T, int N, bool VEC> __device__ __forceinline__ void store_row
                 w = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
                                __float_as_uint(v[4 * i + 3]));
             } else {
-                __half2 h[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    h[e] = __floats2half2_rn(v[8 * i + 2 * e], v[8 * i + 2 * e + 1]);
-                w = *reinterpret_cast<uint4 *>(h);
+                w = make_uint4(pack_halves(v[8 * i], v[8 * i + 1]), pack_halves(v[8 * i + 2], v[8 * i + 3]),
+                               pack_halves(v[8 * i + 4], v[8 * i + 5]), pack_halves(v[8 * i + 6], v[8 * i + 7]));
             }
             reinterpret_cast<uint4 *>(p)[i] = w;
         }

@@ -120,11 +120,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t a)
 __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half(uint16_t(w))); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half(uint16_t(w >> 16))); }
-__device__ __forceinline__ uint32_t pack_halves(float lo, float hi)
-{
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 // Two codes as halves: the nibbles at bits 0-3 and 16-19 of `w` (SECOND: 4-7 and 20-23).
 template <bool SUBNORMAL, bool SECOND> __device__ __forceinline__ uint32_t codes_at(uint32_t w)
 {

@@ -259,6 +259,10 @@ extern "C" int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p
         return p->head_dim <= 64    ? launch_simt<float, 64>(ctx, a, tiles)
                : p->head_dim <= 128 ? launch_simt<float, 128>(ctx, a, tiles)
                                     : launch_simt<float, 256>(ctx, a, tiles);
+    bool taken = false;
+    rc = ovk_prompt_tc(ctx, a, &taken);
+    if (taken || rc != OVK_OK)
+        return rc;
     return p->head_dim <= 64    ? launch_simt<__half, 64>(ctx, a, tiles)
            : p->head_dim <= 128 ? launch_simt<__half, 128>(ctx, a, tiles)
                                 : launch_simt<__half, 256>(ctx, a, tiles);

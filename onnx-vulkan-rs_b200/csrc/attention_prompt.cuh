@@ -87,3 +87,6 @@ __device__ __forceinline__ KeyRange key_range(const PromptArgs &a, const PromptT
     return r;
 }
 #endif
+
+// f16 on the tensor cores; *taken says whether the call's layout is one it takes
+int32_t ovk_prompt_tc(ovk_ctx *ctx, const PromptArgs &a, bool *taken);

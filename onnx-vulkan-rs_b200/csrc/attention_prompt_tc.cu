@@ -1,0 +1,587 @@
+// f16 attention over packed prompts on the 5th-generation tensor cores.
+//
+//   S = Q K^T (128 query rows x 128 keys, f32 in tensor memory),
+//   P = 2^(scale' S - m) (f16, written back over S),  O = O + P V (f32 in tensor memory),
+//
+// m a per-row reference that follows the running maximum, out = O / sum of P.
+// The two products are 4 head_dim operations per score, the exponential one of 16
+// a cycle and SM: at head_dim 128 both pipes need the same 1024 cycles a tile, so
+// the point of the layout is that neither waits for the other.
+//
+//   warp 0 of the control group    TMA: Q once, then K and V tiles into one ring in
+//                                  the order the products use them
+//   warp 1                         issues every tcgen05.mma from one thread
+//   warps 2, 3                     guard V tiles that some row of the block does
+//                                  not read entirely (below)
+//   softmax groups of four warps   a thread owns a row: tcgen05.ld, maximum, exp2,
+//                                  tcgen05.st, and at the end its row of the result
+//
+// Up to 128 elements a head two independent query tiles share each K and V tile
+// (two heads of a group, or neighbouring rows where the group is odd): while one
+// tile's softmax runs, the tensor core works for the other.  256-wide heads fill
+// tensor memory with one tile's O, so there one tile has two S buffers, and the
+// next scores are computed before the last weights are used.
+//
+// The reference m moves only when a row's maximum passes it by 2^8 (P is then at
+// most 256, sums are f32), so O is rarely rescaled; the softmax group does it
+// itself, between the products that write O.
+//
+// Masked weights are exactly 0, and 0 times an infinity is NaN: in tiles that are
+// not read whole, the guards zero the V rows behind the sequence's end and every
+// V element that is not finite, and note its column.  A row adds such elements of
+// the keys that it does read when it stores its result.
+#include "attention_prompt.cuh"
+#include "umma.cuh"
+
+namespace {
+
+constexpr int BM = 128, BN = 128;
+
+template <int DP_> struct Tc {
+    static constexpr int DP = DP_;                       // head_dim rounded up; TMA fills the rest with zeros
+    static constexpr int NS = DP == 256 ? 1 : 2;         // query tiles of a block
+    static constexpr int SB = DP == 256 ? 2 : 1;         // S buffers of a tile
+    static constexpr int CH = DP == 256 ? 2 : 1;         // ring stages of a K or V tile
+    static constexpr int ATOMS = DP / 64;                // 128-byte columns of a row
+    static constexpr int Q_BYTES = BM * DP * 2;
+    static constexpr int STAGE = BN * DP * 2 / CH;
+    static constexpr int STAGES = 5;
+    static constexpr int THREADS = NS * 128 + 128;
+    static constexpr int SMEM = NS * Q_BYTES + STAGES * STAGE + 1024;
+    static constexpr int O_COL = 256;                    // S of the two tiles (or buffers) at 0 and 128
+};
+
+struct TcParams {
+    PromptArgs a;
+    int pairs;     // blocks along the heads
+    int by_heads;  // the two query tiles are two heads of a group; else neighbouring rows
+    int window, vec_out;
+};
+
+struct Shared {
+    uint64_t q_full[2], full[5], empty[5], raw[5], s_full[2][2], p_full[2], pv_done[2], drain;
+    uint32_t tmem;
+    int dead;
+    uint32_t odd[8];  // columns in which a V element that is not finite was zeroed
+    PromptTile tile;
+};
+
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *dead, int *status, int code)
+{
+    for (uint32_t i = 0; i < umma::WAIT_LIMIT; i++) {
+        if (umma::mbar_try_wait(bar, parity))
+            return true;
+        if ((i & 255) == 255 && *dead)
+            return false;
+    }
+    *dead = 1;
+    atomicExch(status, code);
+    return false;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(Tc<DP>::THREADS, 1)
+attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                           const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TcParams p)
+{
+    using C = Tc<DP>;
+    constexpr int NS = C::NS, SB = C::SB, CH = C::CH;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Shared sh;
+    const uint32_t smem_base = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *const smem = smem_raw + (smem_base - umma::smem_u32(smem_raw));
+    uint8_t *const ring = smem + NS * C::Q_BYTES;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = tid >> 7;
+    volatile int *const dead = &sh.dead;
+    int *const status = p.a.status;
+    const PromptArgs &a = p.a;
+
+    const int index = blockIdx.x / p.pairs, pair = blockIdx.x - index * p.pairs;
+    if (warp == 0) {
+        if (NS == 2 && !p.by_heads)
+            find_prompt_tile<2 * BM>(a, index, sh.tile);
+        else
+            find_prompt_tile<BM>(a, index, sh.tile);
+    }
+    if (tid == 32) {
+        sh.dead = 0;
+        for (int i = 0; i < 8; i++)
+            sh.odd[i] = 0;
+        for (int i = 0; i < 2; i++) {
+            umma::mbar_init(&sh.q_full[i], 1);
+            umma::mbar_init(&sh.s_full[i][0], 1);
+            umma::mbar_init(&sh.s_full[i][1], 1);
+            umma::mbar_init(&sh.p_full[i], 4);
+            umma::mbar_init(&sh.pv_done[i], 1);
+        }
+        for (int i = 0; i < C::STAGES; i++) {
+            umma::mbar_init(&sh.full[i], 1);
+            umma::mbar_init(&sh.empty[i], 1);
+            umma::mbar_init(&sh.raw[i], 1);
+        }
+        umma::mbar_init(&sh.drain, 1);
+        umma::fence_barrier_init();
+    }
+    __syncthreads();
+    const PromptTile w = sh.tile;
+    if (w.b < 0)
+        return;  // the batch has fewer tiles; nothing is allocated or in flight yet
+    // a block's query tiles: head and first row of each, and how many rows are left for it
+    const int head0 = NS == 2 && p.by_heads ? 2 * pair : pair;
+    const int kv_head = head0 / a.group;
+    const bool rows_split = NS == 2 && !p.by_heads;
+    const int rows_all = min(rows_split ? 2 * BM : BM, w.n_q - w.row0);
+    const int streams = NS == 1 || (rows_split && rows_all <= BM) ? 1 : 2;
+    const int pos0 = w.n_k - w.n_q + w.row0;  // position of the block's first row
+    const int key_begin = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+    const int key_end = a.causal ? min(w.n_k, pos0 + rows_all) : w.n_k;
+    const int tiles = key_end > key_begin ? (key_end - key_begin + BN - 1) / BN : 0;
+    // whether some of the rows first .. last do not read the whole of tile i
+    auto partial = [&](int i, int first, int last) {
+        const int j0 = key_begin + i * BN;
+        return j0 + BN > key_end || (a.causal && j0 + BN - 1 > first) || (p.window > 0 && j0 <= last - p.window);
+    };
+    const int pos_last = pos0 + rows_all - 1;
+
+    if (group == NS) {
+        if constexpr (NS == 2)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        const int role = warp - NS * 4;
+        if (role == 1) {
+            umma::tmem_alloc(&sh.tmem, 512);
+            umma::tmem_relinquish();
+        }
+        umma::tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(C::THREADS) : "memory");
+        umma::tc_fence_after();
+        const uint32_t tmem = sh.tmem;
+        if (role == 0) {
+            // ------------------------------------------------------------ loads
+            if (lane == 0 && tiles > 0) {
+                for (int s = 0; s < streams; s++) {
+                    umma::mbar_expect_tx(&sh.q_full[s], C::Q_BYTES);
+                    for (int x = 0; x < C::ATOMS; x++)
+                        umma::tma_load_3d(smem + s * C::Q_BYTES + x * BM * 128, &tm_q, &sh.q_full[s], 64 * x,
+                                          rows_split ? head0 : head0 + s, w.first_q + w.row0 + (rows_split ? s * BM : 0));
+                }
+                int stage = 0, issued = 0;
+                uint32_t phase = 0;
+                uint32_t in_raw = 0, raw_phase = 0;  // a bit per stage: its last copy is counted at `raw`; uses of `raw` so far
+                bool ok = true;
+                auto load = [&](bool value, int tile) {
+                    for (int c = 0; c < CH && ok; c++) {
+                        ok = wait(&sh.empty[stage], phase ^ 1, dead, status, OVK_DEV_TIMEOUT_SLOT);
+                        if (!ok)
+                            return;
+                        uint8_t *dst = ring + stage * C::STAGE;
+                        // a V tile that the guards look through first is theirs to pass on
+                        uint64_t *const bar = value && partial(tile, pos0, pos_last) ? &sh.raw[stage] : &sh.full[stage];
+                        umma::mbar_expect_tx(bar, C::STAGE);
+                        const int row = w.first_k + key_begin + tile * BN;
+                        if (CH == 1 || !value) {  // whole rows, or (K) half of the columns of each
+                            for (int x = 0; x < C::ATOMS / CH; x++)
+                                umma::tma_load_3d(dst + x * BN * 128, value ? &tm_v : &tm_k, bar,
+                                                  64 * (c * (C::ATOMS / CH) + x), kv_head, row);
+                        } else {  // V: half of the keys; its box has half the rows
+                            for (int x = 0; x < C::ATOMS; x++)
+                                umma::tma_load_3d(dst + x * (BN / CH) * 128, &tm_v, bar, 64 * x, kv_head, row + c * (BN / CH));
+                        }
+                        issued++;
+                        in_raw = bar == &sh.raw[stage] ? in_raw | (1u << stage) : in_raw & ~(1u << stage);
+                        raw_phase ^= bar == &sh.raw[stage] ? 1u << stage : 0u;
+                        if (++stage == C::STAGES)
+                            stage = 0, phase ^= 1;
+                    }
+                };
+                for (int j = 0; j < SB && j < tiles; j++)
+                    load(false, j);
+                for (int i = 0; i < tiles && ok; i++) {
+                    load(true, i);
+                    if (i + SB < tiles)
+                        load(false, i + SB);
+                }
+                if (!ok) {  // copies in flight end before the block does
+                    for (int k = max(0, issued - C::STAGES); k < issued; k++)
+                        if ((in_raw >> (k % C::STAGES)) & 1)
+                            umma::mbar_wait(&sh.raw[k % C::STAGES], ((raw_phase >> (k % C::STAGES)) & 1) ^ 1);
+                        else
+                            umma::mbar_wait(&sh.full[k % C::STAGES], (k / C::STAGES) & 1);
+                    for (int s = 0; s < streams; s++)
+                        umma::mbar_wait(&sh.q_full[s], 0);
+                }
+            }
+        } else if (role == 1) {
+            // --------------------------------------------------------- products
+            if (lane == 0 && tiles > 0) {
+                constexpr uint32_t k_hi = ((1024u >> 4) & 0x3fffu) | (1u << 14) | (umma::LAYOUT_SW128 << 29);
+                constexpr uint32_t qk_desc = umma::instr_desc(1, 0, 0, BM, BN);
+                constexpr uint32_t pv_desc = umma::instr_desc(1, 0, 0, BM, DP) | (1u << 16);  // V: keys along the rows
+                constexpr uint32_t v_lbo = DP == 64 ? 1u : uint32_t(BN / CH) * 128u >> 4;
+                const uint32_t q_lo = ((umma::smem_u32(smem) >> 4) & 0x3fffu) | (1u << 16);
+                const uint32_t ring_addr = umma::smem_u32(ring) >> 4;
+                bool ok = true;
+                auto arrived = [&](int n) {  // waits for the n-th chunk of the ring
+                    ok = ok && wait(&sh.full[n % C::STAGES], (n / C::STAGES) & 1, dead, status, OVK_DEV_TIMEOUT_TMA);
+                };
+                // position in the ring of tile i's first K and V chunk
+                auto k_at = [&](int i) { return CH * (i < SB ? i : 2 * i - SB + 1); };
+                auto v_at = [&](int i) { return CH * (min(SB, tiles) + i + min(i, max(0, tiles - SB))); };
+                auto qk = [&](int s, int i, bool release) {
+                    const uint32_t d = tmem + (SB == 2 ? (i & 1) : s) * 128;
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        const int n = k_at(i) + c;
+                        const uint32_t b_lo = ((ring_addr + uint32_t(n % C::STAGES) * (C::STAGE >> 4)) & 0x3fffu) | (1u << 16);
+                        const uint32_t a_lo = q_lo + s * (C::Q_BYTES >> 4) + c * (C::ATOMS / CH) * (BM * 128 >> 4);
+                        if (c > 0)
+                            arrived(n);
+                        if (!ok)
+                            return;
+#pragma unroll
+                        for (int k = 0; k < DP / CH / 16; k++) {
+                            const uint32_t off = (k >> 2) * (BM * 128 >> 4) + (k & 3) * 2;
+                            umma::mma_f16_lohi(d, a_lo + off, k_hi, b_lo + off, k_hi, qk_desc, c > 0 || k > 0);
+                        }
+                        if (release)
+                            umma::mma_commit(&sh.empty[n % C::STAGES]);
+                    }
+                    umma::mma_commit(&sh.s_full[s][SB == 2 ? (i & 1) : 0]);
+                };
+                auto pv = [&](int s, int i, bool wait_v, bool release) {
+                    const uint32_t d = tmem + C::O_COL + s * DP, pt = tmem + (SB == 2 ? (i & 1) : s) * 128;
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        const int n = v_at(i) + c, stage = n % C::STAGES;
+                        if (wait_v)
+                            arrived(n);
+                        if (!ok)
+                            return;
+                        umma::tc_fence_after();
+                        const uint32_t b_lo = ((ring_addr + uint32_t(stage) * (C::STAGE >> 4)) & 0x3fffu) | (v_lbo << 16);
+#pragma unroll
+                        for (int k = 0; k < BN / CH / 16; k++)
+                            umma::mma_f16_ts(d, pt + c * (BN / CH / 2) + 8 * k, b_lo + k * (2048 >> 4), k_hi, pv_desc, i > 0 || c > 0 || k > 0);
+                        if (release)
+                            umma::mma_commit(&sh.empty[stage]);
+                    }
+                    umma::mma_commit(&sh.pv_done[s]);
+                };
+                for (int j = 0; j < SB && j < tiles && ok; j++) {
+                    arrived(k_at(j));
+                    for (int s = 0; s < streams && ok; s++) {
+                        if (j == 0)
+                            ok = ok && wait(&sh.q_full[s], 0, dead, status, OVK_DEV_TIMEOUT_TMA);
+                        if (ok)
+                            qk(s, j, s == streams - 1);
+                    }
+                }
+                for (int i = 0; i < tiles && ok; i++) {
+                    for (int s = 0; s < streams && ok; s++) {
+                        ok = wait(&sh.p_full[SB == 2 ? i & 1 : s], SB == 2 ? (i >> 1) & 1 : i & 1, dead, status, OVK_DEV_TIMEOUT_SLOT);
+                        if (!ok)
+                            break;
+                        umma::tc_fence_after();
+                        pv(s, i, s == 0, s == streams - 1);
+                        if (ok && i + SB < tiles) {
+                            if (s == 0)
+                                arrived(k_at(i + SB));
+                            if (ok)
+                                qk(s, i + SB, s == streams - 1);
+                        }
+                    }
+                }
+                if (!ok) {  // products in flight end before tensor memory is freed
+                    umma::mma_commit(&sh.drain);
+                    umma::mbar_wait(&sh.drain, 0);
+                }
+            }
+            __syncwarp();
+        } else if (tiles > 0) {
+            // ------------------------------------------------------------ guards
+            int n = CH * min(SB, tiles);  // place in the ring
+            uint32_t raw_phase = 0;       // a bit per stage
+            bool ok = true;
+            for (int i = 0; i < tiles && ok; i++) {
+                for (int c = 0; c < CH && ok; c++, n++) {
+                    if (!partial(i, pos0, pos_last))
+                        continue;
+                    const int stage = n % C::STAGES;
+                    ok = wait(&sh.raw[stage], (raw_phase >> stage) & 1, dead, status, OVK_DEV_TIMEOUT_TMA);
+                    raw_phase ^= 1u << stage;
+                    constexpr int KEYS = BN / CH, WORDS = KEYS * DP / 8;  // 16-byte words of the chunk
+                    const int left = key_end - (key_begin + i * BN + c * KEYS);  // keys before the end
+                    uint4 *const words = reinterpret_cast<uint4 *>(ring + stage * C::STAGE);
+                    for (int at = (role - 2) * 32 + lane; at < WORDS && ok; at += 64) {
+                        const int row = (at >> 3) % KEYS;
+                        if (row >= left) {
+                            words[at] = make_uint4(0, 0, 0, 0);
+                            continue;
+                        }
+                        const uint4 v = words[at];
+                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+                        uint32_t bad = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            bad |= (u[e] & 0x7c007c00u) + 0x04000400u;  // carries into the sign bit for an exponent of ones
+                        if (bad & 0x80008000u) {
+                            const int atom = at / (KEYS * 8), col = atom * 64 + (((at & 7) ^ (row & 7)) << 3);
+                            uint32_t z[4];
+                            for (int e = 0; e < 4; e++) {
+                                z[e] = u[e];
+                                if ((u[e] & 0x7c00u) == 0x7c00u) {
+                                    z[e] &= 0xffff0000u;
+                                    atomicOr(&sh.odd[(col + 2 * e) >> 5], 1u << ((col + 2 * e) & 31));
+                                }
+                                if ((u[e] & 0x7c000000u) == 0x7c000000u) {
+                                    z[e] &= 0x0000ffffu;
+                                    atomicOr(&sh.odd[(col + 2 * e + 1) >> 5], 1u << ((col + 2 * e + 1) & 31));
+                                }
+                            }
+                            words[at] = make_uint4(z[0], z[1], z[2], z[3]);
+                        }
+                    }
+                    umma::fence_proxy_async();
+                    // both warps, also after a wait that gave up: then both leave
+                    uint32_t all;
+                    asm volatile(
+                        "{\n\t.reg .pred p, q;\n\t"
+                        "setp.ne.b32 p, %1, 0;\n\t"
+                        "bar.red.and.pred q, 2, 64, p;\n\t"
+                        "selp.u32 %0, 1, 0, q;\n\t}"
+                        : "=r"(all)
+                        : "r"(uint32_t(ok))
+                        : "memory");
+                    ok = all != 0;
+                    if (ok && role == 2 && lane == 0)
+                        umma::mbar_arrive(&sh.full[stage]);
+                }
+                n += i + SB < tiles ? CH : 0;
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- softmax
+        if constexpr (NS == 2)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        umma::tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(C::THREADS) : "memory");
+        umma::tc_fence_after();
+        const uint32_t tmem = sh.tmem;
+        const int s = group;
+        if (s < streams) {
+            const int r = tid & 127, rows = min(BM, rows_all - (rows_split ? s * BM : 0));
+            const int first = pos0 + (rows_split ? s * BM : 0), pos = first + r;
+            const uint32_t lanes = uint32_t(warp & 3) << 21;  // 32 lanes a warp
+            const uint32_t t_o = tmem + lanes + C::O_COL + s * DP;
+            const float scale = a.scale_log2e;
+            float m = -1e30f, l = 0.0f;
+            bool ok = true;
+            for (int i = 0; i < tiles; i++) {
+                const int buffer = SB == 2 ? (i & 1) : 0;
+                const uint32_t t_s = tmem + lanes + (SB == 2 ? buffer : s) * 128;
+                ok = wait(&sh.s_full[s][buffer], SB == 2 ? (i >> 1) & 1 : i & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                umma::tc_fence_after();
+                uint32_t x[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    umma::tmem_ld_32x32(t_s + 32 * c, x[c]);
+                umma::tmem_ld_wait();
+                if (partial(i, first, first + rows - 1)) {
+                    const int j0 = key_begin + i * BN;
+                    const int hi = (a.causal ? min(pos, w.n_k - 1) : w.n_k - 1) - j0;
+                    const int lo = p.window > 0 ? pos - p.window + 1 - j0 : 0;
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (32 * c + e > hi || 32 * c + e < lo)
+                                x[c][e] = 0xff800000u;  // -infinity
+                }
+                float most[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    most[c] = __uint_as_float(x[c][0]);
+#pragma unroll
+                    for (int e = 1; e < 32; e++)
+                        most[c] = fmaxf(most[c], __uint_as_float(x[c][e]));
+                }
+                const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * scale;
+                if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                    const float to = fmaxf(m, top), f = exp2_approx(m - to);
+                    m = to;
+                    l *= f;
+                    if (i > 0) {
+                        if constexpr (SB == 2) {  // the product before this one may still be writing O
+                            ok = wait(&sh.pv_done[s], (i - 1) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
+                            if (!__all_sync(0xffffffffu, ok)) {
+                                ok = false;
+                                break;
+                            }
+                            umma::tc_fence_after();
+                        }
+#pragma unroll
+                        for (int c = 0; c < DP / 16; c++) {
+                            uint32_t o[16];
+                            umma::tmem_ld_32x16(t_o + 16 * c, o);
+                            umma::tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            umma::tmem_st_32x16(t_o + 16 * c, o);
+                        }
+                    }
+                }
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t out[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const int at = 64 * c + 2 * e;
+                        const float p0 = exp2_approx(fmaf(__uint_as_float(x[at >> 5][at & 31]), scale, -m));
+                        const float p1 = exp2_approx(fmaf(__uint_as_float(x[at >> 5][(at & 31) + 1]), scale, -m));
+                        sum[(2 * e) & 3] += p0;
+                        sum[(2 * e + 1) & 3] += p1;
+                        out[e] = pack_halves(p0, p1);
+                    }
+                    umma::tmem_st_32x32(t_s + 32 * c, out);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                umma::tmem_st_wait();
+                umma::tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    umma::mbar_arrive(&sh.p_full[SB == 2 ? buffer : s]);
+            }
+            if (ok && tiles > 0) {
+                // the last scores imply that the second to last product into O is done (with two S buffers: the
+                // third to last), and a parity tells only neighbouring phases apart
+                if (SB == 2 && tiles > 1)
+                    ok = wait(&sh.pv_done[s], (tiles - 2) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
+                ok = ok && wait(&sh.pv_done[s], (tiles - 1) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
+                ok = __all_sync(0xffffffffu, ok);
+                umma::tc_fence_after();
+            }
+            if (ok) {
+                const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+                __half *const out = static_cast<__half *>(a.out) +
+                                    int64_t(w.first_q + w.row0 + (rows_split ? s * BM : 0) + r) * a.o_token +
+                                    int64_t(rows_split ? head0 : head0 + s) * a.o_head;
+                bool any_odd = false;
+                for (int i = 0; i < DP / 32; i++)
+                    any_odd |= sh.odd[i] != 0;
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++) {
+                    uint32_t o[32];
+                    if (tiles > 0) {
+                        umma::tmem_ld_32x32(t_o + 32 * c, o);
+                        umma::tmem_ld_wait();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            o[e] = 0;
+                    }
+                    if (r >= rows || 32 * c >= a.head_dim)
+                        continue;
+                    if (any_odd && sh.odd[c]) {
+                        // elements that the guards took out, of the keys that this row reads
+                        for (int i = 0; i < tiles; i++) {
+                            if (!partial(i, pos0, pos_last))
+                                continue;
+                            const int j0 = key_begin + i * BN;
+                            const int from = p.window > 0 ? max(j0, pos - p.window + 1) : j0;
+                            const int to = min(j0 + BN, a.causal ? min(w.n_k, pos + 1) : w.n_k);
+                            for (int j = from; j < to; j++) {
+                                const __half *v = static_cast<const __half *>(a.v) + int64_t(w.first_k + j) * a.v_token +
+                                                  int64_t(kv_head) * a.v_head + 32 * c;
+#pragma unroll
+                                for (int e = 0; e < 32; e++)
+                                    if ((sh.odd[c] >> e) & 1) {
+                                        const float x = __half2float(v[e]);
+                                        if (!(x - x == 0.0f))
+                                            o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                                    }
+                            }
+                        }
+                    }
+                    if (p.vec_out && 32 * c + 32 <= a.head_dim) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int u = 0; u < 4; u++)
+                                h[u] = pack_halves(__uint_as_float(o[e + 2 * u]) * inverse, __uint_as_float(o[e + 2 * u + 1]) * inverse);
+                            *reinterpret_cast<uint4 *>(out + 32 * c + e) = make_uint4(h[0], h[1], h[2], h[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (32 * c + e < a.head_dim)
+                                out[32 * c + e] = __float2half_rn(__uint_as_float(o[e]) * inverse);
+                    }
+                }
+            }
+        }
+    }
+    umma::tc_fence_before();
+    __syncthreads();
+    umma::tc_fence_after();
+    if (warp == NS * 4 + 1)
+        umma::tmem_dealloc(sh.tmem, 512);
+}
+
+bool make_map(CUtensorMap *map, const void *base, int64_t tokens, int64_t heads, int64_t head_dim, int64_t token_stride,
+              int64_t head_stride, uint32_t rows)
+{
+    ovk_encode_tiled_fn fn = ovk_get_encode_tiled();
+    if (!fn)
+        return false;
+    // a stride that no step uses may be anything; the map wants a positive one
+    const int64_t hs = heads > 1 ? head_stride * 2 : 16, ts = tokens > 1 ? token_stride * 2 : 16;
+    cuuint64_t dims[3] = {cuuint64_t(head_dim), cuuint64_t(heads), cuuint64_t(tokens)};
+    cuuint64_t strides[2] = {cuuint64_t(hs), cuuint64_t(ts)};
+    cuuint32_t box[3] = {64, 1, rows}, step[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP> int32_t launch(ovk_ctx *ctx, const PromptArgs &a, bool *taken)
+{
+    using C = Tc<DP>;
+    CUtensorMap q, k, v;
+    const int kv_heads = a.heads / a.group;
+    if (!make_map(&q, a.q, a.q_tokens, a.heads, a.head_dim, a.q_token, a.q_head, BM) ||
+        !make_map(&k, a.k, a.k_tokens, kv_heads, a.head_dim, a.k_token, a.k_head, BN) ||
+        !make_map(&v, a.v, a.k_tokens, kv_heads, a.head_dim, a.v_token, a.v_head, BN / C::CH))
+        return OVK_OK;
+    TcParams p = {};
+    p.a = a;
+    p.by_heads = C::NS == 2 && a.group % 2 == 0;
+    p.pairs = p.by_heads ? a.heads / 2 : a.heads;
+    p.window = a.window >= (int64_t(1) << 30) ? 0 : int(a.window);
+    p.vec_out = aligned_to(a.out, 16) && a.o_token % 8 == 0 && a.o_head % 8 == 0;
+    const int64_t rows = C::NS == 2 && !p.by_heads ? 2 * BM : BM;
+    const int64_t grid = (ceil_div64(a.q_tokens, rows) + a.batch) * p.pairs;
+    if (grid >= (int64_t(1) << 31))
+        return OVK_OK;
+    OVK_CUDA(ctx, cudaFuncSetAttribute(attention_prompt_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attention_prompt_tc_kernel<DP><<<unsigned(grid), C::THREADS, C::SMEM, ctx->stream>>>(q, k, v, p);
+    *taken = true;
+    OVK_LAUNCHED(ctx, "attention_prompt_tc");
+    return OVK_OK;
+}
+
+}  // namespace
+
+// *taken stays false where the layout is not one that a tensor map describes, or the scale is not positive
+// (the maximum is taken before scaling).
+int32_t ovk_prompt_tc(ovk_ctx *ctx, const PromptArgs &a, bool *taken)
+{
+    *taken = false;
+    if (!a.vec || !(a.scale_log2e > 0.0f) || a.k_tokens == 0)
+        return OVK_OK;
+    return a.head_dim <= 64 ? launch<64>(ctx, a, taken) : a.head_dim <= 128 ? launch<128>(ctx, a, taken) : launch<256>(ctx, a, taken);
+}
