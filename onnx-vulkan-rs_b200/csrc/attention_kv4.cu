@@ -5,14 +5,14 @@ namespace {
 
 struct Plan {
     int tiles;    // 8-row column tiles of a CTA: 1 or 2
-    int per_sm;   // CTAs an SM holds
+    int unit;     // tokens that a CTA takes at a time
     size_t slot;  // floats of a partial result
 };
 
 template <int D, int NT, int PARTS> Plan plan_of()
 {
     using S = kv4::Shape<D, NT, PARTS>;
-    return {NT, S::CTAS, size_t(S::SLOT)};
+    return {NT, S::UNIT, size_t(S::SLOT)};
 }
 template <int D> Plan plan_for(int tiles, bool f32)
 {
@@ -56,7 +56,7 @@ extern "C" int32_t ovk_attention_kv4_workspace(ovk_ctx *ctx, const ovk_kv4_cache
     *bytes = 0;
     for (int tiles = 1; tiles <= tiles_for(max_tokens, q_heads / cache->kv_heads); tiles++) {
         const Plan p = plan_for(cache->head_dim, tiles, dtype == OVK_FLOAT);
-        *bytes = std::max(*bytes, bytes_for(p, int64_t(p.per_sm) * ctx->sm_count));
+        *bytes = std::max(*bytes, bytes_for(p, ctx->sm_count));
     }
     return OVK_OK;
 }
@@ -82,6 +82,8 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
     OVK_REQUIRE(ctx, out->heads == q->heads, "%s: %lld query heads, %lld in the output", op, (long long)q->heads, (long long)out->heads);
     OVK_REQUIRE(ctx, batch->tokens == 0 || (ovk_rows_aligned(q, elem) && ovk_rows_aligned(out, elem)),
                 "%s: rows of q and out must be 16-byte aligned", op);
+    OVK_REQUIRE(ctx, batch->tokens * q->heads < (int64_t(1) << 31) - 64, "%s: %lld tokens of %lld heads are too many for one call", op,
+                (long long)batch->tokens, (long long)q->heads);
     OVK_REQUIRE(ctx, window >= 0, "%s: window %lld", op, (long long)window);
     OVK_REQUIRE(ctx, scale == scale && scale - scale == 0.0f, "%s: scale is not finite", op);
     OVK_REQUIRE(ctx, ctx, "%s: null context", op);
@@ -111,9 +113,9 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
     const int tiles = tiles_for(max_tokens, a.group);
     const Plan p = plan_for(cache->head_dim, tiles, dtype == OVK_FLOAT);
     // no more CTAs than the longest sequences the block table has room for would fill
-    const int64_t units = batch->max_pages * cache->page_size / kv4::UNIT + 2;
+    const int64_t units = batch->max_pages * cache->page_size / p.unit + 2;
     const int64_t items = (batch->batch + ceil_div64(batch->tokens * a.group, 8 * tiles)) * cache->kv_heads;
-    const int64_t full = int64_t(p.per_sm) * ctx->sm_count;
+    const int64_t full = ctx->sm_count;
     const int64_t ctas = items >= full || units >= full ? full : std::min(full, units * items);
     if (workspace) {
         OVK_REQUIRE(ctx, aligned_to(workspace, 16) && workspace_bytes >= bytes_for(p, ctas),

@@ -21,21 +21,27 @@
 //    operation more.
 //  - Tokens are the 16 rows of A, query rows the 8 columns of B, so a group of up
 //    to eight query rows costs no more than one.
+//  - ldmatrix brings the words of both operands: K's as they lie, V's transposed,
+//    four codes of two neighbouring tokens in one register.
 //  - K: a chunk of 32 elements has its own accumulator (f16: started at -zero *
 //    sum(q) of the chunk, one product instead of a subtraction per code), then
 //    scaled by its f32 scale: codes and queries enter the product exactly.
-//  - V: codes minus zero (exact) times p * s rounded to fp16.
+//  - V: codes minus zero (exact, so that a value of 0 adds nothing: the zeros as a
+//    product of their own left 2^-17 of them behind) times p * s rounded to fp16.
 //    f32 callers get q and p * s as two fp16 parts, 22 bits.
 //  - The running maximum moves only when a score passes it by 6 (p by 2^6) or a V
 //    scale its own largest by 2^3: p * s starts at 2^6 to 2^7, so it stays below
 //    2^16 and is a normal fp16 number down to 2^-20 of the largest, and a step
 //    needs one vote, not a reduction.
 //
-// Every CTA takes an equal run of 64-token units of the whole batch (lengths are
-// read on the device), four warps of it alternate 16-token steps, each with its
-// own cp.async ring.  A run that begins or ends inside a sequence leaves a partial
-// result; a second kernel joins those in CTA order, so results do not depend on
-// timing.
+// One CTA per SM takes an equal run of units - 16 tokens for each of its consumer
+// warps - of the whole batch (lengths are read on the device).  Four producer
+// warps bring units into a ring with 16-byte copies, row by row, so that a page may
+// have any size, and go on with the next sequence while the consumers finish one.
+// (Tensor and bulk copies, six to a page of 16 tokens, were issued too slowly: 70
+// instead of 37 us for 48 contexts of 4000.)  A run that begins or ends inside a
+// sequence leaves a partial result; a second kernel joins those in CTA order, so
+// results do not depend on timing.
 #pragma once
 
 #include <type_traits>
@@ -62,39 +68,56 @@ struct Kv4Args {
 
 namespace kv4 {
 
-constexpr int WARPS = 4, STEP = 16, UNIT = WARPS * STEP;
+constexpr int STEP = 16;
 constexpr float NONE = -1e30f;  // the maximum of a row that has seen nothing (in powers of two)
 
 template <int D_, int NT_, int PARTS_> struct Shape {
     static constexpr int D = D_, NT = NT_, PARTS = PARTS_;
     static constexpr int NCH = D / 32, ROWS = 8 * NT, ROW_BYTES = D / 2, CPR = D / 32;
-    static constexpr int STAGES = (D == 256 && NT == 1) ? 3 : 4;
-    static constexpr int CODES = STEP * ROW_BYTES;        // of K or of V, one stage
-    static constexpr int RAW = 32 * (16 + 4 + 4);         // scales, zero points, row numbers of a stage
-    static constexpr int STAGE = 2 * CODES + RAW;
-    static constexpr int SZ = 2 * STEP * NCH * 4;         // {scale, zero} per token and chunk, K and V
-    static constexpr int WARP_BYTES = STAGES * STAGE + SZ;
+    // consumer warps, and the registers each thread of theirs and of the producer's group gets; 256-wide heads with
+    // two tiles of rows hold 128 accumulators a thread
+    static constexpr int WARPS = D == 256 && NT == 2 ? 8 : 12;
+    static constexpr int REGS = WARPS == 8 ? 208 : 144, PRODUCER_REGS = WARPS == 8 ? 88 : 80;
+    static constexpr int THREADS = WARPS * 32 + 128, UNIT = WARPS * STEP;
+    static constexpr int STAGES = D == 256 ? 2 : 4;
+    static constexpr int CODES = UNIT * ROW_BYTES;        // of K or of V, one stage
+    static constexpr int SCALES = UNIT * 16, ZEROS = UNIT * 4;
+    static constexpr int PRESENT = 2 * CODES + 2 * (SCALES + ZEROS) + UNIT * 4;  // behind scales, zero points and row numbers
+    static constexpr int STAGE = (PRESENT + WARPS * 2 + 1023) / 1024 * 1024;     // the copies' swizzle counts from such a boundary
+    // of a warp: {scale, zero} of K per token and chunk, scale of V, zeros of V per pair of tokens and chunk
+    static constexpr int K_SZ = STEP * NCH * 8, V_S = STEP * NCH * 4, V_Z = STEP / 2 * NCH * 4, SZ = K_SZ + V_S + V_Z;
     static constexpr int QF = PARTS * NT * NCH * 512;     // query fragments
-    static constexpr int MERGE = WARPS * ROWS * (D + 4) * 4;
-    static constexpr int RING = WARPS * WARP_BYTES > MERGE ? WARPS * WARP_BYTES : MERGE;
-    static constexpr int SMEM = RING + QF + ROWS * (NCH + 1) * 4 + WARPS * ROWS * 8 + 64;
+    static constexpr int SLOTS = D == 256 && NT == 1 ? WARPS / 4 : WARPS / 2;    // warps that add their sums at a time
+    static constexpr int MERGE = SLOTS * ROWS * (D + 4) * 4;
+    static constexpr int RING = STAGES * STAGE;
+    static constexpr int SMEM = 1024 + RING + WARPS * SZ + MERGE + QF + ROWS * (NCH + 1) * 4 + 2 * WARPS * ROWS * 4;
     static constexpr bool Q_REGS = PARTS * NT * NCH * 4 <= 16;
-    static constexpr int CTAS = D == 256 ? (NT == 1 ? 3 : 2) : (NT * PARTS == 1 ? 4 : 3);  // on an SM
     static constexpr bool SUBNORMAL = PARTS == 1;         // how codes enter the products
     static constexpr int SLOT = ROWS * (D + 2);           // floats of a partial result
+    static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
 {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
+}
+// Four 8 x 8 matrices of 16-bit elements, rows at the addresses of lanes 0-7, 8-15, 16-23, 24-31
+template <bool TRANS> __device__ __forceinline__ uint4 load_matrices(uint32_t a)
+{
+    uint4 v;
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
 }
 template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int valid)
 {
@@ -103,21 +126,37 @@ template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, co
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(valid) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint32_t lds32(uint32_t a)
+// Ordinary loads and stores of shared memory (an address in its window), which the compiler may move between barriers
+__device__ __forceinline__ uint32_t lds32(uint32_t a) { return *static_cast<const uint32_t *>(__cvta_shared_to_generic(a)); }
+__device__ __forceinline__ uint2 lds64(uint32_t a) { return *static_cast<const uint2 *>(__cvta_shared_to_generic(a)); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) { return *static_cast<const uint4 *>(__cvta_shared_to_generic(a)); }
+template <typename V> __device__ __forceinline__ void sts(uint32_t a, V v) { *static_cast<V *>(__cvta_shared_to_generic(a)) = v; }
+// N 32-bit words, a multiple of two
+template <int N> __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N])
 {
-    uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 w = lds128(a + 4 * i);
+            v[i] = w.x, v[i + 1] = w.y, v[i + 2] = w.z, v[i + 3] = w.w;
+        }
+    } else {
+        static_assert(N == 2, "words");
+        const uint2 w = lds64(a);
+        v[0] = w.x, v[1] = w.y;
+    }
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a)
+template <int N> __device__ __forceinline__ void sts_words(uint32_t a, const uint32_t (&v)[N])
 {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            sts(a + 4 * i, make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+    } else {
+        static_assert(N == 2, "words");
+        sts(a, make_uint2(v[0], v[1]));
+    }
 }
-__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 __device__ __forceinline__ float half_lo(uint32_t w) { return __half2float(__ushort_as_half(uint16_t(w))); }
 __device__ __forceinline__ float half_hi(uint32_t w) { return __half2float(__ushort_as_half(uint16_t(w >> 16))); }
 // Two codes as halves: the nibbles at bits 0-3 and 16-19 of `w` (SECOND: 4-7 and 20-23).
@@ -125,24 +164,46 @@ template <bool SUBNORMAL, bool SECOND> __device__ __forceinline__ uint32_t codes
 {
     return (w & (SECOND ? 0x00f000f0u : 0x000f000fu)) | (SUBNORMAL ? 0u : SECOND ? 0x54005400u : 0x64006400u);
 }
-// The same form of a zero point's halves, from the first position's.
-template <bool SUBNORMAL> __device__ __forceinline__ uint32_t second_zero(uint32_t z)
+// code - zero of two codes; `z` holds the zeros as subnormal halves.
+template <bool SUBNORMAL, bool SECOND> __device__ __forceinline__ uint32_t minus_zero(uint32_t w, uint32_t z)
 {
-    return SUBNORMAL ? z << 4 : ((z & 0x000f000fu) << 4) | 0x54005400u;
-}
-__device__ __forceinline__ uint32_t sub_halves(uint32_t a, uint32_t b)
-{
-    const __half2 h = __hsub2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+    const uint32_t code = codes_at<SUBNORMAL, SECOND>(w);
+    __half2 h;
+    if constexpr (SUBNORMAL && SECOND)  // 16 zero * 2^-24
+        h = __hfma2(*reinterpret_cast<const __half2 *>(&z), __half2half2(__ushort_as_half(0xcc00)), *reinterpret_cast<const __half2 *>(&code));
+    else {
+        const uint32_t zero = SUBNORMAL ? z : SECOND ? (z << 4) | 0x54005400u : z | 0x64006400u;
+        h = __hsub2(*reinterpret_cast<const __half2 *>(&code), *reinterpret_cast<const __half2 *>(&zero));
+    }
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+
+// a / b for b > 0; 64-bit divisions cost a hundred instructions, so the usual sizes take a 32-bit one
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b)
+{
+    if (((a | b) >> 32) == 0)
+        return int64_t(uint32_t(a) / uint32_t(b));
+    return a / b;
+}
+// An equal share of `total` units for each of `ctas` CTAs, the first ones one more.
+struct Shares {
+    int64_t base, more;
+    __device__ __forceinline__ Shares(int64_t total, int64_t ctas) : base(divide(total, ctas)), more(total - base * ctas) {}
+    __device__ __forceinline__ int64_t begin(int64_t cta) const { return cta * base + min(cta, more); }
+    __device__ __forceinline__ int64_t holder(int64_t unit) const  // the CTA that has this unit
+    {
+        const int64_t large = more * (base + 1);
+        return unit < large ? divide(unit, base + 1) : more + divide(unit - large, base);
+    }
+};
 
 // What the sequence arrays say about sequence b.
 struct Sequence {
     int first, n;       // packed rows
     int len, start;     // tokens in the cache; the first one that is read, on a step's boundary
-    int units, tiles;   // 64-token units; tiles of query rows
+    int units, tiles;   // units; tiles of query rows
 };
-template <int ROWS> __device__ __forceinline__ Sequence sequence(const Kv4Args &a, int b, bool report)
+template <int ROWS, int UNIT> __device__ __forceinline__ Sequence sequence(const Kv4Args &a, int b, bool report)
 {
     Sequence s;
     const int end = a.cu[b + 1];
@@ -165,58 +226,83 @@ template <int ROWS> __device__ __forceinline__ Sequence sequence(const Kv4Args &
         s.start = from > 0 ? int(from) & ~(STEP - 1) : 0;
     }
     s.units = s.n > 0 ? max(1, (s.len - s.start + UNIT - 1) / UNIT) : 0;
-    s.tiles = int((int64_t(s.n) * a.group + ROWS - 1) / ROWS);
+    s.tiles = (s.n * a.group + ROWS - 1) / ROWS;  // tokens x query heads < 2^31
     return s;
 }
 
+template <int N> __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
+// The same, and whether `ok` holds for all of them.
+template <int N> __device__ __forceinline__ bool consumers_all(bool ok)
+{
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(uint32_t(ok)), "n"(N)
+        : "memory");
+    return all != 0;
+}
+// A wait that has run out ends every other wait of the CTA soon after.
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *dead, int *status, int code)
+{
+    for (uint32_t i = 0; i < umma::WAIT_LIMIT; i++) {
+        if (umma::mbar_try_wait(bar, parity))
+            return true;
+        if ((i & 255) == 255 && *dead)
+            return false;
+    }
+    *dead = 1;
+    atomicExch(status, code);
+    return false;
+}
+
 template <typename T, int D, int NT, int PARTS>
-__global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attention_kv4_kernel(const __grid_constant__ Kv4Args a)
+__global__ void __launch_bounds__(Shape<D, NT, PARTS>::THREADS, 1)
+attention_kv4_kernel(const __grid_constant__ Kv4Args a)
 {
     using S = Shape<D, NT, PARTS>;
-    constexpr int NCH = S::NCH, ROWS = S::ROWS;
-    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int NCH = S::NCH, ROWS = S::ROWS, STAGES = S::STAGES, WARPS = S::WARPS, UNIT = S::UNIT, THREADS = S::THREADS;
+    constexpr int CONSUMERS = WARPS * 32;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int64_t warp_sums[THREADS / 32], found[2];
+    __shared__ uint64_t full[STAGES], empty[STAGES];
+    __shared__ int dead_word;
+    volatile int *const dead = &dead_word;
+    const uint32_t ring = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *const smem = smem_raw + (ring - umma::smem_u32(smem_raw));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint8_t *const qf = smem + S::RING;
+    float *const merge = reinterpret_cast<float *>(smem + S::RING + WARPS * S::SZ);
+    uint8_t *const qf = reinterpret_cast<uint8_t *>(merge) + S::MERGE;
     float *const q_sum = reinterpret_cast<float *>(qf + S::QF);       // [NCH][ROWS]
     float *const q_factor = q_sum + ROWS * NCH;                       // [ROWS]
-    float *const stat = q_factor + ROWS;                              // [WARPS][ROWS] maxima, then sums
-    int64_t *const shared64 = reinterpret_cast<int64_t *>(smem + S::SMEM - 64);
-    const uint32_t ring = umma::smem_u32(smem) + warp * S::WARP_BYTES;
-    const uint32_t sz = ring + S::STAGES * S::STAGE;
+    float *const stat = q_factor + ROWS;                              // [WARPS][ROWS] references, then sums
+    const uint32_t sz = ring + S::RING + warp * S::SZ;
 
     OVK_PDL_LAUNCH_DEPENDENTS();
-    if (tid == 0)
+    if (tid == 0) {
         a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+        dead_word = 0;
+        for (int i = 0; i < STAGES; i++) {
+            umma::mbar_init(&full[i], 4 * 33);  // the producers' lanes, and one of each warp again for what it stores itself
+            umma::mbar_init(&empty[i], WARPS);
+        }
+        umma::fence_barrier_init();
+    }
 
     // ------------------------------------------------ this CTA's run of units
-    int64_t total = 0;
-    for (int b = tid; b < a.batch; b += WARPS * 32) {
-        const Sequence s = sequence<ROWS>(a, b, blockIdx.x == 0);
-        total += int64_t(s.units) * s.tiles * a.kv_heads;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0)
-        shared64[warp] = total;
-    __syncthreads();
-    total = shared64[0] + shared64[1] + shared64[2] + shared64[3];
-    const int64_t ctas = min(int64_t(gridDim.x), total);  // each has at least one unit
-    if (blockIdx.x >= ctas)
-        return;
-    int64_t at = blockIdx.x * total / ctas;
-    const int64_t end = (blockIdx.x + 1) * total / ctas;
-    // the sequence that holds unit `at`: a scan over the batch, 128 sequences at a time
-    int b = 0;
-    int64_t before = 0;  // units of the sequences before b
-    for (int base = 0;; base += WARPS * 32) {
-        const int mine = base + tid;
-        int64_t sum = 0;
-        if (mine < a.batch) {
-            const Sequence s = sequence<ROWS>(a, mine, false);
-            sum = int64_t(s.units) * s.tiles * a.kv_heads;
-        }
-        const int64_t own = sum;
+    // A scan over the batch, a sequence a thread; more sequences than threads take a pass for the total first.
+    auto units_of = [&](int b, bool report) -> int64_t {
+        if (b >= a.batch)
+            return 0;
+        const Sequence s = sequence<ROWS, UNIT>(a, b, report);
+        return int64_t(s.units) * s.tiles * a.kv_heads;
+    };
+    // the units of this thread's sequence and those before it in the chunk; the chunk's total
+    auto scan = [&](int64_t own, int64_t &before) -> int64_t {
+        int64_t sum = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t left = __shfl_up_sync(0xffffffffu, sum, o);
@@ -225,45 +311,171 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
         }
         __syncthreads();
         if (lane == 31)
-            shared64[warp] = sum;
+            warp_sums[warp] = sum;
         __syncthreads();
-        int64_t offset = before;
-        for (int w = 0; w < warp; w++)
-            offset += shared64[w];
-        const int64_t chunk_end = before + shared64[0] + shared64[1] + shared64[2] + shared64[3];
-        if (at >= offset + sum - own && at < offset + sum) {
-            shared64[4] = mine;
-            shared64[5] = offset + sum - own;
+        int64_t all = 0;
+        before = sum - own;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; w++) {
+            before += w < warp ? warp_sums[w] : 0;
+            all += warp_sums[w];
         }
-        __syncthreads();
-        if (at < chunk_end) {
-            b = int(shared64[4]);
-            before = shared64[5];
-            break;
-        }
-        before = chunk_end;
+        return all;
+    };
+    int64_t own = units_of(tid, blockIdx.x == 0), place_before, total = scan(own, place_before);
+    for (int base = THREADS; base < a.batch; base += THREADS) {
+        int64_t unused;
+        total += scan(units_of(base + tid, blockIdx.x == 0), unused);
     }
-    Sequence seq = sequence<ROWS>(a, b, false);
-    int64_t in_seq = at - before;
-    int item = int(in_seq / seq.units), unit = int(in_seq - int64_t(item) * seq.units);
+    const int64_t ctas = min(int64_t(gridDim.x), total);  // each has at least one unit
+    if (blockIdx.x >= ctas)
+        return;
+    const Shares shares(total, ctas);
+    int64_t at = shares.begin(blockIdx.x);
+    const int64_t end = shares.begin(blockIdx.x + 1);
+    int64_t chunk = 0;  // units of the chunks before
+    for (int base = 0;; base += THREADS) {
+        int64_t all = total;
+        if (a.batch > THREADS) {
+            own = units_of(base + tid, false);
+            all = scan(own, place_before);
+        }
+        const int64_t mine = chunk + place_before;
+        if (at >= mine && at < mine + own)
+            found[0] = base + tid, found[1] = mine;
+        if (at < chunk + all)
+            break;
+        chunk += all;
+    }
+    __syncthreads();
+    int b = int(found[0]);
+    Sequence seq = sequence<ROWS, UNIT>(a, b, false);
+    int item = int(divide(at - found[1], seq.units)), unit = int(at - found[1] - int64_t(item) * seq.units);
+    // both kinds of warps walk the run's segments - a piece of one item - with this
+    auto next_segment = [&](int units_here) {
+        at += units_here;
+        if (at >= end)
+            return false;
+        unit = 0;
+        if (++item == seq.tiles * a.kv_heads) {
+            item = 0;
+            do {
+                b++;
+                seq = sequence<ROWS, UNIT>(a, b, false);
+            } while (seq.units == 0);
+        }
+        return true;
+    };
 
+    if (warp >= WARPS) {
+        // ----------------------------------------------------------- producers
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::PRODUCER_REGS));
+        constexpr int ROUNDS = UNIT / 32, MINE = (ROUNDS + 3) / 4;  // 32 tokens a round, a lane each; rounds are dealt to the warps
+        const int producer = warp - WARPS, zero_bytes = (a.blocks + 1) >> 1;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        do {
+            const int units_here = int(min(int64_t(seq.units - unit), end - at));
+            const int head = item % a.kv_heads;
+            const int first = seq.start + unit * UNIT + 32 * producer + lane, t_end = min(seq.len, seq.start + (unit + units_here) * UNIT);
+            const int32_t *const table = a.table + int64_t(b) * a.max_pages;
+            auto row_of = [&](int token) {  // the cache row of a token; -1: none
+                if (token >= t_end)
+                    return -1;
+                const int page = a.page_shift >= 0 ? token >> a.page_shift : token / a.page_size;
+                const int where = table[page];
+                if (where < 0 || where >= a.pages) {
+                    atomicExch(a.status, OVK_DEV_BAD_PAGE);
+                    return -1;
+                }
+                return (where * a.kv_heads + head) * a.page_size + (token - page * a.page_size);
+            };
+            int row[MINE];  // of the unit that is next
+#pragma unroll
+            for (int i = 0; i < MINE; i++)
+                row[i] = producer + 4 * i < ROUNDS ? row_of(first + 128 * i) : -1;
+            for (int u = 0; u < units_here; u++) {
+                ok = wait(&empty[stage], phase ^ 1, dead, a.status, OVK_DEV_TIMEOUT_SLOT);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t to = ring + stage * S::STAGE, raw = to + 2 * S::CODES;
+#pragma unroll
+                for (int i = 0; i < MINE; i++) {
+                    const int round = producer + 4 * i;
+                    if (round >= ROUNDS)
+                        break;
+                    const int now = row[i], place = 32 * round + lane, r0 = max(now, 0);
+                    const bool there = now >= 0;
+#pragma unroll
+                    for (int j = 0; j < S::CPR; j++) {
+                        const int index = lane + 32 * j, r = index / S::CPR, c = index % S::CPR;
+                        const int src = __shfl_sync(0xffffffffu, now, r);
+                        const int64_t offset = int64_t(max(src, 0)) * S::ROW_BYTES + c * 16;
+                        const int swizzle = S::CPR == 2 ? (r >> 2) & 1 : S::CPR == 4 ? (r >> 1) & 3 : r & 7;
+                        const uint32_t dst = to + (32 * round + r) * S::ROW_BYTES + ((c ^ swizzle) << 4);
+                        copy_async<16>(dst, a.codes[0] + offset, src >= 0 ? 16 : 0);
+                        copy_async<16>(dst + S::CODES, a.codes[1] + offset, src >= 0 ? 16 : 0);
+                    }
+                    // this lane's row: scales into 16 bytes, zero points into four; pieces below four bytes are read from
+                    // the word that holds them, up to their own end
+                    const int64_t scale = int64_t(r0) * (2 * a.blocks), zero = int64_t(r0) * zero_bytes;
+                    const uint32_t scale_to = raw + place * 16, zero_to = raw + 2 * S::SCALES + place * 4;
+                    const int zero_size = there ? int(zero & 3) + zero_bytes : 0, odd = r0 & 1;
+#pragma unroll
+                    for (int kv = 0; kv < 2; kv++) {
+                        if (a.blocks == 4)
+                            copy_async<8>(scale_to + kv * S::SCALES, a.scales[kv] + scale, there ? 8 : 0);
+                        else if (a.blocks == 8)
+                            copy_async<16>(scale_to + kv * S::SCALES, a.scales[kv] + scale, there ? 16 : 0);
+                        else if (a.blocks == 2)
+                            copy_async<4>(scale_to + kv * S::SCALES, a.scales[kv] + scale, there ? 4 : 0);
+                        else
+                            copy_async<4>(scale_to + kv * S::SCALES, a.scales[kv] + scale - 2 * odd, there ? 2 + 2 * odd : 0);
+                        if (a.zero_points[0])
+                            copy_async<4>(zero_to + kv * S::ZEROS, a.zero_points[kv] + (zero & ~int64_t(3)), zero_size);
+                    }
+                    sts(raw + 2 * (S::SCALES + S::ZEROS) + place * 4, uint32_t(now));
+                    const uint32_t present = __ballot_sync(0xffffffffu, there);
+                    if (lane == 0)
+                        sts(to + S::PRESENT + round * 4, present);
+                    if (u + 1 < units_here)
+                        row[i] = row_of(first + (u + 1) * UNIT + 128 * i);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(umma::smem_u32(&full[stage])) : "memory");
+                __syncwarp();
+                if (lane == 0)
+                    umma::mbar_arrive(&full[stage]);
+                if (++stage == STAGES)
+                    stage = 0, phase ^= 1;
+            }
+        } while (ok && next_segment(int(min(int64_t(seq.units - unit), end - at))));
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        return;
+    }
+
+    // ---------------------------------------------------------------- consumers
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::REGS));
+    int stage = 0;
+    uint32_t phase = 0;
     while (true) {
         const int units_here = int(min(int64_t(seq.units - unit), end - at));
         const int tile = item / a.kv_heads, head = item - tile * a.kv_heads;
-        const int rows = int(min(int64_t(ROWS), int64_t(seq.n) * a.group - int64_t(tile) * ROWS));
-        const int t_begin = seq.start + unit * UNIT, t_end = min(seq.len, seq.start + (unit + units_here) * UNIT);
+        const int rows = min(ROWS, seq.n * a.group - tile * ROWS);
+        const int t_begin = seq.start + unit * UNIT;
 
         // -------------------------------------------------- query fragments
-        __syncthreads();  // the segment before has been read
+        consumers_sync<CONSUMERS>();  // the segment before has been read
         if (tid < ROWS * 8) {
             const int r = tid >> 3, j = tid & 7;
             constexpr int GROUPS = D / 64;  // groups of eight elements a thread
             float v[GROUPS][8], top = 0.0f;
             if (r < rows) {
-                const int64_t row = int64_t(tile) * ROWS + r;
-                const int token = int(row / a.group);
+                const int row = tile * ROWS + r, token = row / a.group;
                 const T *src = static_cast<const T *>(a.q) + int64_t(seq.first + token) * a.q_token +
-                               (int64_t(head) * a.group + (row - int64_t(token) * a.group)) * a.q_head;
+                               (int64_t(head) * a.group + (row - token * a.group)) * a.q_head;
 #pragma unroll
                 for (int i = 0; i < GROUPS; i++)
                     load_row<T, 8, true>(src + 8 * (j + 8 * i), v[i]);
@@ -311,12 +523,12 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
                     dst[NT * NCH * 32 + slot] = make_uint4(pack_halves(lo[0], lo[4]), pack_halves(lo[1], lo[5]),
                                                            pack_halves(lo[2], lo[6]), pack_halves(lo[3], lo[7]));
                 if ((j & 3) == 0)
-                    q_sum[c * ROWS + r] = sum;
+                    q_sum[c * ROWS + r] = -sum;  // K's accumulators start at zero times this
             }
             if (j == 0)
                 q_factor[r] = ldexpf(a.scale_log2e, (S::SUBNORMAL ? 24 : 0) - k);
         }
-        __syncthreads();
+        consumers_sync<CONSUMERS>();
         uint4 bq[S::Q_REGS ? PARTS : 1][S::Q_REGS ? NT : 1][S::Q_REGS ? NCH : 1];
         if constexpr (S::Q_REGS) {
 #pragma unroll
@@ -337,84 +549,38 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
         }
         float factor[NT][2];
         int pos[NT][2];  // the last position that column reads; -1 for a column without a row
-        const int64_t row0 = int64_t(tile) * ROWS;
+        const int row0 = tile * ROWS;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const int r = n * 8 + 2 * t + e;
                 factor[n][e] = q_factor[r];
-                pos[n][e] = r < rows ? seq.len - seq.n + int((row0 + r) / a.group) : -1;
+                pos[n][e] = r < rows ? seq.len - seq.n + (row0 + r) / a.group : -1;
             }
-        const int pos_first = seq.len - seq.n + int(row0 / a.group);                    // of the tile's first row
-        const int pos_last = seq.len - seq.n + int((row0 + rows - 1) / a.group);
-
-        // ------------------------------------------------------ the ring
-        const int steps = t_end > t_begin + warp * STEP ? (t_end - t_begin - warp * STEP + UNIT - 1) / UNIT : 0;
-        auto row_of = [&](int step) -> int {  // the cache row of this lane's token of a step, -1: none
-            const int token = t_begin + (warp + WARPS * step) * STEP + (lane & 15);
-            if (step >= steps || token >= t_end)
-                return -1;
-            const int page = a.page_shift >= 0 ? token >> a.page_shift : token / a.page_size;
-            const int where = a.table[int64_t(b) * a.max_pages + page];
-            if (where < 0 || where >= a.pages) {
-                atomicExch(a.status, OVK_DEV_BAD_PAGE);
-                return -1;
-            }
-            return (where * a.kv_heads + head) * a.page_size + (token - page * a.page_size);
-        };
-        auto fetch = [&](int stage, int row) {
-            const uint32_t to = ring + stage * S::STAGE;
+        const int pos_first = seq.len - seq.n + row0 / a.group;                    // of the tile's first row
+        const int pos_last = seq.len - seq.n + (row0 + rows - 1) / a.group;
+        const int window = int(min(a.window, int64_t(1) << 30));  // positions are below 2^30
+        // where the rows that this lane addresses for ldmatrix lie: token lane % 16, and of two neighbouring chunks
+        // the one that lanes 16-31 read.  Rows eight apart have the same swizzle.
+        uint32_t k_at[NCH / 2];
 #pragma unroll
-            for (int i = 0; i < S::CPR / 2; i++) {
-                const int index = lane + 32 * i, r = index / S::CPR, c = index % S::CPR;
-                const int src = __shfl_sync(0xffffffffu, row, r);
-                const int64_t offset = int64_t(max(src, 0)) * S::ROW_BYTES + c * 16;
-                const int swizzle = S::CPR == 2 ? (r >> 2) & 1 : S::CPR == 4 ? (r >> 1) & 3 : r & 7;
-                const uint32_t dst = to + r * S::ROW_BYTES + ((c ^ swizzle) << 4);
-                copy_async<16>(dst, a.codes[0] + offset, src >= 0 ? 16 : 0);
-                copy_async<16>(dst + S::CODES, a.codes[1] + offset, src >= 0 ? 16 : 0);
-            }
-            // lanes 0-15 bring the keys' scales and zero points, lanes 16-31 the values'; pieces below four
-            // bytes are read from the word that holds them, up to their own end
-            const int kv = lane >> 4;
-            const int64_t r0 = max(row, 0);
-            const uint32_t raw = to + 2 * S::CODES;
-            const uint8_t *scale = a.scales[kv] + r0 * (2 * a.blocks);
-            if (a.blocks == 8)
-                copy_async<16>(raw + lane * 16, scale, row >= 0 ? 16 : 0);
-            else if (a.blocks == 4)
-                copy_async<8>(raw + lane * 16, scale, row >= 0 ? 8 : 0);
-            else if (a.blocks == 2)
-                copy_async<4>(raw + lane * 16, scale, row >= 0 ? 4 : 0);
-            else
-                copy_async<4>(raw + lane * 16, scale - 2 * (r0 & 1), row >= 0 ? 2 + 2 * int(r0 & 1) : 0);
-            if (a.zero_points[0]) {
-                const int bytes = (a.blocks + 1) >> 1;
-                const int64_t byte = r0 * bytes;
-                copy_async<4>(raw + 512 + lane * 4, a.zero_points[kv] + (byte & ~int64_t(3)), row >= 0 ? int(byte & 3) + bytes : 0);
-            }
-            sts32(raw + 640 + lane * 4, uint32_t(row));
-        };
-        {
-            int row[S::STAGES - 1];
-#pragma unroll
-            for (int i = 0; i < S::STAGES - 1; i++)
-                row[i] = row_of(i);
-#pragma unroll
-            for (int i = 0; i < S::STAGES - 1; i++) {
-                if (i < steps)
-                    fetch(i, row[i]);
-                copy_commit();
-            }
+        for (int i = 0; i < NCH / 2; i++) {
+            const int r = lane & 15, c = 2 * i + (lane >> 4);
+            const int swizzle = S::CPR == 2 ? (r >> 2) & 1 : S::CPR == 4 ? (r >> 1) & 3 : r & 7;
+            k_at[i] = ring + (warp * STEP + r) * S::ROW_BYTES + ((c ^ swizzle) << 4);
         }
-        int next_row = row_of(S::STAGES - 1);
+        // where the raw scales and zero points of this lane's row lie: lanes 0-15 keys, 16-31 values
+        const int place = warp * STEP + (lane & 15), kv = lane >> 4, zero_bytes = (a.blocks + 1) >> 1;
+        const uint32_t scale_at = ring + 2 * S::CODES + kv * S::SCALES + place * 16;
+        const uint32_t zero_at = ring + 2 * S::CODES + 2 * S::SCALES + kv * S::ZEROS + place * 4;
+        const uint32_t row_at = ring + 2 * S::CODES + 2 * (S::SCALES + S::ZEROS) + place * 4;
 
         float o[NCH][2][NT][4];
-        float m[NT][2], l[NT][2];
+        float m[NT][2], l[NT][2], reference[NT][2];  // reference: m and the scale's exponent, what p is relative to
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            m[n][0] = m[n][1] = NONE;
+            m[n][0] = m[n][1] = reference[n][0] = reference[n][1] = NONE;
             l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
             for (int c = 0; c < NCH; c++)
@@ -423,124 +589,144 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
                     o[c][0][n][e] = o[c][1][n][e] = 0.0f;
         }
         uint32_t top_scale = 0;  // fp16 bits of the V scale that the maximum allows for
+        bool ok = true;
+        for (int u = 0; u < units_here; u++) {
+            ok = wait(&full[stage], phase, dead, a.status, OVK_DEV_TIMEOUT_TMA);
+            if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
+                break;
+            }
+            const uint32_t to_stage = stage * S::STAGE;
+            const int token0 = t_begin + u * UNIT + warp * STEP;
+            // the step's tokens that are there
+            const uint32_t present = (lds32(ring + to_stage + S::PRESENT + (warp >> 1) * 4) >> (16 * (warp & 1))) & 0xffffu;
 
-        int stage = 0, ahead = S::STAGES - 1;
-        for (int step = 0; step < steps; step++) {
-            copy_wait<S::STAGES - 2>();
-            __syncwarp();
-            if (step + S::STAGES - 1 < steps)
-                fetch(ahead, next_row);
-            copy_commit();
-            next_row = row_of(step + S::STAGES);
-            const uint32_t from = ring + stage * S::STAGE, raw = from + 2 * S::CODES;
-
-            // ---------------- {scale, zero} of each chunk of this lane's row
-            const int row = int(lds32(raw + 640 + lane * 4));
-            uint32_t high = 0;
+            // -------- scale and zero of each chunk of this lane's row, as the products want them
+            uint32_t high;
             {
-                const uint4 s4 = lds128(raw + lane * 16);
-                uint32_t z = a.zero_points[0] ? lds32(raw + 512 + lane * 4) : 0x88888888u;
-                if (a.zero_points[0])
-                    z >>= 8 * ((uint32_t(row) * ((a.blocks + 1) >> 1)) & 3);
-                const uint32_t words[4] = {a.blocks == 1 && (row & 1) ? s4.x >> 16 : s4.x, s4.y, s4.z, s4.w};
-                const uint32_t sign = lane < 16 ? 0x80000000u : 0u;  // subnormal: K adds -zero
-                uint32_t out[NCH];
-                auto expand = [&](auto shift) {
-#pragma unroll
-                    for (int c = 0; c < NCH; c++) {
-                        const int blk = c >> decltype(shift)::value;
-                        const uint32_t h = (blk & 1) ? words[blk >> 1] >> 16 : words[blk >> 1] & 0xffffu;
-                        const uint32_t zero = (z >> (4 * blk)) & 15u;
-                        out[c] = h | (zero << 16) | (S::SUBNORMAL ? (zero ? sign : 0u) : 0x64000000u);
-                        high = max(high, h & 0x7fffu);
+                const uint32_t where = scale_at + to_stage;
+                uint32_t words[4] = {0, 0, 0, 0}, z = 0x88888888u;
+                if (a.blocks == 4) {
+                    const uint2 two = lds64(where);
+                    words[0] = two.x, words[1] = two.y;
+                } else if (a.blocks == 8) {
+                    lds_words(where, words);
+                } else {
+                    words[0] = lds32(where);
+                    if (a.blocks == 1) {
+                        words[0] = (lds32(row_at + to_stage) & 1u) ? words[0] >> 16 : words[0] & 0xffffu;
                     }
+                }
+                if (a.zero_points[0]) {
+                    z = lds32(zero_at + to_stage);
+                    if (zero_bytes < 4)
+                        z >>= 8 * ((lds32(row_at + to_stage) * zero_bytes) & 3);
+                }
+                if (!((present >> (lane & 15)) & 1u))
+                    words[0] = words[1] = words[2] = words[3] = 0;
+                const uint32_t z_next = __shfl_down_sync(0xffffffffu, z, 1);  // the next token's, for pairs of V
+                auto expand = [&](auto shift) {
+                    constexpr int SHIFT = decltype(shift)::value, BLOCKS = NCH >> SHIFT;
+                    float s[BLOCKS];
+#pragma unroll
+                    for (int i = 0; i < BLOCKS; i++)
+                        s[i] = (i & 1) ? half_hi(words[i >> 1]) : half_lo(words[i >> 1]);
+                    if (kv == 0) {
+                        uint32_t out[2 * NCH];
+#pragma unroll
+                        for (int c = 0; c < NCH; c++) {
+                            const int blk = c >> SHIFT;
+                            out[2 * c] = __float_as_uint(s[blk]);
+                            const uint32_t zero = (z >> (4 * blk)) & 15u;
+                            // f16: what the accumulator's start multiplies; f32: the zero of a pair of codes
+                            out[2 * c + 1] = S::SUBNORMAL ? __float_as_uint(half_lo(zero)) : zero * 0x00010001u;
+                        }
+                        sts_words(sz + (lane & 15) * (NCH * 8), out);
+                    } else {
+                        uint32_t out[NCH];
+#pragma unroll
+                        for (int c = 0; c < NCH; c++)
+                            out[c] = __float_as_uint(s[c >> SHIFT]);
+                        sts_words(sz + S::K_SZ + (lane & 15) * (NCH * 4), out);
+                        if ((lane & 1) == 0) {
+                            const uint32_t low = __byte_perm(z, z_next, 0x5410), up = __byte_perm(z, z_next, 0x7632);
+#pragma unroll
+                            for (int c = 0; c < NCH; c++) {
+                                const int blk = c >> SHIFT;
+                                out[c] = ((blk < 4 ? low : up) >> (4 * (blk & 3))) & 0x000f000fu;
+                            }
+                            sts_words(sz + S::K_SZ + S::V_S + (lane & 15) / 2 * (NCH * 4), out);
+                        }
+                    }
+                    // the largest scale of the row (the order of fp16 numbers is that of their bits)
+                    uint32_t two = words[0] & (BLOCKS == 1 ? 0x7fffu : 0x7fff7fffu);
+#pragma unroll
+                    for (int i = 1; i < BLOCKS / 2; i++)
+                        two = __vmaxu2(two, words[i] & 0x7fff7fffu);
+                    high = kv == 0 ? 0u : max(two & 0xffffu, two >> 16);
                 };
                 if (a.chunk_shift == 0)
                     expand(std::integral_constant<int, 0>());
                 else if (a.chunk_shift == 1)
                     expand(std::integral_constant<int, 1>());
                 else
-                    expand(std::integral_constant<int, 2>());
-                const uint32_t dst = sz + lane * (NCH * 4);
-                if constexpr (NCH == 2) {
-                    asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(dst), "r"(out[0]), "r"(out[1]) : "memory");
-                } else {
-#pragma unroll
-                    for (int c = 0; c < NCH; c += 4)
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + c * 4), "r"(out[c]), "r"(out[c + 1]),
-                                     "r"(out[c + 2]), "r"(out[c + 3])
-                                     : "memory");
-                }
+                    expand(std::integral_constant<int, NCH >= 4 ? 2 : 1>());
             }
-            const uint32_t present = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-            high = lane < 16 || row < 0 ? 0u : high;
-            // (ballot and the vote below order the stores above before the reads)
             const bool scale_moves = __any_sync(0xffffffffu, high > top_scale + (3u << 10));
             __syncwarp();
-            const int token0 = t_begin + (warp + WARPS * step) * STEP;
 
             // ---------------------------------------------------- scores
             float x[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++)
                 x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
-            const uint32_t k_row = from + g * S::ROW_BYTES + t * 4;
-            const int swz = S::CPR == 2 ? (g >> 2) & 1 : S::CPR == 4 ? (g >> 1) & 3 : g & 7;
-            const int swz8 = S::CPR == 2 ? ((g + 8) >> 2) & 1 : S::CPR == 4 ? ((g + 8) >> 1) & 3 : (g + 8) & 7;
-            uint32_t sz_a[NCH], sz_b[NCH];  // tokens g and g + 8
-            auto load_sz = [&](uint32_t base, uint32_t (&v)[NCH]) {
-                if constexpr (NCH == 2) {
-                    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(base));
-                } else {
 #pragma unroll
-                    for (int c = 0; c < NCH; c += 4) {
-                        const uint4 w = lds128(base + c * 4);
-                        v[c] = w.x, v[c + 1] = w.y, v[c + 2] = w.z, v[c + 3] = w.w;
+            for (int i = 0; i < NCH / 2; i++) {
+                // tokens 0-7 and 8-15 of chunk 2i, then of chunk 2i + 1
+                const uint4 words = load_matrices<false>(k_at[i] + to_stage);
+                const uint4 sz_a = lds128(sz + g * (NCH * 8) + 16 * i), sz_b = lds128(sz + (g + 8) * (NCH * 8) + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    constexpr bool SUB = S::SUBNORMAL;
+                    const int c = 2 * i + j;
+                    const uint32_t w0 = j ? words.z : words.x, w1 = j ? words.w : words.y, v0 = w0 >> 8, v1 = w1 >> 8;
+                    const float s0 = __uint_as_float(j ? sz_a.z : sz_a.x), s1 = __uint_as_float(j ? sz_b.z : sz_b.x);
+                    const uint32_t z0 = j ? sz_a.w : sz_a.y, z1 = j ? sz_b.w : sz_b.y;
+                    uint32_t a0[4] = {codes_at<SUB, false>(w0), codes_at<SUB, false>(w1), codes_at<SUB, true>(w0), codes_at<SUB, true>(w1)};
+                    uint32_t a1[4] = {codes_at<SUB, false>(v0), codes_at<SUB, false>(v1), codes_at<SUB, true>(v0), codes_at<SUB, true>(v1)};
+                    if constexpr (!SUB) {
+                        a0[0] = minus_zero<SUB, false>(w0, z0), a0[1] = minus_zero<SUB, false>(w1, z1);
+                        a0[2] = minus_zero<SUB, true>(w0, z0), a0[3] = minus_zero<SUB, true>(w1, z1);
+                        a1[0] = minus_zero<SUB, false>(v0, z0), a1[1] = minus_zero<SUB, false>(v1, z1);
+                        a1[2] = minus_zero<SUB, true>(v0, z0), a1[3] = minus_zero<SUB, true>(v1, z1);
                     }
-                }
-            };
-            load_sz(sz + g * (NCH * 4), sz_a);
-            load_sz(sz + (g + 8) * (NCH * 4), sz_b);
 #pragma unroll
-            for (int c = 0; c < NCH; c++) {
-                const uint32_t w0 = lds32(k_row + ((c ^ swz) << 4)), w1 = lds32(k_row + 8 * S::ROW_BYTES + ((c ^ swz8) << 4));
-                constexpr bool SUB = S::SUBNORMAL;
-                const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
-                uint32_t a0[4] = {codes_at<SUB, false>(w0), codes_at<SUB, false>(w1), codes_at<SUB, true>(w0), codes_at<SUB, true>(w1)};
-                uint32_t a1[4] = {codes_at<SUB, false>(v0), codes_at<SUB, false>(v1), codes_at<SUB, true>(v0), codes_at<SUB, true>(v1)};
-                float s0 = half_lo(sz_a[c]), s1 = half_lo(sz_b[c]), z0 = 0.0f, z1 = 0.0f;
-                if constexpr (SUB) {
-                    z0 = half_hi(sz_a[c]), z1 = half_hi(sz_b[c]);
-                } else {
-                    const uint32_t za = __byte_perm(sz_a[c], 0, 0x3232), zb = __byte_perm(sz_b[c], 0, 0x3232);
-                    const uint32_t za2 = second_zero<SUB>(za), zb2 = second_zero<SUB>(zb);
-                    a0[0] = sub_halves(a0[0], za), a0[1] = sub_halves(a0[1], zb), a0[2] = sub_halves(a0[2], za2), a0[3] = sub_halves(a0[3], zb2);
-                    a1[0] = sub_halves(a1[0], za), a1[1] = sub_halves(a1[1], zb), a1[2] = sub_halves(a1[2], za2), a1[3] = sub_halves(a1[3], zb2);
-                }
+                    for (int n = 0; n < NT; n++) {
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if constexpr (SUB) {
+                            float2 sum;
+                            if constexpr (S::Q_REGS)
+                                sum = qs[n][c];
+                            else
+                                sum = *reinterpret_cast<const float2 *>(q_sum + c * ROWS + n * 8 + 2 * t);
+                            acc[0] = __uint_as_float(z0) * sum.x, acc[1] = __uint_as_float(z0) * sum.y;
+                            acc[2] = __uint_as_float(z1) * sum.x, acc[3] = __uint_as_float(z1) * sum.y;
+                        }
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float2 sum = make_float2(0.0f, 0.0f);
-                    if constexpr (SUB) {
-                        if constexpr (S::Q_REGS)
-                            sum = qs[n][c];
-                        else
-                            sum = *reinterpret_cast<const float2 *>(q_sum + c * ROWS + n * 8 + 2 * t);
+                        for (int p = 0; p < PARTS; p++) {
+                            uint4 q4;
+                            if constexpr (S::Q_REGS)
+                                q4 = bq[p][n][c];
+                            else
+                                q4 = reinterpret_cast<const uint4 *>(qf)[((p * NT + n) * NCH + c) * 32 + lane];
+                            mma(acc, a0, q4.x, q4.y);
+                            mma(acc, a1, q4.z, q4.w);
+                        }
+                        x[n][0] = fmaf(s0, acc[0], x[n][0]);
+                        x[n][1] = fmaf(s0, acc[1], x[n][1]);
+                        x[n][2] = fmaf(s1, acc[2], x[n][2]);
+                        x[n][3] = fmaf(s1, acc[3], x[n][3]);
                     }
-                    float acc[4] = {z0 * sum.x, z0 * sum.y, z1 * sum.x, z1 * sum.y};
-#pragma unroll
-                    for (int p = 0; p < PARTS; p++) {
-                        uint4 q4;
-                        if constexpr (S::Q_REGS)
-                            q4 = bq[p][n][c];
-                        else
-                            q4 = reinterpret_cast<const uint4 *>(qf)[((p * NT + n) * NCH + c) * 32 + lane];
-                        mma(acc, a0, q4.x, q4.y);
-                        mma(acc, a1, q4.z, q4.w);
-                    }
-                    x[n][0] = fmaf(s0, acc[0], x[n][0]);
-                    x[n][1] = fmaf(s0, acc[1], x[n][1]);
-                    x[n][2] = fmaf(s1, acc[2], x[n][2]);
-                    x[n][3] = fmaf(s1, acc[3], x[n][3]);
                 }
             }
 #pragma unroll
@@ -548,8 +734,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     x[n][e] *= factor[n][e & 1];
-            const bool masked = present != 0xffffu || token0 + STEP - 1 > pos_first ||
-                                (a.window > 0 && int64_t(token0) < int64_t(pos_last) - a.window + 1);
+            const bool masked = present != 0xffffu || token0 + STEP - 1 > pos_first || (window > 0 && token0 < pos_last - window + 1);
             if (masked) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
@@ -557,7 +742,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
                     for (int e = 0; e < 4; e++) {
                         const int token = token0 + g + (e >= 2 ? 8 : 0), p = pos[n][e & 1];
                         const bool read = ((present >> (g + (e >= 2 ? 8 : 0))) & 1u) && token <= p &&
-                                          (a.window <= 0 || int64_t(token) > int64_t(p) - a.window);
+                                          (window == 0 || token > p - window);
                         if (!read)
                             x[n][e] = -INFINITY;
                     }
@@ -575,8 +760,9 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
                 for (int o_ = 16; o_ > 0; o_ >>= 1)
                     high = max(high, __shfl_xor_sync(0xffffffffu, high, o_));
                 const uint32_t new_scale = max(top_scale, min(high, 0x7800u) & 0x7c00u);
-                const float shift = float(int(new_scale >> 10) - int(top_scale >> 10));
                 top_scale = new_scale;
+                // p is smaller by the exponent of the largest scale, less 6
+                const float lower = float(int(new_scale >> 10) - 21);
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -586,8 +772,9 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
                         for (int o_ = 4; o_ < 32; o_ <<= 1)
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o_));
                         const float to = fmaxf(m[n][e], most);
-                        const float f = exp2_approx(m[n][e] - to - shift);
+                        const float f = exp2_approx(reference[n][e] - (to + lower));
                         m[n][e] = to;
+                        reference[n][e] = to + lower;
                         l[n][e] *= f;
 #pragma unroll
                         for (int c = 0; c < NCH; c++) {
@@ -596,75 +783,68 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
                         }
                     }
             }
-            // p carries 2^-(exponent of the largest scale - 6): top_scale >> 10 is the exponent + 15
-            const float lower = float(int(top_scale >> 10) - 21);
             float p[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    p[n][e] = exp2_approx(x[n][e] - m[n][e & 1] - lower);
+                    p[n][e] = exp2_approx(x[n][e] - reference[n][e & 1]);
                 l[n][0] += p[n][0] + p[n][2];
                 l[n][1] += p[n][1] + p[n][3];
             }
             // ---------------------------------------------------- values
-            load_sz(sz + (STEP + g) * (NCH * 4), sz_a);
-            load_sz(sz + (STEP + g + 8) * (NCH * 4), sz_b);
-            uint32_t za[NCH], zb[NCH], zc[NCH], zd[NCH];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-            load_sz(sz + (STEP + 2 * t) * (NCH * 4), za);
-            load_sz(sz + (STEP + 2 * t + 1) * (NCH * 4), zb);
-            load_sz(sz + (STEP + 2 * t + 8) * (NCH * 4), zc);
-            load_sz(sz + (STEP + 2 * t + 9) * (NCH * 4), zd);
-            const uint32_t v_base = from + S::CODES + (g >> 1) * 4;
-            const uint32_t select = (g & 1) ? 0x7632u : 0x5410u;
+            auto values = [&](auto is_masked) {
 #pragma unroll
-            for (int c = 0; c < NCH; c++) {
-                uint32_t w[4];
+                for (int i = 0; i < NCH / 2; i++) {
+                    // pairs of tokens 2t, 2t + 1 and 2t + 8, 2t + 9 of chunk 2i, then of chunk 2i + 1
+                    const uint4 words = load_matrices<true>(k_at[i] + to_stage + S::CODES);
+                    const uint2 s_a = lds64(sz + S::K_SZ + g * (NCH * 4) + 8 * i), s_b = lds64(sz + S::K_SZ + (g + 8) * (NCH * 4) + 8 * i);
+                    const uint2 z_a = lds64(sz + S::K_SZ + S::V_S + t * (NCH * 4) + 8 * i), z_b = lds64(sz + S::K_SZ + S::V_S + (t + 4) * (NCH * 4) + 8 * i);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int token = 2 * t + (i & 1) + (i >> 1) * 8;
-                    const int sw = S::CPR == 2 ? (token >> 2) & 1 : S::CPR == 4 ? (token >> 1) & 3 : token & 7;
-                    w[i] = lds32(v_base + token * S::ROW_BYTES + ((c ^ sw) << 4));
-                }
-                const uint32_t y0 = __byte_perm(w[0], w[1], select), y1 = __byte_perm(w[2], w[3], select);
-                const uint32_t z0 = __byte_perm(za[c], zb[c], 0x7632), z1 = __byte_perm(zc[c], zd[c], 0x7632);
-                constexpr bool SUB = S::SUBNORMAL;
-                const uint32_t z0s = second_zero<SUB>(z0), z1s = second_zero<SUB>(z1);
-                const uint32_t h0 = y0 >> 8, h1 = y1 >> 8;
-                const uint32_t a0[4] = {sub_halves(codes_at<SUB, false>(y0), z0), sub_halves(codes_at<SUB, true>(y0), z0s),
-                                        sub_halves(codes_at<SUB, false>(y1), z1), sub_halves(codes_at<SUB, true>(y1), z1s)};
-                const uint32_t a1[4] = {sub_halves(codes_at<SUB, false>(h0), z0), sub_halves(codes_at<SUB, true>(h0), z0s),
-                                        sub_halves(codes_at<SUB, false>(h1), z1), sub_halves(codes_at<SUB, true>(h1), z1s)};
-                const float s0 = half_lo(sz_a[c]), s1 = half_lo(sz_b[c]);
+                    for (int j = 0; j < 2; j++) {
+                        constexpr bool SUB = S::SUBNORMAL;
+                        const int c = 2 * i + j;
+                        const uint32_t y0 = j ? words.z : words.x, y1 = j ? words.w : words.y, h0 = y0 >> 8, h1 = y1 >> 8;
+                        const uint32_t z0 = j ? z_a.y : z_a.x, z1 = j ? z_b.y : z_b.x;
+                        const uint32_t a0[4] = {minus_zero<SUB, false>(y0, z0), minus_zero<SUB, true>(y0, z0), minus_zero<SUB, false>(y1, z1),
+                                                minus_zero<SUB, true>(y1, z1)};
+                        const uint32_t a1[4] = {minus_zero<SUB, false>(h0, z0), minus_zero<SUB, true>(h0, z0), minus_zero<SUB, false>(h1, z1),
+                                                minus_zero<SUB, true>(h1, z1)};
+                        const float s0 = __uint_as_float(j ? s_a.y : s_a.x), s1 = __uint_as_float(j ? s_b.y : s_b.x);
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float w0 = p[n][0] * s0, w1 = p[n][1] * s0, w2 = p[n][2] * s1, w3 = p[n][3] * s1;
-                    if (masked) {  // a scale that is not finite must not reach rows that do not read its token
-                        w0 = p[n][0] == 0.0f ? 0.0f : w0, w1 = p[n][1] == 0.0f ? 0.0f : w1;
-                        w2 = p[n][2] == 0.0f ? 0.0f : w2, w3 = p[n][3] == 0.0f ? 0.0f : w3;
-                    }
-                    const uint32_t h01 = pack_halves(w0, w1), h23 = pack_halves(w2, w3);
-                    const uint32_t b0 = transpose8x8(h01), b1 = transpose8x8(h23);
-                    mma(o[c][0][n], a0, b0, b1);
-                    mma(o[c][1][n], a1, b0, b1);
-                    if constexpr (PARTS == 2) {
-                        const uint32_t l01 = pack_halves(w0 - half_lo(h01), w1 - half_hi(h01));
-                        const uint32_t l23 = pack_halves(w2 - half_lo(h23), w3 - half_hi(h23));
-                        const uint32_t c0 = transpose8x8(l01), c1 = transpose8x8(l23);
-                        mma(o[c][0][n], a0, c0, c1);
-                        mma(o[c][1][n], a1, c0, c1);
+                        for (int n = 0; n < NT; n++) {
+                            float w0 = p[n][0] * s0, w1 = p[n][1] * s0, w2 = p[n][2] * s1, w3 = p[n][3] * s1;
+                            if constexpr (decltype(is_masked)::value) {  // a scale that is not finite stays with the rows that read its token
+                                w0 = p[n][0] == 0.0f ? 0.0f : w0, w1 = p[n][1] == 0.0f ? 0.0f : w1;
+                                w2 = p[n][2] == 0.0f ? 0.0f : w2, w3 = p[n][3] == 0.0f ? 0.0f : w3;
+                            }
+                            const uint32_t h01 = pack_halves(w0, w1), h23 = pack_halves(w2, w3);
+                            const uint32_t b0 = transpose8x8(h01), b1 = transpose8x8(h23);
+                            mma(o[c][0][n], a0, b0, b1);
+                            mma(o[c][1][n], a1, b0, b1);
+                            if constexpr (PARTS == 2) {
+                                const uint32_t l01 = pack_halves(w0 - half_lo(h01), w1 - half_hi(h01));
+                                const uint32_t l23 = pack_halves(w2 - half_lo(h23), w3 - half_hi(h23));
+                                const uint32_t c0 = transpose8x8(l01), c1 = transpose8x8(l23);
+                                mma(o[c][0][n], a0, c0, c1);
+                                mma(o[c][1][n], a1, c0, c1);
+                            }
+                        }
                     }
                 }
-            }
-            if (++stage == S::STAGES)
-                stage = 0;
-            if (++ahead == S::STAGES)
-                ahead = 0;
+            };
+            if (masked)
+                values(std::true_type());
+            else
+                values(std::false_type());
+            __syncwarp();
+            if (lane == 0)
+                umma::mbar_arrive(&empty[stage]);
+            if (++stage == STAGES)
+                stage = 0, phase ^= 1;
         }
 
-        // ------------------------------------------------ join the four warps
-        copy_wait<0>();
-        const float lower = float(int(top_scale >> 10) - 21);
+        // ------------------------------------------------ join the warps
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -673,56 +853,69 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
                 for (int o_ = 4; o_ < 32; o_ <<= 1)
                     l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o_);
                 if (g == 0) {
-                    stat[warp * ROWS + n * 8 + 2 * t + e] = m[n][e] + lower;
+                    stat[warp * ROWS + n * 8 + 2 * t + e] = reference[n][e];
                     stat[(WARPS + warp) * ROWS + n * 8 + 2 * t + e] = l[n][e];
                 }
             }
-        __syncthreads();  // every ring is idle: its memory takes the accumulators
-        float *const merge = reinterpret_cast<float *>(smem);
+        if (!consumers_all<CONSUMERS>(ok))
+            return;
+        // groups of SLOTS warps add their sums, relative to the largest reference of all, one group after the other
         constexpr float first = S::SUBNORMAL ? 0x1p24f : 1.0f, second = S::SUBNORMAL ? 0x1p20f : 1.0f;
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int round = 0; round < WARPS / S::SLOTS; round++) {
+            if (warp / S::SLOTS == round) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float *dst = merge + (warp * ROWS + n * 8 + 2 * t + e) * (D + 4) + 4 * g;
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int c = 0; c < NCH; c++)
-                    *reinterpret_cast<float4 *>(dst + 32 * c) =
-                        make_float4(o[c][0][n][e] * first, o[c][0][n][e + 2] * second, o[c][1][n][e] * first, o[c][1][n][e + 2] * second);
+                    for (int e = 0; e < 2; e++) {
+                        const int r = n * 8 + 2 * t + e;
+                        float most = NONE;
+#pragma unroll
+                        for (int w = 0; w < WARPS; w++)
+                            most = fmaxf(most, stat[w * ROWS + r]);
+                        const float f = exp2_approx(reference[n][e] - most), f1 = f * first, f2 = f * second;
+                        float *dst = merge + (warp % S::SLOTS * ROWS + r) * (D + 4) + 4 * g;
+#pragma unroll
+                        for (int c = 0; c < NCH; c++) {
+                            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (round > 0)
+                                v = *reinterpret_cast<float4 *>(dst + 32 * c);
+                            v.x = fmaf(o[c][0][n][e], f1, v.x), v.y = fmaf(o[c][0][n][e + 2], f2, v.y);
+                            v.z = fmaf(o[c][1][n][e], f1, v.z), v.w = fmaf(o[c][1][n][e + 2], f2, v.w);
+                            *reinterpret_cast<float4 *>(dst + 32 * c) = v;
+                        }
+                    }
             }
-        __syncthreads();
+            consumers_sync<CONSUMERS>();
+        }
         const bool whole = unit == 0 && units_here == seq.units;
         const int which = unit == 0 ? 1 : 0;  // a partial result that begins an item, or goes on with one
         float *const slot = a.partial + (int64_t(blockIdx.x) * 2 + which) * S::SLOT;
-        for (int i = tid; i < ROWS * (D / 4); i += WARPS * 32) {
+        for (int i = tid; i < rows * (D / 4); i += CONSUMERS) {
             const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-            if (r >= rows)
-                break;
-            float most = stat[r], weight[WARPS], sum = 0.0f;
+            float most = NONE, sum = 0.0f;
 #pragma unroll
-            for (int w = 1; w < WARPS; w++)
+            for (int w = 0; w < WARPS; w++)
                 most = fmaxf(most, stat[w * ROWS + r]);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < WARPS; w++) {
-                weight[w] = exp2_approx(stat[w * ROWS + r] - most);
-                sum = fmaf(weight[w], stat[(WARPS + w) * ROWS + r], sum);
+            for (int w = 0; w < WARPS; w++)
+                sum = fmaf(exp2_approx(stat[w * ROWS + r] - most), stat[(WARPS + w) * ROWS + r], sum);
+            float4 v = *reinterpret_cast<const float4 *>(merge + r * (D + 4) + d);
+#pragma unroll
+            for (int w = 1; w < S::SLOTS; w++) {
                 const float4 u = *reinterpret_cast<const float4 *>(merge + (w * ROWS + r) * (D + 4) + d);
-                v.x = fmaf(weight[w], u.x, v.x), v.y = fmaf(weight[w], u.y, v.y);
-                v.z = fmaf(weight[w], u.z, v.z), v.w = fmaf(weight[w], u.w, v.w);
+                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
             }
             if (whole) {
                 const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const int64_t row = row0 + r;
-                const int token = int(row / a.group);
+                const int row = row0 + r, token = row / a.group;
                 T *dst = static_cast<T *>(a.out) + int64_t(seq.first + token) * a.o_token +
-                         (int64_t(head) * a.group + (row - int64_t(token) * a.group)) * a.o_head + d;
-                if constexpr (sizeof(T) == 4) {
+                         (int64_t(head) * a.group + (row - token * a.group)) * a.o_head + d;
+                if constexpr (sizeof(T) == 4)
                     *reinterpret_cast<float4 *>(dst) = make_float4(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
-                } else {
+                else
                     *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_halves(v.x * inverse, v.y * inverse),
                                                                  pack_halves(v.z * inverse, v.w * inverse));
-                }
             } else {
                 *reinterpret_cast<float4 *>(slot + r * D + d) = v;
                 if (d == 0) {
@@ -734,20 +927,10 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT, PARTS>::CTAS) attenti
         if (!whole && which == 1 && tid == 0) {
             // the CTAs that hold the rest of this item: the last is the one with its last unit
             const int64_t last_unit = at - unit + seq.units - 1;
-            const int64_t last = ((last_unit + 1) * ctas - 1) / total;
-            a.meta[blockIdx.x] = make_int4(int(last) + 1 - int(blockIdx.x), b, tile, head);
+            a.meta[blockIdx.x] = make_int4(int(shares.holder(last_unit)) + 1 - int(blockIdx.x), b, tile, head);
         }
-        at += units_here;
-        if (at >= end)
+        if (!next_segment(units_here))
             break;
-        unit = 0;
-        if (++item == seq.tiles * a.kv_heads) {
-            item = 0;
-            do {
-                b++;
-                seq = sequence<ROWS>(a, b, false);
-            } while (seq.units == 0 || seq.tiles == 0);
-        }
     }
 }
 
@@ -766,8 +949,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_kv4_join_kernel(const 
     if (count == 0)
         return;
     const int first = a.cu[b], n = a.cu[b + 1] - first;
-    const int64_t row = int64_t(tile) * ROWS + r;
-    if (row >= int64_t(n) * a.group)
+    const int row = tile * ROWS + r;
+    if (row >= n * a.group)
         return;
     const int tid = threadIdx.x;
     auto part = [&](int i) { return a.partial + (int64_t(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * SLOT; };
@@ -808,9 +991,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_kv4_join_kernel(const 
         sum += group_sum[i];
     }
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int token = int(row / a.group);
+    const int token = row / a.group;
     T *dst = static_cast<T *>(a.out) + int64_t(first + token) * a.o_token +
-             (int64_t(head) * a.group + (row - int64_t(token) * a.group)) * a.o_head + 4 * lane;
+             (int64_t(head) * a.group + (row - token * a.group)) * a.o_head + 4 * lane;
     if constexpr (sizeof(T) == 4)
         *reinterpret_cast<float4 *>(dst) = make_float4(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
     else
@@ -822,7 +1005,7 @@ template <typename T, int D, int NT> int32_t launch(ovk_ctx *ctx, const Kv4Args 
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     using S = Shape<D, NT, PARTS>;
     OVK_CUDA(ctx, cudaFuncSetAttribute(attention_kv4_kernel<T, D, NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
-    attention_kv4_kernel<T, D, NT, PARTS><<<ctas, WARPS * 32, S::SMEM, ctx->stream>>>(a);
+    attention_kv4_kernel<T, D, NT, PARTS><<<ctas, S::THREADS, S::SMEM, ctx->stream>>>(a);
     OVK_LAUNCHED(ctx, NT == 1 ? "attention_kv4" : "attention_kv4_rows16");
     if (ctas > 1) {
         OVK_CUDA(ctx, ovk_launch_pdl(attention_kv4_join_kernel<T, D, S::ROWS>, dim3(unsigned(ctas - 1), S::ROWS), dim3(JOIN_THREADS), 0,
