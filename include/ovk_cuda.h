@@ -515,9 +515,9 @@ OVK_API int32_t ovk_qlinear_global_average_pool(ovk_ctx *ctx, const void *x, int
  *
  * Lengths and page numbers live on the device and cannot be refused before the
  * launch: a sequence, position or page outside what the call describes is left
- * out (its rows are written as zeros, or not stored to the cache), nothing
- * outside the tensors is touched, and the next ovk_flush returns
- * OVK_INVALID_ARGUMENT.
+ * out (rows of a sequence whose bounds make sense are written as zeros, others
+ * stay as they are, and nothing of it is stored to the cache), nothing outside
+ * the tensors is touched, and the next ovk_flush returns OVK_INVALID_ARGUMENT.
  *
  * Like every operator these only enqueue on the context's stream.  They keep no
  * state in the context, so calls on several contexts and replays of captured
@@ -593,7 +593,8 @@ OVK_API int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, const o
  * that brings more is left out as described above.
  * workspace: partial results of sequences that several CTAs share, 16-byte
  * aligned, ovk_attention_kv4_workspace() bytes; NULL takes the context's own
- * workspace, which grows on demand (bring one where the call is captured). */
+ * workspace, which grows on demand.  A call that is being captured into a graph
+ * has to bring one, which replays of other graphs must not use at the same time. */
 OVK_API int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, const ovk_kv4_batch *batch,
                                   const ovk_heads *q, const ovk_heads *out, int32_t dtype,
                                   int64_t max_tokens, float scale, int64_t window, void *workspace,
@@ -615,6 +616,7 @@ typedef struct ovk_prompt_params {
     int32_t dtype, causal;
     int64_t window;
     float scale;
+    int32_t max_q; /* the most queries a sequence has, 0: not known; one with more is left out */
 } ovk_prompt_params;
 OVK_API int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p, const ovk_heads *q,
                                      const ovk_heads *k, const ovk_heads *v, const int32_t *cu_q,

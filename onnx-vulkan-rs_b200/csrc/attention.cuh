@@ -20,6 +20,29 @@ struct DeviceGuard {
     }
 };
 
+// Lets a kernel use `bytes` of dynamic shared memory on this device: once per kernel and device, since the
+// call costs about as much as a launch.  Threads that ask at the same time set the same value.
+template <typename... A> static inline cudaError_t ovk_allow_smem(void (*kernel)(A...), size_t bytes, int device)
+{
+    struct Done {
+        void (*kernel)(A...);
+        uint64_t devices;
+    };
+    constexpr int MOST = 16;  // kernels of one signature
+    static thread_local Done done[MOST] = {};
+    for (int i = 0; i < MOST; i++) {
+        if (done[i].kernel == kernel || !done[i].kernel) {
+            if (device < 64 && done[i].kernel == kernel && (done[i].devices >> device & 1))
+                return cudaSuccess;
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+            if (e == cudaSuccess && device < 64)
+                done[i].kernel = kernel, done[i].devices |= uint64_t(1) << device;
+            return e;
+        }
+    }
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+}
+
 constexpr int64_t OVK_MAX_HEADS = 1 << 16;
 
 // A [tokens, heads, head_dim] tensor with contiguous heads; `what` names it in the message.  Strides

@@ -122,6 +122,11 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
                     "%s: a workspace of %zu bytes at %p, %zu are needed on a 16-byte boundary", op, workspace_bytes, workspace,
                     bytes_for(p, ctas));
     } else {
+        // the context's workspace would be shared by every graph captured from it
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        OVK_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+        OVK_REQUIRE(ctx, capture == cudaStreamCaptureStatusNone, "%s: a captured call needs a workspace of its own (%zu bytes)", op,
+                    bytes_for(p, ctas));
         rc = ovk_scratch(ctx, bytes_for(p, ctas), &workspace);
         if (rc != OVK_OK)
             return rc;

@@ -1004,7 +1004,7 @@ template <typename T, int D, int NT> int32_t launch(ovk_ctx *ctx, const Kv4Args 
 {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     using S = Shape<D, NT, PARTS>;
-    OVK_CUDA(ctx, cudaFuncSetAttribute(attention_kv4_kernel<T, D, NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    OVK_CUDA(ctx, ovk_allow_smem(attention_kv4_kernel<T, D, NT, PARTS>, S::SMEM, ctx->device));
     attention_kv4_kernel<T, D, NT, PARTS><<<ctas, S::THREADS, S::SMEM, ctx->stream>>>(a);
     OVK_LAUNCHED(ctx, NT == 1 ? "attention_kv4" : "attention_kv4_rows16");
     if (ctas > 1) {

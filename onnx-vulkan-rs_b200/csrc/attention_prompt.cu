@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(THREADS) attention_prompt_simt_kernel(const Pr
 template <typename T, int DMAX> int32_t launch_simt(ovk_ctx *ctx, const PromptArgs &a, unsigned tiles)
 {
     constexpr size_t smem = simt_smem<DMAX>();
-    OVK_CUDA(ctx, cudaFuncSetAttribute(attention_prompt_simt_kernel<T, DMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    OVK_CUDA(ctx, ovk_allow_smem(attention_prompt_simt_kernel<T, DMAX>, smem, ctx->device));
     attention_prompt_simt_kernel<T, DMAX><<<dim3(tiles, unsigned(a.heads)), THREADS, smem, ctx->stream>>>(a);
     OVK_LAUNCHED(ctx, sizeof(T) == 4 ? "attention_prompt_f32" : "attention_prompt_simt");
     return OVK_OK;
@@ -222,6 +222,7 @@ extern "C" int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p
     OVK_REQUIRE(ctx, p->q_tokens >= 0 && p->q_tokens < (int64_t(1) << 30) && p->k_tokens >= 0 && p->k_tokens < (int64_t(1) << 30) &&
                          p->batch >= 0 && p->batch < (1 << 24),
                 "%s: %lld query and %lld key rows of %lld sequences", op, (long long)p->q_tokens, (long long)p->k_tokens, (long long)p->batch);
+    OVK_REQUIRE(ctx, p->max_q >= 0, "%s: max_q %d", op, p->max_q);
     OVK_REQUIRE(ctx, p->window >= 0, "%s: window %lld", op, (long long)p->window);
     OVK_REQUIRE(ctx, p->scale - p->scale == 0.0f, "%s: scale is not finite", op);
     const size_t elem = ovk_elem_bytes(p->dtype);
@@ -252,9 +253,10 @@ extern "C" int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p
     a.q_tokens = int(p->q_tokens), a.k_tokens = int(p->k_tokens), a.batch = int(p->batch);
     a.heads = int(q->heads), a.group = int(q->heads / k->heads), a.head_dim = int(p->head_dim);
     a.causal = p->causal != 0, a.window = p->window, a.scale_log2e = p->scale * 1.4426950408889634f;
+    a.max_q = p->max_q;
     a.vec = ovk_rows_aligned(q, elem) && ovk_rows_aligned(k, elem) && ovk_rows_aligned(v, elem);
     a.status = ctx->dev_status;
-    const unsigned tiles = unsigned(ceil_div64(p->q_tokens, BM) + p->batch);
+    const unsigned tiles = unsigned(prompt_tiles(a, BM));
     if (p->dtype == OVK_FLOAT)
         return p->head_dim <= 64    ? launch_simt<float, 64>(ctx, a, tiles)
                : p->head_dim <= 128 ? launch_simt<float, 128>(ctx, a, tiles)

@@ -10,7 +10,7 @@ struct PromptArgs {
     int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
     const int32_t *cu_q, *cu_k;
     int q_tokens, k_tokens, batch, heads, group, head_dim;
-    int causal, vec;
+    int causal, vec, max_q;
     int64_t window;
     float scale_log2e;
     int *status;
@@ -40,7 +40,7 @@ template <int BM> __device__ __forceinline__ void find_prompt_tile(const PromptA
             first = a.cu_q[b];
             const int end = a.cu_q[b + 1];
             n = end - first;
-            if (first < 0 || end < first || end > a.q_tokens) {
+            if (first < 0 || end < first || end > a.q_tokens || (a.max_q > 0 && n > a.max_q)) {
                 n = 0;
                 if (index == 0)
                     atomicExch(a.status, OVK_DEV_BAD_SEQUENCE);
@@ -87,6 +87,13 @@ __device__ __forceinline__ KeyRange key_range(const PromptArgs &a, const PromptT
     return r;
 }
 #endif
+
+// Tiles of BM query rows that a batch may have.
+static inline int64_t prompt_tiles(const PromptArgs &a, int64_t bm)
+{
+    const int64_t by_rows = ceil_div64(a.q_tokens, bm) + a.batch;
+    return a.max_q > 0 ? std::min(by_rows, a.batch * ceil_div64(a.max_q, bm)) : by_rows;
+}
 
 // f16 on the tensor cores; *taken says whether the call's layout is one it takes
 int32_t ovk_prompt_tc(ovk_ctx *ctx, const PromptArgs &a, bool *taken);

@@ -308,35 +308,34 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                     const int stage = n % C::STAGES;
                     ok = wait(&sh.raw[stage], (raw_phase >> stage) & 1, dead, status, OVK_DEV_TIMEOUT_TMA);
                     raw_phase ^= 1u << stage;
-                    constexpr int KEYS = BN / CH, WORDS = KEYS * DP / 8;  // 16-byte words of the chunk
-                    const int left = key_end - (key_begin + i * BN + c * KEYS);  // keys before the end
-                    uint4 *const words = reinterpret_cast<uint4 *>(ring + stage * C::STAGE);
-                    for (int at = (role - 2) * 32 + lane; at < WORDS && ok; at += 64) {
-                        const int row = (at >> 3) % KEYS;
-                        if (row >= left) {
-                            words[at] = make_uint4(0, 0, 0, 0);
-                            continue;
-                        }
-                        const uint4 v = words[at];
-                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+                    // in each 128-byte column the chunk's rows lie one after the other, eight 16-byte words a row
+                    constexpr int KEYS = BN / CH;
+                    const int left = min(KEYS, max(0, key_end - (key_begin + i * BN + c * KEYS)));  // rows before the end
+                    const int self = (role - 2) * 32 + lane;
+                    for (int x = 0; x < C::ATOMS && ok; x++) {
+                        uint4 *const words = reinterpret_cast<uint4 *>(ring + stage * C::STAGE) + x * KEYS * 8;
                         uint32_t bad = 0;
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            bad |= (u[e] & 0x7c007c00u) + 0x04000400u;  // carries into the sign bit for an exponent of ones
-                        if (bad & 0x80008000u) {
-                            const int atom = at / (KEYS * 8), col = atom * 64 + (((at & 7) ^ (row & 7)) << 3);
-                            uint32_t z[4];
-                            for (int e = 0; e < 4; e++) {
-                                z[e] = u[e];
-                                if ((u[e] & 0x7c00u) == 0x7c00u) {
-                                    z[e] &= 0xffff0000u;
-                                    atomicOr(&sh.odd[(col + 2 * e) >> 5], 1u << ((col + 2 * e) & 31));
-                                }
-                                if ((u[e] & 0x7c000000u) == 0x7c000000u) {
-                                    z[e] &= 0x0000ffffu;
-                                    atomicOr(&sh.odd[(col + 2 * e + 1) >> 5], 1u << ((col + 2 * e + 1) & 31));
-                                }
+                        for (int k = 0; k < KEYS * 8 / 64; k++) {
+                            const int at = self + 64 * k;
+                            if (at < left * 8) {
+                                const uint4 v = words[at];  // a carry into the sign bit marks an exponent of ones
+                                bad |= ((v.x & 0x7c007c00u) + 0x04000400u) | ((v.y & 0x7c007c00u) + 0x04000400u) |
+                                       ((v.z & 0x7c007c00u) + 0x04000400u) | ((v.w & 0x7c007c00u) + 0x04000400u);
+                            } else {
+                                words[at] = make_uint4(0, 0, 0, 0);
                             }
+                        }
+                        if (!(bad & 0x80008000u))
+                            continue;
+                        for (int at = self; at < left * 8; at += 64) {
+                            const int col = x * 64 + (((at & 7) ^ ((at >> 3) & 7)) << 3);  // of the word's first element
+                            uint32_t z[4] = {words[at].x, words[at].y, words[at].z, words[at].w};
+                            for (int e = 0; e < 8; e++)
+                                if ((z[e >> 1] >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u) {
+                                    z[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+                                    atomicOr(&sh.odd[(col + e) >> 5], 1u << ((col + e) & 31));
+                                }
                             words[at] = make_uint4(z[0], z[1], z[2], z[3]);
                         }
                     }
@@ -564,10 +563,10 @@ template <int DP> int32_t launch(ovk_ctx *ctx, const PromptArgs &a, bool *taken)
     p.window = a.window >= (int64_t(1) << 30) ? 0 : int(a.window);
     p.vec_out = aligned_to(a.out, 16) && a.o_token % 8 == 0 && a.o_head % 8 == 0;
     const int64_t rows = C::NS == 2 && !p.by_heads ? 2 * BM : BM;
-    const int64_t grid = (ceil_div64(a.q_tokens, rows) + a.batch) * p.pairs;
+    const int64_t grid = prompt_tiles(a, rows) * p.pairs;
     if (grid >= (int64_t(1) << 31))
         return OVK_OK;
-    OVK_CUDA(ctx, cudaFuncSetAttribute(attention_prompt_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    OVK_CUDA(ctx, ovk_allow_smem(attention_prompt_tc_kernel<DP>, C::SMEM, ctx->device));
     attention_prompt_tc_kernel<DP><<<unsigned(grid), C::THREADS, C::SMEM, ctx->stream>>>(q, k, v, p);
     *taken = true;
     OVK_LAUNCHED(ctx, "attention_prompt_tc");

@@ -14,7 +14,9 @@ The wrappers mirror the reference's operator functions
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
+import struct
 
 FLOAT, UINT8, INT8, INT32, INT64, FLOAT16 = 1, 2, 3, 6, 7, 10
 OK, INVALID_ARGUMENT, UNSUPPORTED, BACKEND, TIMEOUT = 0, 1, 2, 3, 4
@@ -61,7 +63,62 @@ class KV4Batch(C.Structure):
 
 class PromptParams(C.Structure):
     _fields_ = [("q_tokens", C.c_int64), ("k_tokens", C.c_int64), ("batch", C.c_int64), ("head_dim", C.c_int64),
-                ("dtype", C.c_int32), ("causal", C.c_int32), ("window", C.c_int64), ("scale", C.c_float)]
+                ("dtype", C.c_int32), ("causal", C.c_int32), ("window", C.c_int64), ("scale", C.c_float), ("max_q", C.c_int32)]
+
+
+# the same structs as packed bytes
+_PACK_HEADS, _PACK_HEADS2 = struct.Struct("@Pqqq").pack, struct.Struct("@PqqqPqqq").pack
+_PACK_ROTARY = struct.Struct("@qqqqiiiiiiiii4x").pack
+_PACK_BATCH = struct.Struct("@qqqPPP").pack
+_PACK_PROMPT = struct.Struct("@qqqqiiqfi").pack
+
+
+@functools.cache
+def _activation_codes() -> dict:
+    import torch
+    return {torch.float32: FLOAT, torch.float16: FLOAT16}
+
+
+@functools.cache
+def _index_codes() -> dict:
+    import torch
+    return {torch.int64: INT64, torch.int32: INT32}
+
+
+@functools.cache
+def _int32() -> tuple:
+    import torch
+    return (torch.int32,)
+
+
+@functools.cache
+def _raw_stream():
+    """device -> the handle of torch's current stream there."""
+    import torch
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+@functools.cache
+def _capturing():
+    import torch
+    return torch.cuda.is_current_stream_capturing
+
+
+class _PackedCalls:
+    """The attention entry points with their structs as addresses or bytes."""
+
+    def __init__(self):
+        for name in ("ovk_rotary", "ovk_kv4_append", "ovk_attention_kv4", "ovk_attention_prompt"):
+            fn = lib()[name]
+            fn.restype = SIGNATURES[name][0]
+            fn.argtypes = [_P if hasattr(t, "_type_") and isinstance(t._type_, type) and issubclass(t._type_, C.Structure) else t
+                           for t in SIGNATURES[name][1]]
+            setattr(self, name, fn)
+
+
+@functools.cache
+def _packed_calls() -> _PackedCalls:
+    return _PackedCalls()
 
 
 _lib = None
@@ -200,7 +257,7 @@ class Context:
         self.h = h
         self.device = device
         self._stream = lib().ovk_stream(h)
-        self._kv4_workspace = {}  # (cache shape, query heads, most new tokens, type) -> bytes
+        self._fast = _packed_calls()
 
     def check(self, rc: int):
         if rc:
@@ -562,154 +619,179 @@ class Context:
         return out
 
     # -------------------------------------------- the attention of a decoder layer
+    # A decode step makes a few of these calls per layer, each a few microseconds of GPU time, so the wrappers check with
+    # few attribute reads and hand the C structs over as packed bytes.
     def _activation(self, what, t, tokens=None, heads=None, head_dim=None, dtype=None):
-        """A [tokens, heads, head_dim] tensor whose heads are contiguous, as the C struct; a slice of a wider one will do."""
-        import torch
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.device.index == self.device):
-            raise OvkError(INVALID_ARGUMENT, f"{what}: a tensor on cuda:{self.device} is needed")
-        if t.dim() != 3 or t.dtype not in (torch.float32, torch.float16):
-            raise OvkError(INVALID_ARGUMENT, f"{what}: [tokens, heads, head_dim] of float32 or float16 is needed, not "
-                                             f"{tuple(t.shape)} of {t.dtype}")
-        n, h, d = t.shape
-        if (tokens is not None and n != tokens) or (heads is not None and h != heads) or (head_dim is not None and d != head_dim) \
-                or (dtype is not None and t.dtype != dtype):
-            raise OvkError(INVALID_ARGUMENT, f"{what}: {tuple(t.shape)} of {t.dtype} does not fit [{tokens or n}, {heads or h}, "
-                                             f"{head_dim or d}] of {dtype or t.dtype}")
-        st, sh, sd = t.stride()
-        if sd != 1 and d != 1:
-            raise OvkError(INVALID_ARGUMENT, f"{what}: the elements of a head must be contiguous (strides {t.stride()})")
-        return Heads(t.data_ptr(), h, st, sh)
+        """(data, heads, token stride, head stride) of a [tokens, heads, head_dim] tensor whose heads are contiguous; a slice
+        of a wider one will do."""
+        try:
+            n, h, d = t.shape
+            st, sh, sd = t.stride()
+            if ((sd == 1 or d == 1) and t.get_device() == self.device and t.dtype in _activation_codes()
+                    and (tokens is None or n == tokens) and (heads is None or h == heads) and (head_dim is None or d == head_dim)
+                    and (dtype is None or t.dtype is dtype)):
+                return t.data_ptr(), h, st, sh
+        except (AttributeError, TypeError, ValueError):
+            pass
+        got = f"{list(t.shape)} of {t.dtype} on {t.device} with strides {t.stride()}" if hasattr(t, "stride") else f"{type(t).__name__}"
+        raise OvkError(INVALID_ARGUMENT, f"{what}: [{tokens if tokens is not None else 'tokens'}, {heads or 'heads'}, {head_dim or 'head_dim'}] of "
+                                         f"{dtype or 'float32 or float16'} on cuda:{self.device} with contiguous heads is needed, not {got}")
 
     def _indices(self, what, t, shape, dtypes):
-        import torch
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.device.index == self.device and t.is_contiguous()) \
-                or t.dtype not in dtypes or tuple(t.shape) != tuple(shape):
-            raise OvkError(INVALID_ARGUMENT, f"{what}: a contiguous {list(shape)} tensor of {' or '.join(str(d) for d in dtypes)} on "
-                                             f"cuda:{self.device} is needed")
-        return t.data_ptr()
+        try:
+            if t.shape == shape and t.dtype in dtypes and t.is_contiguous() and t.get_device() == self.device:
+                return t.data_ptr()
+        except AttributeError:
+            pass
+        got = f"{list(t.shape)} of {t.dtype} on {t.device}" if hasattr(t, "stride") else f"{type(t).__name__}"
+        raise OvkError(INVALID_ARGUMENT, f"{what}: a contiguous {list(shape)} tensor of {' or '.join(str(d) for d in dtypes)} on "
+                                         f"cuda:{self.device} is needed, not {got}")
 
-    def _on_stream(self, used, make):
-        """Runs `make` (allocations) for work on this context's stream.  Where that is not torch's current stream the new
-        tensors come from its pool, and those the call reads are kept until it has passed them."""
+    def _foreign_stream(self):
+        """None where torch's current stream is this context's, else the latter as a torch stream."""
+        if (_raw_stream()(self.device) or 1) == self._stream:
+            return None
         import torch
-        if (torch.cuda.current_stream(self.device).cuda_stream or 1) == self._stream:
-            return make()
-        stream = torch.cuda.ExternalStream(self._stream, device=torch.device("cuda", self.device))
-        for t in used:
-            if t is not None:
-                t.record_stream(stream)
+        return torch.cuda.ExternalStream(self._stream, device=torch.device("cuda", self.device))
+
+    @staticmethod
+    def _new(like, stream):
+        """A contiguous tensor of this shape and type, from the pool of the stream that will write it."""
+        import torch
+        if stream is None:
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
         with torch.cuda.stream(stream):
-            return make()
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
+
+    @staticmethod
+    def _keep(stream, *used):
+        """Tensors that a call on another stream reads or writes are not reused before it has passed them."""
+        if stream is not None:
+            for t in used:
+                if t is not None:
+                    t.record_stream(stream)
 
     def rotary(self, q, cos, sin, positions, k=None, sections=None, interleaved=False, out=None, k_out=None):
         """Rotary positions of q (and k) [tokens, heads, head_dim]: cos and sin are [positions, rotary_dim / 2] tables,
         positions [tokens] or [axes, tokens], sections the pairs of each axis.  Returns q (and k) turned; out may be q."""
-        import torch
-        n, _, d = q.shape if q.dim() == 3 else (0, 0, 0)
-        x = (Heads * 2)(self._activation("Rotary: q", q))
-        if k is not None:
-            x[1] = self._activation("Rotary: k", k, n, None, d, q.dtype)
-        pairs = cos.shape[-1]
+        x = self._activation("Rotary: q", q)
+        n, h, d = q.shape
+        kind = q.dtype
+        rows, pairs = cos.shape if cos.dim() == 2 else (0, 0)
         axes = 1 if positions.dim() == 1 else positions.shape[0]
-        at = self._indices("Rotary: positions", positions, (n,) if positions.dim() == 1 else (axes, n), (torch.int64, torch.int32))
-        tables = [self._indices(f"Rotary: {c}", t, (cos.shape[0], pairs), (torch.float32, torch.float16)) for c, t in
-                  (("cos", cos), ("sin", sin))]
-        if cos.dtype != sin.dtype:
-            raise OvkError(INVALID_ARGUMENT, "Rotary: tables of two types")
-        sections = [pairs] if sections is None else [int(v) for v in sections]
+        codes = _activation_codes()
+        at = self._indices("Rotary: positions", positions, (n,) if positions.dim() == 1 else (axes, n), _index_codes())
+        c = self._indices("Rotary: cos", cos, (rows, pairs), codes)
+        s = self._indices("Rotary: sin", sin, (rows, pairs), (cos.dtype,))
+        if sections is None:
+            sections = (pairs,)
         if len(sections) != axes or axes > 4:
             raise OvkError(INVALID_ARGUMENT, f"Rotary: {len(sections)} sections for {axes} axes (1 to 4)")
-        if out is None or (k is not None and k_out is None):
-            def make():
-                return (torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out,
-                        torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None and k_out is None else k_out)
-            out, k_out = self._on_stream((q, k, cos, sin, positions, out, k_out), make)
-        else:
-            self._on_stream((q, k, cos, sin, positions, out, k_out), lambda: None)
-        y = (Heads * 2)(self._activation("Rotary: out", out, n, q.shape[1], d, q.dtype))
+        stream = self._foreign_stream()
         if k is not None:
-            y[1] = self._activation("Rotary: k_out", k_out, n, k.shape[1], d, q.dtype)
-        p = RotaryParams(n, d, 2 * pairs, cos.shape[0], FLOAT if q.dtype == torch.float32 else FLOAT16,
-                         FLOAT if cos.dtype == torch.float32 else FLOAT16, INT64 if positions.dtype == torch.int64 else INT32,
-                         int(interleaved), axes, (C.c_int32 * 4)(*sections))
-        self.check(lib().ovk_rotary(self.h, p, 1 if k is None else 2, x, y, at, *tables))
-        return out if k is None else (out, k_out)
+            x += self._activation("Rotary: k", k, n, None, d, kind)
+            if k_out is None:
+                k_out = self._new(k, stream)
+            y_k = self._activation("Rotary: k_out", k_out, n, x[5], d, kind)
+        if out is None:
+            out = self._new(q, stream)
+        y = self._activation("Rotary: out", out, n, h, d, kind)
+        self._keep(stream, q, k, cos, sin, positions, out, k_out)
+        p = _PACK_ROTARY(n, d, 2 * pairs, rows, codes[kind], codes[cos.dtype], _index_codes()[positions.dtype], 1 if interleaved else 0, axes,
+                         *sections, *(0,) * (4 - axes))
+        if k is None:
+            self.check(self._fast.ovk_rotary(self.h, p, 1, _PACK_HEADS(*x), _PACK_HEADS(*y), at, c, s))
+            return out
+        self.check(self._fast.ovk_rotary(self.h, p, 2, _PACK_HEADS2(*x), _PACK_HEADS2(*y, *y_k), at, c, s))
+        return out, k_out
 
     def kv4_cache(self, pages, kv_heads, page_size, head_dim, block_size=32, zero_points=True):
         """An empty paged 4-bit cache; with pages = batch and a block table of one column, a [batch, kv_heads, capacity] one."""
         import torch
         blocks = head_dim // block_size if block_size else 0
-        device = torch.device("cuda", self.device)
-        code = lambda: torch.zeros((pages, kv_heads, page_size, head_dim // 2), dtype=torch.uint8, device=device)  # noqa: E731
-        scale = lambda: torch.zeros((pages, kv_heads, page_size, blocks), dtype=torch.float16, device=device)  # noqa: E731
-        zero = lambda: torch.zeros((pages, kv_heads, page_size, (blocks + 1) // 2), dtype=torch.uint8,  # noqa: E731
-                                   device=device) if zero_points else None
-        return self._on_stream((), lambda: KV4Cache(code(), code(), scale(), scale(), zero(), zero()))
+        zeros = lambda last, dtype: torch.zeros((pages, kv_heads, page_size, last), dtype=dtype, device=torch.device("cuda", self.device))  # noqa: E731
+
+        def make():
+            code = [zeros(head_dim // 2, torch.uint8) for _ in range(2)]
+            scale = [zeros(blocks, torch.float16) for _ in range(2)]
+            zero = [zeros((blocks + 1) // 2, torch.uint8) if zero_points else None for _ in range(2)]
+            return KV4Cache(*code, *scale, *zero)
+        stream = self._foreign_stream()
+        if stream is None:
+            return make()
+        with torch.cuda.stream(stream):
+            return make()
 
     def _kv4_batch(self, what, cache, tokens, block_table, cu_tokens, lens):
-        import torch
-        if cache.k.device.index != self.device:
-            raise OvkError(INVALID_ARGUMENT, f"{what}: the cache is not on cuda:{self.device}")
+        if cache.device != self.device:
+            raise OvkError(INVALID_ARGUMENT, f"{what}: the cache is on cuda:{cache.device}, the context on cuda:{self.device}")
         batch = lens.shape[0] if lens.dim() == 1 else -1
-        i32 = (torch.int32,)
         pages = block_table.shape[1] if block_table.dim() == 2 else -1
-        return KV4Batch(tokens, batch, pages, self._indices(f"{what}: cu_tokens", cu_tokens, (batch + 1,), i32),
-                        self._indices(f"{what}: lens", lens, (batch,), i32),
-                        self._indices(f"{what}: block_table", block_table, (batch, pages), i32))
+        i32 = _int32()
+        return _PACK_BATCH(tokens, batch, pages, self._indices(what + ": cu_tokens", cu_tokens, (batch + 1,), i32),
+                           self._indices(what + ": lens", lens, (batch,), i32),
+                           self._indices(what + ": block_table", block_table, (batch, pages), i32))
 
     def kv4_append(self, cache: "KV4Cache", k, v, block_table, cu_tokens, lens):
         """Rounds the new tokens' keys and values [tokens, kv_heads, head_dim] to 4 bits and writes them: sequence b brings rows
-        cu_tokens[b] .. cu_tokens[b + 1] - 1, its last lens[b] .. positions; block_table is [batch, max_pages]."""
+        cu_tokens[b] .. cu_tokens[b + 1] - 1, the last of its lens[b] positions; block_table is [batch, max_pages]."""
         hk = self._activation("KV4Append: k", k, None, cache.kv_heads, cache.head_dim)
-        hv = self._activation("KV4Append: v", v, k.shape[0], cache.kv_heads, cache.head_dim, k.dtype)
-        b = self._kv4_batch("KV4Append", cache, k.shape[0], block_table, cu_tokens, lens)
-        self._on_stream((k, v, block_table, cu_tokens, lens, *cache.tensors), lambda: None)
-        self.check(lib().ovk_kv4_append(self.h, cache.params, b, hk, hv, _dtype_code(k)))
+        n = k.shape[0]
+        hv = self._activation("KV4Append: v", v, n, cache.kv_heads, cache.head_dim, k.dtype)
+        b = self._kv4_batch("KV4Append", cache, n, block_table, cu_tokens, lens)
+        stream = self._foreign_stream()
+        if stream is not None:
+            self._keep(stream, k, v, block_table, cu_tokens, lens, *cache.tensors)
+        self.check(self._fast.ovk_kv4_append(self.h, cache.packed, b, _PACK_HEADS(*hk), _PACK_HEADS(*hv), _activation_codes()[k.dtype]))
 
     def attention_kv4(self, cache: "KV4Cache", q, block_table, cu_tokens, lens, max_tokens=1, scale=None, window=0, out=None):
         """Causal attention of the new tokens q [tokens, q_heads, head_dim] over the cache, which holds their own rows already.
         max_tokens: the most new tokens a sequence brings; scale: 1 / sqrt(head_dim) unless given; window: positions a
         token reads, its own included (0: all before it)."""
-        import torch
         hq = self._activation("AttentionKV4: q", q, None, None, cache.head_dim)
-        b = self._kv4_batch("AttentionKV4", cache, q.shape[0], block_table, cu_tokens, lens)
-        code = _dtype_code(q)
-        key = (cache.shape, q.shape[1], max_tokens, code)
-        need = self._kv4_workspace.get(key)
-        if need is None:
-            n = _SZ()
-            self.check(lib().ovk_attention_kv4_workspace(self.h, cache.params, q.shape[1], max_tokens, code, C.byref(n)))
-            need = self._kv4_workspace[key] = n.value
-
-        def make():
-            return (torch.empty(need, dtype=torch.uint8, device=q.device),
-                    torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out)
-        space, out = self._on_stream((q, block_table, cu_tokens, lens, out, *cache.tensors), make)
-        ho = self._activation("AttentionKV4: out", out, *q.shape, q.dtype)
-        self.check(lib().ovk_attention_kv4(self.h, cache.params, b, hq, ho, code, max_tokens,
-                                           cache.head_dim ** -0.5 if scale is None else scale, window, space.data_ptr(), need))
+        n, h, d = q.shape
+        b = self._kv4_batch("AttentionKV4", cache, n, block_table, cu_tokens, lens)
+        code = _activation_codes()[q.dtype]
+        stream = self._foreign_stream()
+        if out is None:
+            out = self._new(q, stream)
+        ho = self._activation("AttentionKV4: out", out, n, h, d, q.dtype)
+        space, need = None, 0
+        if stream is not None:
+            self._keep(stream, q, block_table, cu_tokens, lens, out, *cache.tensors)
+        elif _capturing()():
+            # a graph has a workspace of its own (outside of one, calls on the stream follow each other in the context's)
+            import torch
+            size = _SZ()
+            self.check(lib().ovk_attention_kv4_workspace(self.h, cache.params, h, max_tokens, code, C.byref(size)))
+            need = size.value
+            space = torch.empty(need, dtype=torch.uint8, device=q.device)
+        self.check(self._fast.ovk_attention_kv4(self.h, cache.packed, b, _PACK_HEADS(*hq), _PACK_HEADS(*ho), code, max_tokens,
+                                                cache.head_dim ** -0.5 if scale is None else scale, window,
+                                                None if space is None else space.data_ptr(), need))
         return out
 
-    def attention_prompt(self, q, k, v, cu_q, max_q=None, cu_k=None, scale=None, causal=True, window=0, out=None):
+    def attention_prompt(self, q, k, v, cu_q, max_q=0, cu_k=None, scale=None, causal=True, window=0, out=None):
         """Attention within packed sequences: q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim], cu_q the
         sequences' first rows.  With cu_k the keys have rows of their own and the queries are the last tokens of the keys'
-        sequence.  max_q (the longest sequence's queries) is accepted for callers that have it; the lengths are read on
-        the device."""
-        import torch
+        sequence.  max_q: the most queries a sequence has, where the caller knows it (0: not known; rows beyond it are
+        left out)."""
         hq = self._activation("AttentionPrompt: q", q)
-        hk = self._activation("AttentionPrompt: k", k, None, None, q.shape[2], q.dtype)
-        hv = self._activation("AttentionPrompt: v", v, k.shape[0], k.shape[1], q.shape[2], q.dtype)
-        batch = cu_q.shape[0] - 1
-        pq = self._indices("AttentionPrompt: cu_q", cu_q, (batch + 1,), (torch.int32,))
-        if batch < 0:
-            raise OvkError(INVALID_ARGUMENT, "AttentionPrompt: cu_q is empty")
-        pk = pq if cu_k is None or cu_k is cu_q else self._indices("AttentionPrompt: cu_k", cu_k, (batch + 1,), (torch.int32,))
-        used = (q, k, v, cu_q, cu_k, out)
-        out = self._on_stream(used, lambda: torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out)
-        ho = self._activation("AttentionPrompt: out", out, *q.shape, q.dtype)
-        p = PromptParams(q.shape[0], k.shape[0], batch, q.shape[2], _dtype_code(q), int(causal), window,
-                         q.shape[2] ** -0.5 if scale is None else scale)
-        self.check(lib().ovk_attention_prompt(self.h, p, hq, hk, hv, pq, pk, ho))
+        n, h, d = q.shape
+        kind = q.dtype
+        hk = self._activation("AttentionPrompt: k", k, None, None, d, kind)
+        hv = self._activation("AttentionPrompt: v", v, k.shape[0], k.shape[1], d, kind)
+        batch = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
+        pq = self._indices("AttentionPrompt: cu_q", cu_q, (max(batch, 0) + 1,), _int32())
+        pk = pq if cu_k is None or cu_k is cu_q else self._indices("AttentionPrompt: cu_k", cu_k, (batch + 1,), _int32())
+        stream = self._foreign_stream()
+        if out is None:
+            out = self._new(q, stream)
+        ho = self._activation("AttentionPrompt: out", out, n, h, d, kind)
+        self._keep(stream, q, k, v, cu_q, cu_k, out)
+        p = _PACK_PROMPT(n, k.shape[0], batch, d, _activation_codes()[kind], 1 if causal else 0, window, d ** -0.5 if scale is None else scale,
+                         int(max_q or 0))
+        self.check(self._fast.ovk_attention_prompt(self.h, p, _PACK_HEADS(*hq), _PACK_HEADS(*hk), _PACK_HEADS(*hv), pq, pk, _PACK_HEADS(*ho)))
         return out
 
     # ------------------------------------ the QOperator chain around QLinearConv
@@ -802,9 +884,10 @@ class KV4Cache:
         if self.head_dim % blocks:
             raise OvkError(INVALID_ARGUMENT, f"KV4Cache: {blocks} scales for {self.head_dim} elements")
         self.block_size = self.head_dim // blocks
-        self.shape = (pages, heads, size, self.head_dim, self.block_size)
+        self.device = k.get_device()
         self.params = KV4CacheParams(*[None if t is None else t.data_ptr() for t in (k, v, k_scales, v_scales, k_zero_points, v_zero_points)],
                                      pages, heads, size, self.head_dim, self.block_size)
+        self.packed = bytes(self.params)
 
 
 class NBitsWeight:

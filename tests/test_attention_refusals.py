@@ -133,7 +133,7 @@ def test_attention_kv4(changes, status, word):
 
 
 def prompt(q=None, k=None, v=None, out=None, cu_q=BASE, cu_k=BASE, **changes):
-    fields = dict(q_tokens=5, k_tokens=5, batch=2, head_dim=64, dtype=FLOAT16, causal=1, window=0, scale=0.1) | changes
+    fields = dict(q_tokens=5, k_tokens=5, batch=2, head_dim=64, dtype=FLOAT16, causal=1, window=0, scale=0.1, max_q=0) | changes
     q, k, v, out = q or heads(4), k or heads(2), v or heads(2), out or heads(4, at=2 * BASE)
     return outcome(ovk_b200.lib().ovk_attention_prompt(None, PromptParams(**fields), q, k, v, cu_q, cu_k, out))
 
@@ -141,7 +141,7 @@ def prompt(q=None, k=None, v=None, out=None, cu_q=BASE, cu_k=BASE, **changes):
 @pytest.mark.parametrize("changes,status,word", [
     ({}, INVALID_ARGUMENT, "null context"), ({"dtype": 16}, UNSUPPORTED, "dtype"), ({"head_dim": 0}, UNSUPPORTED, "head_dim"),
     ({"head_dim": 257}, UNSUPPORTED, "head_dim"), ({"q_tokens": -1}, INVALID_ARGUMENT, "rows"), ({"batch": -1}, INVALID_ARGUMENT, "sequences"),
-    ({"window": -2}, INVALID_ARGUMENT, "window"), ({"scale": float("-inf")}, INVALID_ARGUMENT, "scale"), ({"q": heads(5)}, INVALID_ARGUMENT, "heads"),
+    ({"window": -2}, INVALID_ARGUMENT, "window"), ({"max_q": -1}, INVALID_ARGUMENT, "max_q"), ({"scale": float("-inf")}, INVALID_ARGUMENT, "scale"), ({"q": heads(5)}, INVALID_ARGUMENT, "heads"),
     ({"v": heads(1)}, INVALID_ARGUMENT, "heads"), ({"out": heads(2, at=2 * BASE)}, INVALID_ARGUMENT, "heads"),
     ({"out": heads(4, at=2 * BASE, token=64)}, INVALID_ARGUMENT, "overlap"), ({"cu_q": None}, INVALID_ARGUMENT, "bounds"),
     ({"cu_k": BASE + 1}, INVALID_ARGUMENT, "bounds"), ({"k": heads(2, at=None)}, INVALID_ARGUMENT, "no data"),
@@ -171,3 +171,12 @@ def test_cache_object_checks_its_tensors():
         ovk_b200.KV4Cache(code, code, scale, scale, code)
     with pytest.raises(ovk_b200.OvkError):
         ovk_b200.KV4Cache(code[0], code, scale, scale)
+
+
+def test_packed_structs_are_the_declared_ones():
+    """The wrappers hand structs over as packed bytes: same size and same fields as the ctypes declarations."""
+    assert ovk_b200._PACK_HEADS(1, 2, 3, 4) == bytes(Heads(1, 2, 3, 4))
+    assert ovk_b200._PACK_HEADS2(1, 2, 3, 4, 5, 6, 7, 8) == bytes((Heads * 2)(Heads(1, 2, 3, 4), Heads(5, 6, 7, 8)))
+    assert ovk_b200._PACK_ROTARY(*range(1, 14)) == bytes(RotaryParams(*range(1, 10), (C.c_int32 * 4)(10, 11, 12, 13)))
+    assert ovk_b200._PACK_BATCH(*range(1, 7)) == bytes(KV4Batch(*range(1, 7)))
+    assert ovk_b200._PACK_PROMPT(1, 2, 3, 4, 5, 6, 7, 8.5, 9) == bytes(PromptParams(1, 2, 3, 4, 5, 6, 7, 8.5, 9))
