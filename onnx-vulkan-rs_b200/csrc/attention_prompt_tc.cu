@@ -8,19 +8,24 @@
 // a cycle and SM: at head_dim 128 both pipes need the same 1024 cycles a tile, so
 // the point of the layout is that neither waits for the other.
 //
-//   warp 0 of the control group    TMA: Q once, then K and V tiles into one ring in
-//                                  the order the products use them
-//   warp 1                         issues every tcgen05.mma from one thread
-//   warps 2, 3                     guard V tiles that some row of the block does
-//                                  not read entirely (below)
 //   softmax groups of four warps   a thread owns a row: tcgen05.ld, maximum, exp2,
 //                                  tcgen05.st, and at the end its row of the result
+//   control group: warp 0          TMA: Q once, then K and V tiles into one ring in
+//                                  the order the products use them
+//                  warps 1, 2      issue tcgen05.mma, one thread each
+//   guards                         look through V tiles that some row of the block
+//                                  does not read entirely (below): warp 3 of the
+//                                  control group, or a group of their own
 //
 // Up to 128 elements a head two independent query tiles share each K and V tile
-// (two heads of a group, or neighbouring rows where the group is odd): while one
-// tile's softmax runs, the tensor core works for the other.  256-wide heads fill
-// tensor memory with one tile's O, so there one tile has two S buffers, and the
-// next scores are computed before the last weights are used.
+// (two heads of a group, or neighbouring rows where the group is odd), each with
+// its own issuing thread: while one tile's softmax runs, the tensor core works for
+// the other.  (The core's queue is short - a thread that issues runs at the core's
+// pace - and a wait costs some 300 cycles even where nothing is to be waited for:
+// one thread for both tiles left the core idle for half of the time, 308 us for
+// 8192 tokens of 16 heads.)  256-wide heads fill tensor memory with one tile's O, so
+// there one tile has two S buffers, one thread issues Q K^T and the other P V, and
+// the next scores are computed before the last weights are used.
 //
 // The reference m moves only when a row's maximum passes it by 2^8 (P is then at
 // most 256, sums are f32), so O is rarely rescaled; the softmax group does it
@@ -35,18 +40,20 @@
 
 namespace {
 
-constexpr int BM = 128, BN = 128;
+constexpr int BM = 128;
 
 template <int DP_> struct Tc {
     static constexpr int DP = DP_;                       // head_dim rounded up; TMA fills the rest with zeros
     static constexpr int NS = DP == 256 ? 1 : 2;         // query tiles of a block
-    static constexpr int SB = DP == 256 ? 2 : 1;         // S buffers of a tile
+    static constexpr int BN = DP == 256 ? 128 : 64;      // keys of a tile; each query tile has two S buffers of as many columns
     static constexpr int CH = DP == 256 ? 2 : 1;         // ring stages of a K or V tile
     static constexpr int ATOMS = DP / 64;                // 128-byte columns of a row
     static constexpr int Q_BYTES = BM * DP * 2;
     static constexpr int STAGE = BN * DP * 2 / CH;
-    static constexpr int STAGES = 5;
-    static constexpr int THREADS = NS * 128 + 128;
+    static constexpr int STAGES = DP == 256 ? 5 : 10;
+    static constexpr int GUARDS = NS == 2 ? 1 : 4;       // warps
+    static constexpr int THREADS = 384;
+    static constexpr int SOFTMAX_REGS = NS == 2 ? 208 : 232, OTHER_REGS = NS == 2 ? 88 : 104;
     static constexpr int SMEM = NS * Q_BYTES + STAGES * STAGE + 1024;
     static constexpr int O_COL = 256;                    // S of the two tiles (or buffers) at 0 and 128
 };
@@ -59,7 +66,8 @@ struct TcParams {
 };
 
 struct Shared {
-    uint64_t q_full[2], full[5], empty[5], raw[5], s_full[2][2], p_full[2], pv_done[2], drain;
+    // s_full, p_full, pv_done: of each S buffer, 2 * query tile + buffer
+    uint64_t q_full[2], full[10], empty[10], raw[10], s_full[4], p_full[4], pv_done[4], drain[2];
     uint32_t tmem;
     int dead;
     uint32_t odd[8];  // columns in which a V element that is not finite was zeroed
@@ -79,48 +87,67 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
     return false;
 }
 
+// A whole warp waits; what it returns is the same for all lanes, and the compiler knows it.
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *dead, int *status, int code)
+{
+    for (uint32_t i = 0; i < umma::WAIT_LIMIT; i++) {
+        if (__all_sync(0xffffffffu, umma::mbar_try_wait(bar, parity)))
+            return true;
+        if ((i & 255) == 255 && __any_sync(0xffffffffu, *dead))
+            return false;
+    }
+    *dead = 1;
+    atomicExch(status, code);
+    return false;
+}
+
 template <int DP>
 __global__ void __launch_bounds__(Tc<DP>::THREADS, 1)
 attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TcParams p)
 {
     using C = Tc<DP>;
-    constexpr int NS = C::NS, SB = C::SB, CH = C::CH;
+    constexpr int NS = C::NS, SB = 2, CH = C::CH, BN = C::BN;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Shared sh;
     const uint32_t smem_base = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *const smem = smem_raw + (smem_base - umma::smem_u32(smem_raw));
     uint8_t *const ring = smem + NS * C::Q_BYTES;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = tid >> 7;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, group = warp >> 2;
     volatile int *const dead = &sh.dead;
     int *const status = p.a.status;
     const PromptArgs &a = p.a;
 
     const int index = blockIdx.x / p.pairs, pair = blockIdx.x - index * p.pairs;
+    const bool rows_split = NS == 2 && !p.by_heads;
     if (warp == 0) {
-        if (NS == 2 && !p.by_heads)
+        if (rows_split)
             find_prompt_tile<2 * BM>(a, index, sh.tile);
         else
             find_prompt_tile<BM>(a, index, sh.tile);
-    }
-    if (tid == 32) {
-        sh.dead = 0;
-        for (int i = 0; i < 8; i++)
-            sh.odd[i] = 0;
-        for (int i = 0; i < 2; i++) {
-            umma::mbar_init(&sh.q_full[i], 1);
-            umma::mbar_init(&sh.s_full[i][0], 1);
-            umma::mbar_init(&sh.s_full[i][1], 1);
-            umma::mbar_init(&sh.p_full[i], 4);
-            umma::mbar_init(&sh.pv_done[i], 1);
+        __syncwarp();
+        if (lane == 0) {
+            // how many threads give a ring stage back: one for each query tile that there is
+            const int users = NS == 1 || (rows_split && sh.tile.n_q - sh.tile.row0 <= BM) ? 1 : 2;
+            sh.dead = 0;
+            for (int i = 0; i < 8; i++)
+                sh.odd[i] = 0;
+            for (int i = 0; i < 2; i++) {
+                umma::mbar_init(&sh.q_full[i], 1);
+                umma::mbar_init(&sh.drain[i], 1);
+            }
+            for (int i = 0; i < 4; i++) {
+                umma::mbar_init(&sh.s_full[i], 1);
+                umma::mbar_init(&sh.p_full[i], 4);
+                umma::mbar_init(&sh.pv_done[i], 1);
+            }
+            for (int i = 0; i < C::STAGES; i++) {
+                umma::mbar_init(&sh.full[i], 1);
+                umma::mbar_init(&sh.empty[i], users);
+                umma::mbar_init(&sh.raw[i], 1);
+            }
+            umma::fence_barrier_init();
         }
-        for (int i = 0; i < C::STAGES; i++) {
-            umma::mbar_init(&sh.full[i], 1);
-            umma::mbar_init(&sh.empty[i], 1);
-            umma::mbar_init(&sh.raw[i], 1);
-        }
-        umma::mbar_init(&sh.drain, 1);
-        umma::fence_barrier_init();
     }
     __syncthreads();
     const PromptTile w = sh.tile;
@@ -129,7 +156,6 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
     // a block's query tiles: head and first row of each, and how many rows are left for it
     const int head0 = NS == 2 && p.by_heads ? 2 * pair : pair;
     const int kv_head = head0 / a.group;
-    const bool rows_split = NS == 2 && !p.by_heads;
     const int rows_all = min(rows_split ? 2 * BM : BM, w.n_q - w.row0);
     const int streams = NS == 1 || (rows_split && rows_all <= BM) ? 1 : 2;
     const int pos0 = w.n_k - w.n_q + w.row0;  // position of the block's first row
@@ -143,9 +169,8 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
     };
     const int pos_last = pos0 + rows_all - 1;
 
-    if (group == NS) {
-        if constexpr (NS == 2)
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (group >= NS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
         const int role = warp - NS * 4;
         if (role == 1) {
             umma::tmem_alloc(&sh.tmem, 512);
@@ -210,94 +235,131 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                         umma::mbar_wait(&sh.q_full[s], 0);
                 }
             }
-        } else if (role == 1) {
+        } else if (role <= 2) {
             // --------------------------------------------------------- products
-            if (lane == 0 && tiles > 0) {
+            const int self = role - 1;  // of two query tiles the one; of one tile, 0 issues P V and 1 issues Q K^T
+            if (tiles > 0 && (NS == 1 || self < streams)) {
+                const bool leader = umma::elect_one();  // the whole warp keeps step, so that descriptors stay in uniform registers
                 constexpr uint32_t k_hi = ((1024u >> 4) & 0x3fffu) | (1u << 14) | (umma::LAYOUT_SW128 << 29);
                 constexpr uint32_t qk_desc = umma::instr_desc(1, 0, 0, BM, BN);
                 constexpr uint32_t pv_desc = umma::instr_desc(1, 0, 0, BM, DP) | (1u << 16);  // V: keys along the rows
                 constexpr uint32_t v_lbo = DP == 64 ? 1u : uint32_t(BN / CH) * 128u >> 4;
-                const uint32_t q_lo = ((umma::smem_u32(smem) >> 4) & 0x3fffu) | (1u << 16);
-                const uint32_t ring_addr = umma::smem_u32(ring) >> 4;
+                const uint32_t q_lo = (((umma::smem_u32(smem) + (NS == 2 ? self * C::Q_BYTES : 0)) >> 4) & 0x3fffu) | (1u << 16);
+                const uint32_t ring_lo = umma::smem_u32(ring) >> 4;
+                int stage = 0;
+                uint32_t phase = 0;
                 bool ok = true;
-                auto arrived = [&](int n) {  // waits for the n-th chunk of the ring
-                    ok = ok && wait(&sh.full[n % C::STAGES], (n / C::STAGES) & 1, dead, status, OVK_DEV_TIMEOUT_TMA);
-                };
-                // position in the ring of tile i's first K and V chunk
-                auto k_at = [&](int i) { return CH * (i < SB ? i : 2 * i - SB + 1); };
-                auto v_at = [&](int i) { return CH * (min(SB, tiles) + i + min(i, max(0, tiles - SB))); };
-                auto qk = [&](int s, int i, bool release) {
-                    const uint32_t d = tmem + (SB == 2 ? (i & 1) : s) * 128;
+                auto next_tile = [&](int (&at)[CH], bool mine) {  // the ring's next tile; waits for it if it is this thread's
 #pragma unroll
                     for (int c = 0; c < CH; c++) {
-                        const int n = k_at(i) + c;
-                        const uint32_t b_lo = ((ring_addr + uint32_t(n % C::STAGES) * (C::STAGE >> 4)) & 0x3fffu) | (1u << 16);
-                        const uint32_t a_lo = q_lo + s * (C::Q_BYTES >> 4) + c * (C::ATOMS / CH) * (BM * 128 >> 4);
-                        if (c > 0)
-                            arrived(n);
-                        if (!ok)
-                            return;
+                        if (mine)
+                            ok = ok && wait_warp(&sh.full[stage], phase, dead, status, OVK_DEV_TIMEOUT_TMA);
+                        at[c] = stage;
+                        if (++stage == C::STAGES)
+                            stage = 0, phase ^= 1;
+                    }
+                };
+                auto qk = [&](int buffer, const int (&at)[CH]) {
+                    const uint32_t d = tmem + buffer * BN;
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        const uint32_t b_lo = ((ring_lo + uint32_t(at[c]) * (C::STAGE >> 4)) & 0x3fffu) | (1u << 16);
+                        const uint32_t a_lo = q_lo + c * (C::ATOMS / CH) * (BM * 128 >> 4);
 #pragma unroll
                         for (int k = 0; k < DP / CH / 16; k++) {
-                            const uint32_t off = (k >> 2) * (BM * 128 >> 4) + (k & 3) * 2;
-                            umma::mma_f16_lohi(d, a_lo + off, k_hi, b_lo + off, k_hi, qk_desc, c > 0 || k > 0);
+                            const uint32_t step = (k & 3) * 2, a_off = (k >> 2) * (BM * 128 >> 4) + step, b_off = (k >> 2) * (BN * 128 >> 4) + step;
+                            if (leader)
+                                umma::mma_f16_lohi(d, a_lo + a_off, k_hi, b_lo + b_off, k_hi, qk_desc, c > 0 || k > 0);
                         }
-                        if (release)
-                            umma::mma_commit(&sh.empty[n % C::STAGES]);
                     }
-                    umma::mma_commit(&sh.s_full[s][SB == 2 ? (i & 1) : 0]);
+                    if (leader) {
+                        umma::mma_commit(&sh.s_full[buffer]);
+#pragma unroll
+                        for (int c = 0; c < CH; c++)
+                            umma::mma_commit(&sh.empty[at[c]]);
+                    }
                 };
-                auto pv = [&](int s, int i, bool wait_v, bool release) {
-                    const uint32_t d = tmem + C::O_COL + s * DP, pt = tmem + (SB == 2 ? (i & 1) : s) * 128;
+                auto pv = [&](int buffer, const int (&at)[CH], bool accumulate, bool announce) {
+                    const uint32_t d = tmem + C::O_COL + (NS == 2 ? self * DP : 0), pt = tmem + buffer * BN;
 #pragma unroll
                     for (int c = 0; c < CH; c++) {
-                        const int n = v_at(i) + c, stage = n % C::STAGES;
-                        if (wait_v)
-                            arrived(n);
-                        if (!ok)
-                            return;
-                        umma::tc_fence_after();
-                        const uint32_t b_lo = ((ring_addr + uint32_t(stage) * (C::STAGE >> 4)) & 0x3fffu) | (v_lbo << 16);
+                        const uint32_t b_lo = ((ring_lo + uint32_t(at[c]) * (C::STAGE >> 4)) & 0x3fffu) | (v_lbo << 16);
 #pragma unroll
                         for (int k = 0; k < BN / CH / 16; k++)
-                            umma::mma_f16_ts(d, pt + c * (BN / CH / 2) + 8 * k, b_lo + k * (2048 >> 4), k_hi, pv_desc, i > 0 || c > 0 || k > 0);
-                        if (release)
-                            umma::mma_commit(&sh.empty[stage]);
+                            if (leader)
+                                umma::mma_f16_ts(d, pt + c * (BN / CH / 2) + 8 * k, b_lo + k * (2048 >> 4), k_hi, pv_desc, accumulate || c > 0 || k > 0);
                     }
-                    umma::mma_commit(&sh.pv_done[s]);
+                    if (leader) {
+                        if (announce)
+                            umma::mma_commit(&sh.pv_done[buffer]);
+#pragma unroll
+                        for (int c = 0; c < CH; c++)
+                            umma::mma_commit(&sh.empty[at[c]]);
+                    }
                 };
-                for (int j = 0; j < SB && j < tiles && ok; j++) {
-                    arrived(k_at(j));
-                    for (int s = 0; s < streams && ok; s++) {
-                        if (j == 0)
-                            ok = ok && wait(&sh.q_full[s], 0, dead, status, OVK_DEV_TIMEOUT_TMA);
+                int k_at[CH], v_at[CH];
+                if constexpr (NS == 2) {
+                    // tile i's scores go into buffer i & 1, behind the product that uses the weights of tile i - 2 there
+                    ok = wait_warp(&sh.q_full[self], 0, dead, status, OVK_DEV_TIMEOUT_TMA);
+                    for (int j = 0; j < SB && j < tiles; j++) {
+                        next_tile(k_at, true);
                         if (ok)
-                            qk(s, j, s == streams - 1);
+                            qk(2 * self + j, k_at);
                     }
-                }
-                for (int i = 0; i < tiles && ok; i++) {
-                    for (int s = 0; s < streams && ok; s++) {
-                        ok = wait(&sh.p_full[SB == 2 ? i & 1 : s], SB == 2 ? (i >> 1) & 1 : i & 1, dead, status, OVK_DEV_TIMEOUT_SLOT);
+                    for (int i = 0; i < tiles && ok; i++) {
+                        const bool more = i + SB < tiles;
+                        next_tile(v_at, true);
+                        if (more)
+                            next_tile(k_at, true);
+                        ok = ok && wait_warp(&sh.p_full[2 * self + (i & 1)], (i >> 1) & 1, dead, status, OVK_DEV_TIMEOUT_SLOT);
                         if (!ok)
                             break;
                         umma::tc_fence_after();
-                        pv(s, i, s == 0, s == streams - 1);
-                        if (ok && i + SB < tiles) {
-                            if (s == 0)
-                                arrived(k_at(i + SB));
-                            if (ok)
-                                qk(s, i + SB, s == streams - 1);
+                        pv(2 * self + (i & 1), v_at, i > 0, true);
+                        if (more)
+                            qk(2 * self + (i & 1), k_at);
+                    }
+                } else {
+                    // tile i's scores go into buffer i & 1 once the weights of tile i - 2, which lay there, are used
+                    const bool scores = self == 1;
+                    if (scores)
+                        ok = wait_warp(&sh.q_full[0], 0, dead, status, OVK_DEV_TIMEOUT_TMA);
+                    for (int j = 0; j < SB && j < tiles; j++) {
+                        next_tile(k_at, scores);
+                        if (scores && ok)
+                            qk(j, k_at);
+                    }
+                    for (int i = 0; i < tiles && ok; i++) {
+                        next_tile(v_at, !scores);
+                        if (!scores) {
+                            ok = ok && wait_warp(&sh.p_full[i & 1], (i >> 1) & 1, dead, status, OVK_DEV_TIMEOUT_SLOT);
+                            if (!ok)
+                                break;
+                            umma::tc_fence_after();
+                            pv(i & 1, v_at, i > 0, true);
+                        }
+                        if (i + SB < tiles) {
+                            next_tile(k_at, scores);
+                            if (scores) {
+                                ok = ok && wait_warp(&sh.pv_done[i & 1], (i >> 1) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
+                                if (!ok)
+                                    break;
+                                umma::tc_fence_after();
+                                qk(i & 1, k_at);
+                            }
                         }
                     }
                 }
                 if (!ok) {  // products in flight end before tensor memory is freed
-                    umma::mma_commit(&sh.drain);
-                    umma::mbar_wait(&sh.drain, 0);
+                    if (leader)
+                        umma::mma_commit(&sh.drain[self]);
+                    umma::mbar_wait(&sh.drain[self], 0);
                 }
             }
             __syncwarp();
-        } else if (tiles > 0) {
+        } else if (tiles > 0 && (NS == 2 || group == 2)) {
             // ------------------------------------------------------------ guards
+            const int guard = NS == 2 ? 0 : warp & 3;
             int n = CH * min(SB, tiles);  // place in the ring
             uint32_t raw_phase = 0;       // a bit per stage
             bool ok = true;
@@ -306,18 +368,18 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                     if (!partial(i, pos0, pos_last))
                         continue;
                     const int stage = n % C::STAGES;
-                    ok = wait(&sh.raw[stage], (raw_phase >> stage) & 1, dead, status, OVK_DEV_TIMEOUT_TMA);
+                    ok = wait_warp(&sh.raw[stage], (raw_phase >> stage) & 1, dead, status, OVK_DEV_TIMEOUT_TMA);
                     raw_phase ^= 1u << stage;
                     // in each 128-byte column the chunk's rows lie one after the other, eight 16-byte words a row
                     constexpr int KEYS = BN / CH;
                     const int left = min(KEYS, max(0, key_end - (key_begin + i * BN + c * KEYS)));  // rows before the end
-                    const int self = (role - 2) * 32 + lane;
+                    const int self = guard * 32 + lane;
                     for (int x = 0; x < C::ATOMS && ok; x++) {
                         uint4 *const words = reinterpret_cast<uint4 *>(ring + stage * C::STAGE) + x * KEYS * 8;
                         uint32_t bad = 0;
 #pragma unroll
-                        for (int k = 0; k < KEYS * 8 / 64; k++) {
-                            const int at = self + 64 * k;
+                        for (int k = 0; k < KEYS * 8 / (32 * C::GUARDS); k++) {
+                            const int at = self + 32 * C::GUARDS * k;
                             if (at < left * 8) {
                                 const uint4 v = words[at];  // a carry into the sign bit marks an exponent of ones
                                 bad |= ((v.x & 0x7c007c00u) + 0x04000400u) | ((v.y & 0x7c007c00u) + 0x04000400u) |
@@ -328,7 +390,7 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                         }
                         if (!(bad & 0x80008000u))
                             continue;
-                        for (int at = self; at < left * 8; at += 64) {
+                        for (int at = self; at < left * 8; at += 32 * C::GUARDS) {
                             const int col = x * 64 + (((at & 7) ^ ((at >> 3) & 7)) << 3);  // of the word's first element
                             uint32_t z[4] = {words[at].x, words[at].y, words[at].z, words[at].w};
                             for (int e = 0; e < 8; e++)
@@ -340,18 +402,18 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                         }
                     }
                     umma::fence_proxy_async();
-                    // both warps, also after a wait that gave up: then both leave
+                    // all of them, also after a wait that gave up: then all leave
                     uint32_t all;
                     asm volatile(
                         "{\n\t.reg .pred p, q;\n\t"
                         "setp.ne.b32 p, %1, 0;\n\t"
-                        "bar.red.and.pred q, 2, 64, p;\n\t"
+                        "bar.red.and.pred q, 2, %2, p;\n\t"
                         "selp.u32 %0, 1, 0, q;\n\t}"
                         : "=r"(all)
-                        : "r"(uint32_t(ok))
+                        : "r"(uint32_t(ok)), "n"(32 * C::GUARDS)
                         : "memory");
                     ok = all != 0;
-                    if (ok && role == 2 && lane == 0)
+                    if (ok && guard == 0 && lane == 0)
                         umma::mbar_arrive(&sh.full[stage]);
                 }
                 n += i + SB < tiles ? CH : 0;
@@ -359,8 +421,7 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
         }
     } else {
         // ---------------------------------------------------------------- softmax
-        if constexpr (NS == 2)
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
         umma::tc_fence_before();
         asm volatile("bar.sync 1, %0;" ::"n"(C::THREADS) : "memory");
         umma::tc_fence_after();
@@ -375,17 +436,15 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
             float m = -1e30f, l = 0.0f;
             bool ok = true;
             for (int i = 0; i < tiles; i++) {
-                const int buffer = SB == 2 ? (i & 1) : 0;
-                const uint32_t t_s = tmem + lanes + (SB == 2 ? buffer : s) * 128;
-                ok = wait(&sh.s_full[s][buffer], SB == 2 ? (i >> 1) & 1 : i & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
+                const int buffer = 2 * s + (i & 1);
+                const uint32_t t_s = tmem + lanes + buffer * BN;
+                ok = wait_warp(&sh.s_full[buffer], (i >> 1) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
+                if (!ok)
                     break;
-                }
                 umma::tc_fence_after();
-                uint32_t x[4][32];
+                uint32_t x[BN / 32][32];
 #pragma unroll
-                for (int c = 0; c < 4; c++)
+                for (int c = 0; c < BN / 32; c++)
                     umma::tmem_ld_32x32(t_s + 32 * c, x[c]);
                 umma::tmem_ld_wait();
                 if (partial(i, first, first + rows - 1)) {
@@ -393,7 +452,7 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                     const int hi = (a.causal ? min(pos, w.n_k - 1) : w.n_k - 1) - j0;
                     const int lo = p.window > 0 ? pos - p.window + 1 - j0 : 0;
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
+                    for (int c = 0; c < BN / 32; c++)
 #pragma unroll
                         for (int e = 0; e < 32; e++)
                             if (32 * c + e > hi || 32 * c + e < lo)
@@ -401,26 +460,22 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                 }
                 float most[4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    most[c] = __uint_as_float(x[c][0]);
+                for (int e = 0; e < 4; e++)
+                    most[e] = __uint_as_float(x[0][e]);
 #pragma unroll
-                    for (int e = 1; e < 32; e++)
-                        most[c] = fmaxf(most[c], __uint_as_float(x[c][e]));
-                }
+                for (int e = 4; e < BN; e++)
+                    most[e & 3] = fmaxf(most[e & 3], __uint_as_float(x[e >> 5][e & 31]));
                 const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * scale;
                 if (__any_sync(0xffffffffu, top > m + 8.0f)) {
                     const float to = fmaxf(m, top), f = exp2_approx(m - to);
                     m = to;
                     l *= f;
                     if (i > 0) {
-                        if constexpr (SB == 2) {  // the product before this one may still be writing O
-                            ok = wait(&sh.pv_done[s], (i - 1) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
-                            if (!__all_sync(0xffffffffu, ok)) {
-                                ok = false;
-                                break;
-                            }
-                            umma::tc_fence_after();
-                        }
+                        // the product before this one may still be writing O
+                        ok = wait_warp(&sh.pv_done[2 * s + ((i - 1) & 1)], ((i - 1) >> 1) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
+                        if (!ok)
+                            break;
+                        umma::tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < DP / 16; c++) {
                             uint32_t o[16];
@@ -435,7 +490,7 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                 }
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
+                for (int c = 0; c < BN / 64; c++) {
                     uint32_t out[32];
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
@@ -453,15 +508,10 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                 umma::tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    umma::mbar_arrive(&sh.p_full[SB == 2 ? buffer : s]);
+                    umma::mbar_arrive(&sh.p_full[buffer]);
             }
             if (ok && tiles > 0) {
-                // the last scores imply that the second to last product into O is done (with two S buffers: the
-                // third to last), and a parity tells only neighbouring phases apart
-                if (SB == 2 && tiles > 1)
-                    ok = wait(&sh.pv_done[s], (tiles - 2) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
-                ok = ok && wait(&sh.pv_done[s], (tiles - 1) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = wait_warp(&sh.pv_done[2 * s + ((tiles - 1) & 1)], ((tiles - 1) >> 1) & 1, dead, status, OVK_DEV_TIMEOUT_MMA);
                 umma::tc_fence_after();
             }
             if (ok) {
@@ -553,8 +603,8 @@ template <int DP> int32_t launch(ovk_ctx *ctx, const PromptArgs &a, bool *taken)
     CUtensorMap q, k, v;
     const int kv_heads = a.heads / a.group;
     if (!make_map(&q, a.q, a.q_tokens, a.heads, a.head_dim, a.q_token, a.q_head, BM) ||
-        !make_map(&k, a.k, a.k_tokens, kv_heads, a.head_dim, a.k_token, a.k_head, BN) ||
-        !make_map(&v, a.v, a.k_tokens, kv_heads, a.head_dim, a.v_token, a.v_head, BN / C::CH))
+        !make_map(&k, a.k, a.k_tokens, kv_heads, a.head_dim, a.k_token, a.k_head, C::BN) ||
+        !make_map(&v, a.v, a.k_tokens, kv_heads, a.head_dim, a.v_token, a.v_head, C::BN / C::CH))
         return OVK_OK;
     TcParams p = {};
     p.a = a;
