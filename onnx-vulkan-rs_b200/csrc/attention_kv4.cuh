@@ -34,7 +34,7 @@
 //    2^16 and is a normal fp16 number down to 2^-20 of the largest, and a step
 //    needs one vote, not a reduction.
 //
-// One CTA per SM takes an equal run of units - 16 tokens for each of its consumer
+// One CTA per SM takes an equal run of units - 32 tokens for each of its consumer
 // warps - of the whole batch (lengths are read on the device).  Four producer
 // warps bring units into a ring with 16-byte copies, row by row, so that a page may
 // have any size, and go on with the next sequence while the consumers finish one.
@@ -68,7 +68,7 @@ struct Kv4Args {
 
 namespace kv4 {
 
-constexpr int STEP = 16;
+constexpr int STEP = 32;  // tokens of a warp at a time: two products' rows, independent until they meet in the sums
 constexpr float NONE = -1e30f;  // the maximum of a row that has seen nothing (in powers of two)
 
 template <int D_, int NT_, int PARTS_> struct Shape {
@@ -76,21 +76,21 @@ template <int D_, int NT_, int PARTS_> struct Shape {
     static constexpr int NCH = D / 32, ROWS = 8 * NT, ROW_BYTES = D / 2, CPR = D / 32;
     // consumer warps, and the registers each thread of theirs and of the producer's group gets; 256-wide heads with
     // two tiles of rows hold 128 accumulators a thread
-    static constexpr int WARPS = D == 256 && NT == 2 ? 8 : 12;
+    static constexpr int WARPS = 8;
     static constexpr int REGS = WARPS == 8 ? 208 : 144, PRODUCER_REGS = WARPS == 8 ? 88 : 80;
     static constexpr int THREADS = WARPS * 32 + 128, UNIT = WARPS * STEP;
-    static constexpr int STAGES = D == 256 ? 2 : 4;
+    static constexpr int STAGES = D == 256 ? 2 : 3;
     static constexpr int CODES = UNIT * ROW_BYTES;        // of K or of V, one stage
     static constexpr int SCALES = UNIT * 16, ZEROS = UNIT * 4;
     static constexpr int PRESENT = 2 * CODES + 2 * (SCALES + ZEROS) + UNIT * 4;  // behind scales, zero points and row numbers
-    static constexpr int STAGE = (PRESENT + WARPS * 2 + 1023) / 1024 * 1024;     // the copies' swizzle counts from such a boundary
+    static constexpr int STAGE = (PRESENT + WARPS * 4 + 127) / 128 * 128;
     // of a warp: {scale, zero} of K per token and chunk, scale of V, zeros of V per pair of tokens and chunk
     static constexpr int K_SZ = STEP * NCH * 8, V_S = STEP * NCH * 4, V_Z = STEP / 2 * NCH * 4, SZ = K_SZ + V_S + V_Z;
     static constexpr int QF = PARTS * NT * NCH * 512;     // query fragments
-    static constexpr int SLOTS = D == 256 && NT == 1 ? WARPS / 4 : WARPS / 2;    // warps that add their sums at a time
+    static constexpr int SLOTS = D == 256 && NT == 2 ? 1 : WARPS / 2;  // warps that add their sums at a time
     static constexpr int MERGE = SLOTS * ROWS * (D + 4) * 4;
     static constexpr int RING = STAGES * STAGE;
-    static constexpr int SMEM = 1024 + RING + WARPS * SZ + MERGE + QF + ROWS * (NCH + 1) * 4 + 2 * WARPS * ROWS * 4;
+    static constexpr int SMEM = 128 + RING + WARPS * SZ + MERGE + QF + ROWS * (NCH + 1) * 4 + 2 * WARPS * ROWS * 4;
     static constexpr bool Q_REGS = PARTS * NT * NCH * 4 <= 16;
     static constexpr bool SUBNORMAL = PARTS == 1;         // how codes enter the products
     static constexpr int SLOT = ROWS * (D + 2);           // floats of a partial result
@@ -245,13 +245,13 @@ template <int N> __device__ __forceinline__ bool consumers_all(bool ok)
         : "memory");
     return all != 0;
 }
-// A wait that has run out ends every other wait of the CTA soon after.
+// A whole warp waits.  One that has run out ends every other wait of the CTA soon after.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *dead, int *status, int code)
 {
     for (uint32_t i = 0; i < umma::WAIT_LIMIT; i++) {
-        if (umma::mbar_try_wait(bar, parity))
+        if (__all_sync(0xffffffffu, umma::mbar_try_wait(bar, parity)))
             return true;
-        if ((i & 255) == 255 && *dead)
+        if ((i & 255) == 255 && __any_sync(0xffffffffu, *dead))
             return false;
     }
     *dead = 1;
@@ -271,9 +271,9 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
     __shared__ uint64_t full[STAGES], empty[STAGES];
     __shared__ int dead_word;
     volatile int *const dead = &dead_word;
-    const uint32_t ring = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t ring = (umma::smem_u32(smem_raw) + 127u) & ~127u;
     uint8_t *const smem = smem_raw + (ring - umma::smem_u32(smem_raw));
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     float *const merge = reinterpret_cast<float *>(smem + S::RING + WARPS * S::SZ);
     uint8_t *const qf = reinterpret_cast<uint8_t *>(merge) + S::MERGE;
     float *const q_sum = reinterpret_cast<float *>(qf + S::QF);       // [NCH][ROWS]
@@ -397,10 +397,8 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 row[i] = producer + 4 * i < ROUNDS ? row_of(first + 128 * i) : -1;
             for (int u = 0; u < units_here; u++) {
                 ok = wait(&empty[stage], phase ^ 1, dead, a.status, OVK_DEV_TIMEOUT_SLOT);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
+                if (!ok)
                     break;
-                }
                 const uint32_t to = ring + stage * S::STAGE, raw = to + 2 * S::CODES;
 #pragma unroll
                 for (int i = 0; i < MINE; i++) {
@@ -570,10 +568,10 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
             const int swizzle = S::CPR == 2 ? (r >> 2) & 1 : S::CPR == 4 ? (r >> 1) & 3 : r & 7;
             k_at[i] = ring + (warp * STEP + r) * S::ROW_BYTES + ((c ^ swizzle) << 4);
         }
-        // where the raw scales and zero points of this lane's row lie: lanes 0-15 keys, 16-31 values
-        const int place = warp * STEP + (lane & 15), kv = lane >> 4, zero_bytes = (a.blocks + 1) >> 1;
-        const uint32_t scale_at = ring + 2 * S::CODES + kv * S::SCALES + place * 16;
-        const uint32_t zero_at = ring + 2 * S::CODES + 2 * S::SCALES + kv * S::ZEROS + place * 4;
+        // where the raw scales and zero points of this lane's token lie (keys'; values' lie behind all of those)
+        const int place = warp * STEP + lane, zero_bytes = (a.blocks + 1) >> 1;
+        const uint32_t scale_at = ring + 2 * S::CODES + place * 16;
+        const uint32_t zero_at = ring + 2 * S::CODES + 2 * S::SCALES + place * 4;
         const uint32_t row_at = ring + 2 * S::CODES + 2 * (S::SCALES + S::ZEROS) + place * 4;
 
         float o[NCH][2][NT][4];
@@ -592,78 +590,71 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         bool ok = true;
         for (int u = 0; u < units_here; u++) {
             ok = wait(&full[stage], phase, dead, a.status, OVK_DEV_TIMEOUT_TMA);
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
+            if (!ok)
                 break;
-            }
             const uint32_t to_stage = stage * S::STAGE;
             const int token0 = t_begin + u * UNIT + warp * STEP;
-            // the step's tokens that are there
-            const uint32_t present = (lds32(ring + to_stage + S::PRESENT + (warp >> 1) * 4) >> (16 * (warp & 1))) & 0xffffu;
+            const uint32_t present = lds32(ring + to_stage + S::PRESENT + warp * 4);  // which of the step's tokens are there
 
-            // -------- scale and zero of each chunk of this lane's row, as the products want them
+            // -------- scales and zeros of each chunk of this lane's token, as the products want them
             uint32_t high;
             {
-                const uint32_t where = scale_at + to_stage;
-                uint32_t words[4] = {0, 0, 0, 0}, z = 0x88888888u;
-                if (a.blocks == 4) {
-                    const uint2 two = lds64(where);
-                    words[0] = two.x, words[1] = two.y;
-                } else if (a.blocks == 8) {
-                    lds_words(where, words);
-                } else {
-                    words[0] = lds32(where);
-                    if (a.blocks == 1) {
-                        words[0] = (lds32(row_at + to_stage) & 1u) ? words[0] >> 16 : words[0] & 0xffffu;
+                uint32_t words[2][4] = {}, z[2] = {0x88888888u, 0x88888888u};
+                const uint32_t row = lds32(row_at + to_stage);
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    const uint32_t where = scale_at + to_stage + kv * S::SCALES;
+                    if (a.blocks == 4) {
+                        const uint2 two = lds64(where);
+                        words[kv][0] = two.x, words[kv][1] = two.y;
+                    } else if (a.blocks == 8) {
+                        lds_words(where, words[kv]);
+                    } else {
+                        words[kv][0] = lds32(where);
+                        if (a.blocks == 1)
+                            words[kv][0] = (row & 1u) ? words[kv][0] >> 16 : words[kv][0] & 0xffffu;
+                    }
+                    if (a.zero_points[0]) {
+                        z[kv] = lds32(zero_at + to_stage + kv * S::ZEROS);
+                        if (zero_bytes < 4)
+                            z[kv] >>= 8 * ((row * zero_bytes) & 3);
                     }
                 }
-                if (a.zero_points[0]) {
-                    z = lds32(zero_at + to_stage);
-                    if (zero_bytes < 4)
-                        z >>= 8 * ((lds32(row_at + to_stage) * zero_bytes) & 3);
-                }
-                if (!((present >> (lane & 15)) & 1u))
-                    words[0] = words[1] = words[2] = words[3] = 0;
-                const uint32_t z_next = __shfl_down_sync(0xffffffffu, z, 1);  // the next token's, for pairs of V
+                const uint32_t z_next = __shfl_down_sync(0xffffffffu, z[1], 1);  // the next token's, for pairs of V
                 auto expand = [&](auto shift) {
                     constexpr int SHIFT = decltype(shift)::value, BLOCKS = NCH >> SHIFT;
-                    float s[BLOCKS];
+                    uint32_t out[2 * NCH];
 #pragma unroll
-                    for (int i = 0; i < BLOCKS; i++)
-                        s[i] = (i & 1) ? half_hi(words[i >> 1]) : half_lo(words[i >> 1]);
-                    if (kv == 0) {
-                        uint32_t out[2 * NCH];
+                    for (int c = 0; c < NCH; c++) {
+                        const int blk = c >> SHIFT;
+                        const uint32_t zero = (z[0] >> (4 * blk)) & 15u;
+                        out[2 * c] = __float_as_uint((blk & 1) ? half_hi(words[0][blk >> 1]) : half_lo(words[0][blk >> 1]));
+                        // f16: what the accumulator's start multiplies; f32: the zero of a pair of codes
+                        out[2 * c + 1] = S::SUBNORMAL ? __float_as_uint(half_lo(zero)) : zero * 0x00010001u;
+                    }
+                    sts_words(sz + lane * (NCH * 8), out);
+                    uint32_t out_v[NCH];
+#pragma unroll
+                    for (int c = 0; c < NCH; c++) {
+                        const int blk = c >> SHIFT;
+                        out_v[c] = __float_as_uint((blk & 1) ? half_hi(words[1][blk >> 1]) : half_lo(words[1][blk >> 1]));
+                    }
+                    sts_words(sz + S::K_SZ + lane * (NCH * 4), out_v);
+                    if ((lane & 1) == 0) {
+                        const uint32_t low = __byte_perm(z[1], z_next, 0x5410), up = __byte_perm(z[1], z_next, 0x7632);
 #pragma unroll
                         for (int c = 0; c < NCH; c++) {
                             const int blk = c >> SHIFT;
-                            out[2 * c] = __float_as_uint(s[blk]);
-                            const uint32_t zero = (z >> (4 * blk)) & 15u;
-                            // f16: what the accumulator's start multiplies; f32: the zero of a pair of codes
-                            out[2 * c + 1] = S::SUBNORMAL ? __float_as_uint(half_lo(zero)) : zero * 0x00010001u;
+                            out_v[c] = ((blk < 4 ? low : up) >> (4 * (blk & 3))) & 0x000f000fu;
                         }
-                        sts_words(sz + (lane & 15) * (NCH * 8), out);
-                    } else {
-                        uint32_t out[NCH];
-#pragma unroll
-                        for (int c = 0; c < NCH; c++)
-                            out[c] = __float_as_uint(s[c >> SHIFT]);
-                        sts_words(sz + S::K_SZ + (lane & 15) * (NCH * 4), out);
-                        if ((lane & 1) == 0) {
-                            const uint32_t low = __byte_perm(z, z_next, 0x5410), up = __byte_perm(z, z_next, 0x7632);
-#pragma unroll
-                            for (int c = 0; c < NCH; c++) {
-                                const int blk = c >> SHIFT;
-                                out[c] = ((blk < 4 ? low : up) >> (4 * (blk & 3))) & 0x000f000fu;
-                            }
-                            sts_words(sz + S::K_SZ + S::V_S + (lane & 15) / 2 * (NCH * 4), out);
-                        }
+                        sts_words(sz + S::K_SZ + S::V_S + lane / 2 * (NCH * 4), out_v);
                     }
                     // the largest scale of the row (the order of fp16 numbers is that of their bits)
-                    uint32_t two = words[0] & (BLOCKS == 1 ? 0x7fffu : 0x7fff7fffu);
+                    uint32_t two = words[1][0] & (BLOCKS == 1 ? 0x7fffu : 0x7fff7fffu);
 #pragma unroll
                     for (int i = 1; i < BLOCKS / 2; i++)
-                        two = __vmaxu2(two, words[i] & 0x7fff7fffu);
-                    high = kv == 0 ? 0u : max(two & 0xffffu, two >> 16);
+                        two = __vmaxu2(two, words[1][i] & 0x7fff7fffu);
+                    high = max(two & 0xffffu, two >> 16);
                 };
                 if (a.chunk_shift == 0)
                     expand(std::integral_constant<int, 0>());
@@ -676,76 +667,83 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
             __syncwarp();
 
             // ---------------------------------------------------- scores
-            float x[NT][4];
+            float x[2][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-                x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+                    x[h][n][0] = x[h][n][1] = x[h][n][2] = x[h][n][3] = 0.0f;
 #pragma unroll
             for (int i = 0; i < NCH / 2; i++) {
-                // tokens 0-7 and 8-15 of chunk 2i, then of chunk 2i + 1
-                const uint4 words = load_matrices<false>(k_at[i] + to_stage);
-                const uint4 sz_a = lds128(sz + g * (NCH * 8) + 16 * i), sz_b = lds128(sz + (g + 8) * (NCH * 8) + 16 * i);
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    constexpr bool SUB = S::SUBNORMAL;
-                    const int c = 2 * i + j;
-                    const uint32_t w0 = j ? words.z : words.x, w1 = j ? words.w : words.y, v0 = w0 >> 8, v1 = w1 >> 8;
-                    const float s0 = __uint_as_float(j ? sz_a.z : sz_a.x), s1 = __uint_as_float(j ? sz_b.z : sz_b.x);
-                    const uint32_t z0 = j ? sz_a.w : sz_a.y, z1 = j ? sz_b.w : sz_b.y;
-                    uint32_t a0[4] = {codes_at<SUB, false>(w0), codes_at<SUB, false>(w1), codes_at<SUB, true>(w0), codes_at<SUB, true>(w1)};
-                    uint32_t a1[4] = {codes_at<SUB, false>(v0), codes_at<SUB, false>(v1), codes_at<SUB, true>(v0), codes_at<SUB, true>(v1)};
-                    if constexpr (!SUB) {
-                        a0[0] = minus_zero<SUB, false>(w0, z0), a0[1] = minus_zero<SUB, false>(w1, z1);
-                        a0[2] = minus_zero<SUB, true>(w0, z0), a0[3] = minus_zero<SUB, true>(w1, z1);
-                        a1[0] = minus_zero<SUB, false>(v0, z0), a1[1] = minus_zero<SUB, false>(v1, z1);
-                        a1[2] = minus_zero<SUB, true>(v0, z0), a1[3] = minus_zero<SUB, true>(v1, z1);
-                    }
+                for (int h = 0; h < 2; h++) {
+                    // tokens 0-7 and 8-15 of the half for chunk 2i, then for chunk 2i + 1
+                    const uint4 words = load_matrices<false>(k_at[i] + to_stage + h * 16 * S::ROW_BYTES);
+                    const uint4 sz_a = lds128(sz + (16 * h + g) * (NCH * 8) + 16 * i), sz_b = lds128(sz + (16 * h + g + 8) * (NCH * 8) + 16 * i);
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if constexpr (SUB) {
-                            float2 sum;
-                            if constexpr (S::Q_REGS)
-                                sum = qs[n][c];
-                            else
-                                sum = *reinterpret_cast<const float2 *>(q_sum + c * ROWS + n * 8 + 2 * t);
-                            acc[0] = __uint_as_float(z0) * sum.x, acc[1] = __uint_as_float(z0) * sum.y;
-                            acc[2] = __uint_as_float(z1) * sum.x, acc[3] = __uint_as_float(z1) * sum.y;
+                    for (int j = 0; j < 2; j++) {
+                        constexpr bool SUB = S::SUBNORMAL;
+                        const int c = 2 * i + j;
+                        const uint32_t w0 = j ? words.z : words.x, w1 = j ? words.w : words.y, v0 = w0 >> 8, v1 = w1 >> 8;
+                        const float s0 = __uint_as_float(j ? sz_a.z : sz_a.x), s1 = __uint_as_float(j ? sz_b.z : sz_b.x);
+                        const uint32_t z0 = j ? sz_a.w : sz_a.y, z1 = j ? sz_b.w : sz_b.y;
+                        uint32_t a0[4] = {codes_at<SUB, false>(w0), codes_at<SUB, false>(w1), codes_at<SUB, true>(w0), codes_at<SUB, true>(w1)};
+                        uint32_t a1[4] = {codes_at<SUB, false>(v0), codes_at<SUB, false>(v1), codes_at<SUB, true>(v0), codes_at<SUB, true>(v1)};
+                        if constexpr (!SUB) {
+                            a0[0] = minus_zero<SUB, false>(w0, z0), a0[1] = minus_zero<SUB, false>(w1, z1);
+                            a0[2] = minus_zero<SUB, true>(w0, z0), a0[3] = minus_zero<SUB, true>(w1, z1);
+                            a1[0] = minus_zero<SUB, false>(v0, z0), a1[1] = minus_zero<SUB, false>(v1, z1);
+                            a1[2] = minus_zero<SUB, true>(v0, z0), a1[3] = minus_zero<SUB, true>(v1, z1);
                         }
 #pragma unroll
-                        for (int p = 0; p < PARTS; p++) {
-                            uint4 q4;
-                            if constexpr (S::Q_REGS)
-                                q4 = bq[p][n][c];
-                            else
-                                q4 = reinterpret_cast<const uint4 *>(qf)[((p * NT + n) * NCH + c) * 32 + lane];
-                            mma(acc, a0, q4.x, q4.y);
-                            mma(acc, a1, q4.z, q4.w);
+                        for (int n = 0; n < NT; n++) {
+                            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            if constexpr (SUB) {
+                                float2 sum;
+                                if constexpr (S::Q_REGS)
+                                    sum = qs[n][c];
+                                else
+                                    sum = *reinterpret_cast<const float2 *>(q_sum + c * ROWS + n * 8 + 2 * t);
+                                acc[0] = __uint_as_float(z0) * sum.x, acc[1] = __uint_as_float(z0) * sum.y;
+                                acc[2] = __uint_as_float(z1) * sum.x, acc[3] = __uint_as_float(z1) * sum.y;
+                            }
+#pragma unroll
+                            for (int p = 0; p < PARTS; p++) {
+                                uint4 q4;
+                                if constexpr (S::Q_REGS)
+                                    q4 = bq[p][n][c];
+                                else
+                                    q4 = reinterpret_cast<const uint4 *>(qf)[((p * NT + n) * NCH + c) * 32 + lane];
+                                mma(acc, a0, q4.x, q4.y);
+                                mma(acc, a1, q4.z, q4.w);
+                            }
+                            x[h][n][0] = fmaf(s0, acc[0], x[h][n][0]);
+                            x[h][n][1] = fmaf(s0, acc[1], x[h][n][1]);
+                            x[h][n][2] = fmaf(s1, acc[2], x[h][n][2]);
+                            x[h][n][3] = fmaf(s1, acc[3], x[h][n][3]);
                         }
-                        x[n][0] = fmaf(s0, acc[0], x[n][0]);
-                        x[n][1] = fmaf(s0, acc[1], x[n][1]);
-                        x[n][2] = fmaf(s1, acc[2], x[n][2]);
-                        x[n][3] = fmaf(s1, acc[3], x[n][3]);
                     }
                 }
             }
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    x[n][e] *= factor[n][e & 1];
-            const bool masked = present != 0xffffu || token0 + STEP - 1 > pos_first || (window > 0 && token0 < pos_last - window + 1);
-            if (masked) {
+            for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int token = token0 + g + (e >= 2 ? 8 : 0), p = pos[n][e & 1];
-                        const bool read = ((present >> (g + (e >= 2 ? 8 : 0))) & 1u) && token <= p &&
-                                          (window == 0 || token > p - window);
-                        if (!read)
-                            x[n][e] = -INFINITY;
-                    }
+                    for (int e = 0; e < 4; e++)
+                        x[h][n][e] *= factor[n][e & 1];
+            const bool masked = present != 0xffffffffu || token0 + STEP - 1 > pos_first || (window > 0 && token0 < pos_last - window + 1);
+            if (masked) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int place_in = 16 * h + g + (e >= 2 ? 8 : 0), token = token0 + place_in, p = pos[n][e & 1];
+                            if (!((present >> place_in) & 1u) || token > p || (window > 0 && token <= p - window))
+                                x[h][n][e] = -INFINITY;
+                        }
             }
             // ------------------------------------------ the running maximum
             bool moves = scale_moves;
@@ -753,12 +751,10 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    moves |= x[n][e] > m[n][e & 1] + 6.0f;
+                    moves |= x[0][n][e] > m[n][e & 1] + 6.0f || x[1][n][e] > m[n][e & 1] + 6.0f;
             if (__any_sync(0xffffffffu, moves)) {
                 // sums and accumulators so far are brought to the new maximum and the new scale's exponent
-#pragma unroll
-                for (int o_ = 16; o_ > 0; o_ >>= 1)
-                    high = max(high, __shfl_xor_sync(0xffffffffu, high, o_));
+                high = __reduce_max_sync(0xffffffffu, high);
                 const uint32_t new_scale = max(top_scale, min(high, 0x7800u) & 0x7c00u);
                 top_scale = new_scale;
                 // p is smaller by the exponent of the largest scale, less 6
@@ -767,7 +763,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float most = fmaxf(x[n][e], x[n][e + 2]);
+                        float most = fmaxf(fmaxf(x[0][n][e], x[0][n][e + 2]), fmaxf(x[1][n][e], x[1][n][e + 2]));
 #pragma unroll
                         for (int o_ = 4; o_ < 32; o_ <<= 1)
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o_));
@@ -783,51 +779,58 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                         }
                     }
             }
-            float p[NT][4];
+            float p[2][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    p[n][e] = exp2_approx(x[n][e] - reference[n][e & 1]);
-                l[n][0] += p[n][0] + p[n][2];
-                l[n][1] += p[n][1] + p[n][3];
-            }
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        p[h][n][e] = exp2_approx(x[h][n][e] - reference[n][e & 1]);
+                    l[n][0] += p[h][n][0] + p[h][n][2];
+                    l[n][1] += p[h][n][1] + p[h][n][3];
+                }
             // ---------------------------------------------------- values
             auto values = [&](auto is_masked) {
 #pragma unroll
                 for (int i = 0; i < NCH / 2; i++) {
-                    // pairs of tokens 2t, 2t + 1 and 2t + 8, 2t + 9 of chunk 2i, then of chunk 2i + 1
-                    const uint4 words = load_matrices<true>(k_at[i] + to_stage + S::CODES);
-                    const uint2 s_a = lds64(sz + S::K_SZ + g * (NCH * 4) + 8 * i), s_b = lds64(sz + S::K_SZ + (g + 8) * (NCH * 4) + 8 * i);
-                    const uint2 z_a = lds64(sz + S::K_SZ + S::V_S + t * (NCH * 4) + 8 * i), z_b = lds64(sz + S::K_SZ + S::V_S + (t + 4) * (NCH * 4) + 8 * i);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        constexpr bool SUB = S::SUBNORMAL;
-                        const int c = 2 * i + j;
-                        const uint32_t y0 = j ? words.z : words.x, y1 = j ? words.w : words.y, h0 = y0 >> 8, h1 = y1 >> 8;
-                        const uint32_t z0 = j ? z_a.y : z_a.x, z1 = j ? z_b.y : z_b.x;
-                        const uint32_t a0[4] = {minus_zero<SUB, false>(y0, z0), minus_zero<SUB, true>(y0, z0), minus_zero<SUB, false>(y1, z1),
-                                                minus_zero<SUB, true>(y1, z1)};
-                        const uint32_t a1[4] = {minus_zero<SUB, false>(h0, z0), minus_zero<SUB, true>(h0, z0), minus_zero<SUB, false>(h1, z1),
-                                                minus_zero<SUB, true>(h1, z1)};
-                        const float s0 = __uint_as_float(j ? s_a.y : s_a.x), s1 = __uint_as_float(j ? s_b.y : s_b.x);
+                    for (int h = 0; h < 2; h++) {
+                        // pairs of the half's tokens 2t, 2t + 1 and 2t + 8, 2t + 9 for chunk 2i, then for chunk 2i + 1
+                        const uint4 words = load_matrices<true>(k_at[i] + to_stage + S::CODES + h * 16 * S::ROW_BYTES);
+                        const uint32_t s_at = sz + S::K_SZ + (16 * h + g) * (NCH * 4) + 8 * i, z_at = sz + S::K_SZ + S::V_S + (8 * h + t) * (NCH * 4) + 8 * i;
+                        const uint2 s_a = lds64(s_at), s_b = lds64(s_at + 8 * (NCH * 4));
+                        const uint2 z_a = lds64(z_at), z_b = lds64(z_at + 4 * (NCH * 4));
 #pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            float w0 = p[n][0] * s0, w1 = p[n][1] * s0, w2 = p[n][2] * s1, w3 = p[n][3] * s1;
-                            if constexpr (decltype(is_masked)::value) {  // a scale that is not finite stays with the rows that read its token
-                                w0 = p[n][0] == 0.0f ? 0.0f : w0, w1 = p[n][1] == 0.0f ? 0.0f : w1;
-                                w2 = p[n][2] == 0.0f ? 0.0f : w2, w3 = p[n][3] == 0.0f ? 0.0f : w3;
-                            }
-                            const uint32_t h01 = pack_halves(w0, w1), h23 = pack_halves(w2, w3);
-                            const uint32_t b0 = transpose8x8(h01), b1 = transpose8x8(h23);
-                            mma(o[c][0][n], a0, b0, b1);
-                            mma(o[c][1][n], a1, b0, b1);
-                            if constexpr (PARTS == 2) {
-                                const uint32_t l01 = pack_halves(w0 - half_lo(h01), w1 - half_hi(h01));
-                                const uint32_t l23 = pack_halves(w2 - half_lo(h23), w3 - half_hi(h23));
-                                const uint32_t c0 = transpose8x8(l01), c1 = transpose8x8(l23);
-                                mma(o[c][0][n], a0, c0, c1);
-                                mma(o[c][1][n], a1, c0, c1);
+                        for (int j = 0; j < 2; j++) {
+                            constexpr bool SUB = S::SUBNORMAL;
+                            const int c = 2 * i + j;
+                            const uint32_t y0 = j ? words.z : words.x, y1 = j ? words.w : words.y, h0 = y0 >> 8, h1 = y1 >> 8;
+                            const uint32_t z0 = j ? z_a.y : z_a.x, z1 = j ? z_b.y : z_b.x;
+                            const uint32_t a0[4] = {minus_zero<SUB, false>(y0, z0), minus_zero<SUB, true>(y0, z0), minus_zero<SUB, false>(y1, z1),
+                                                    minus_zero<SUB, true>(y1, z1)};
+                            const uint32_t a1[4] = {minus_zero<SUB, false>(h0, z0), minus_zero<SUB, true>(h0, z0), minus_zero<SUB, false>(h1, z1),
+                                                    minus_zero<SUB, true>(h1, z1)};
+                            const float s0 = __uint_as_float(j ? s_a.y : s_a.x), s1 = __uint_as_float(j ? s_b.y : s_b.x);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                const float(&pn)[4] = p[h][n];
+                                float w0 = pn[0] * s0, w1 = pn[1] * s0, w2 = pn[2] * s1, w3 = pn[3] * s1;
+                                if constexpr (decltype(is_masked)::value) {  // a scale that is not finite stays with the rows that read its token
+                                    w0 = pn[0] == 0.0f ? 0.0f : w0, w1 = pn[1] == 0.0f ? 0.0f : w1;
+                                    w2 = pn[2] == 0.0f ? 0.0f : w2, w3 = pn[3] == 0.0f ? 0.0f : w3;
+                                }
+                                const uint32_t h01 = pack_halves(w0, w1), h23 = pack_halves(w2, w3);
+                                const uint32_t b0 = transpose8x8(h01), b1 = transpose8x8(h23);
+                                mma(o[c][0][n], a0, b0, b1);
+                                mma(o[c][1][n], a1, b0, b1);
+                                if constexpr (PARTS == 2) {
+                                    const uint32_t l01 = pack_halves(w0 - half_lo(h01), w1 - half_hi(h01));
+                                    const uint32_t l23 = pack_halves(w2 - half_lo(h23), w3 - half_hi(h23));
+                                    const uint32_t c0 = transpose8x8(l01), c1 = transpose8x8(l23);
+                                    mma(o[c][0][n], a0, c0, c1);
+                                    mma(o[c][1][n], a1, c0, c1);
+                                }
                             }
                         }
                     }
