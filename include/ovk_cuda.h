@@ -594,7 +594,9 @@ OVK_API int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, const o
  * workspace: partial results of sequences that several CTAs share, 16-byte
  * aligned, ovk_attention_kv4_workspace() bytes; NULL takes the context's own
  * workspace, which grows on demand.  A call that is being captured into a graph
- * has to bring one, which replays of other graphs must not use at the same time. */
+ * has to bring one, which replays of other graphs must not use at the same time.
+ * The first 4096 bytes of a workspace are counters: zero them before its first
+ * call; every call leaves them zero (one that timed out may not). */
 OVK_API int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, const ovk_kv4_batch *batch,
                                   const ovk_heads *q, const ovk_heads *out, int32_t dtype,
                                   int64_t max_tokens, float scale, int64_t window, void *workspace,

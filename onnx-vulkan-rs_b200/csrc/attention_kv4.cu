@@ -28,7 +28,10 @@ Plan plan_for(int64_t head_dim, int tiles, bool f32)
 // second tile's products ride on the same unpacked codes.
 int tiles_for(int64_t max_tokens, int64_t group) { return max_tokens * group <= 8 ? 1 : 2; }
 
-size_t bytes_for(const Plan &p, int64_t ctas) { return size_t(ctas) * (sizeof(int4) + 2 * p.slot * sizeof(float)); }
+constexpr size_t COUNTERS = 4096;  // bytes: a counter per CTA
+static_assert(COUNTERS == OVK_KV4_COUNTERS * sizeof(unsigned int), "the context's counters");
+
+size_t bytes_for(const Plan &p, int64_t ctas) { return COUNTERS + size_t(ctas) * 2 * p.slot * sizeof(float); }
 
 int32_t check(ovk_ctx *ctx, const char *op, const ovk_kv4_cache *cache, int64_t q_heads, int64_t max_tokens, int32_t dtype)
 {
@@ -56,7 +59,7 @@ extern "C" int32_t ovk_attention_kv4_workspace(ovk_ctx *ctx, const ovk_kv4_cache
     *bytes = 0;
     for (int tiles = 1; tiles <= tiles_for(max_tokens, q_heads / cache->kv_heads); tiles++) {
         const Plan p = plan_for(cache->head_dim, tiles, dtype == OVK_FLOAT);
-        *bytes = std::max(*bytes, bytes_for(p, ctx->sm_count));
+        *bytes = std::max(*bytes, bytes_for(p, std::min(ctx->sm_count, OVK_KV4_COUNTERS)));
     }
     return OVK_OK;
 }
@@ -115,8 +118,9 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
     // no more CTAs than the longest sequences the block table has room for would fill
     const int64_t units = batch->max_pages * cache->page_size / p.unit + 2;
     const int64_t items = (batch->batch + ceil_div64(batch->tokens * a.group, 8 * tiles)) * cache->kv_heads;
-    const int64_t full = ctx->sm_count;
+    const int64_t full = std::min(ctx->sm_count, OVK_KV4_COUNTERS);
     const int64_t ctas = items >= full || units >= full ? full : std::min(full, units * items);
+    const bool own = !workspace;
     if (workspace) {
         OVK_REQUIRE(ctx, aligned_to(workspace, 16) && workspace_bytes >= bytes_for(p, ctas),
                     "%s: a workspace of %zu bytes at %p, %zu are needed on a 16-byte boundary", op, workspace_bytes, workspace,
@@ -131,8 +135,8 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
         if (rc != OVK_OK)
             return rc;
     }
-    a.meta = static_cast<int4 *>(workspace);
-    a.partial = reinterpret_cast<float *>(a.meta + ctas);
+    a.counters = own ? ctx->kv4_counters : static_cast<unsigned int *>(workspace);
+    a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + COUNTERS);
     return cache->head_dim == 64    ? ovk_kv4_launch_64(ctx, a, dtype, tiles, int(ctas))
            : cache->head_dim == 128 ? ovk_kv4_launch_128(ctx, a, dtype, tiles, int(ctas))
                                     : ovk_kv4_launch_256(ctx, a, dtype, tiles, int(ctas));

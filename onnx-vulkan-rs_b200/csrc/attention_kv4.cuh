@@ -40,8 +40,9 @@
 // have any size, and go on with the next sequence while the consumers finish one.
 // (Tensor and bulk copies, six to a page of 16 tokens, were issued too slowly: 70
 // instead of 37 us for 48 contexts of 4000.)  A run that begins or ends inside a
-// sequence leaves a partial result; a second kernel joins those in CTA order, so
-// results do not depend on timing.
+// sequence leaves a partial result, and the CTA that is the last to leave one of a
+// sequence joins them, always in CTA order, so results do not depend on timing.  (A
+// second kernel for that cost 5 us a call.)
 #pragma once
 
 #include <type_traits>
@@ -62,7 +63,7 @@ struct Kv4Args {
     int blocks, chunk_shift;  // scales a row; log2(block_size / 32)
     float scale_log2e;
     float *partial;
-    int4 *meta;
+    unsigned int *counters;  // one per CTA, zero between calls
     int *status;
 };
 
@@ -178,6 +179,9 @@ template <bool SUBNORMAL, bool SECOND> __device__ __forceinline__ uint32_t minus
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// 2^k for -126 <= k <= 127
+__device__ __forceinline__ float power_of_two(int k) { return __uint_as_float(uint32_t(k + 127) << 23); }
+
 // a / b for b > 0; 64-bit divisions cost a hundred instructions, so the usual sizes take a 32-bit one
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b)
 {
@@ -196,6 +200,10 @@ struct Shares {
         return unit < large ? divide(unit, base + 1) : more + divide(unit - large, base);
     }
 };
+
+// What a CTA spends on an item beside its units - query fragments, the join of the warps - in units: the
+// shares count it with each item, so that CTAs that work on two items end with the others.
+constexpr int ITEM_COST = 2;
 
 // What the sequence arrays say about sequence b.
 struct Sequence {
@@ -259,6 +267,26 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
     return false;
 }
 
+// A part of an item that other CTAs have parts of too.
+struct Part {
+    int first_cta, count;  // the CTAs that have one; count 0: no such part
+    int first_row, row0, rows, head;
+};
+
+// Four elements of a result row: the item's row `row` is query head row % group of the key head, of the
+// sequence's new token row / group.
+template <typename T>
+__device__ __forceinline__ void write_out(const Kv4Args &a, int first_row, int row, int head, int d, float4 v, float sum)
+{
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int token = row / a.group;
+    T *dst = static_cast<T *>(a.out) + int64_t(first_row + token) * a.o_token + (int64_t(head) * a.group + (row - token * a.group)) * a.o_head + d;
+    if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4 *>(dst) = make_float4(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
+    else
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_halves(v.x * inverse, v.y * inverse), pack_halves(v.z * inverse, v.w * inverse));
+}
+
 template <typename T, int D, int NT, int PARTS>
 __global__ void __launch_bounds__(Shape<D, NT, PARTS>::THREADS, 1)
 attention_kv4_kernel(const __grid_constant__ Kv4Args a)
@@ -270,6 +298,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
     __shared__ int64_t warp_sums[THREADS / 32], found[2];
     __shared__ uint64_t full[STAGES], empty[STAGES];
     __shared__ int dead_word;
+    __shared__ bool last_part;
     volatile int *const dead = &dead_word;
     const uint32_t ring = (umma::smem_u32(smem_raw) + 127u) & ~127u;
     uint8_t *const smem = smem_raw + (ring - umma::smem_u32(smem_raw));
@@ -283,7 +312,6 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
 
     OVK_PDL_LAUNCH_DEPENDENTS();
     if (tid == 0) {
-        a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
         dead_word = 0;
         for (int i = 0; i < STAGES; i++) {
             umma::mbar_init(&full[i], 4 * 33);  // the producers' lanes, and one of each warp again for what it stores itself
@@ -291,6 +319,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         }
         umma::fence_barrier_init();
     }
+    OVK_PDL_WAIT();
 
     // ------------------------------------------------ this CTA's run of units
     // A scan over the batch, a sequence a thread; more sequences than threads take a pass for the total first.
@@ -298,7 +327,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         if (b >= a.batch)
             return 0;
         const Sequence s = sequence<ROWS, UNIT>(a, b, report);
-        return int64_t(s.units) * s.tiles * a.kv_heads;
+        return int64_t(s.units > 0 ? s.units + ITEM_COST : 0) * s.tiles * a.kv_heads;
     };
     // the units of this thread's sequence and those before it in the chunk; the chunk's total
     auto scan = [&](int64_t own, int64_t &before) -> int64_t {
@@ -350,13 +379,17 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
     __syncthreads();
     int b = int(found[0]);
     Sequence seq = sequence<ROWS, UNIT>(a, b, false);
-    int item = int(divide(at - found[1], seq.units)), unit = int(at - found[1] - int64_t(item) * seq.units);
-    // both kinds of warps walk the run's segments - a piece of one item - with this
-    auto next_segment = [&](int units_here) {
-        at += units_here;
+    int item = int(divide(at - found[1], seq.units + ITEM_COST));
+    int64_t item_at = found[1] + int64_t(item) * (seq.units + ITEM_COST);  // where the item begins; its units lie behind its cost
+    // both kinds of warps walk the run's segments - a piece of one item, possibly without a unit - with this
+    auto segment = [&](int &unit) -> int {
+        unit = int(max(int64_t(0), at - item_at - ITEM_COST));
+        return int(min(int64_t(seq.units), end - item_at - ITEM_COST)) - unit;
+    };
+    auto next_segment = [&]() {
+        at = item_at += seq.units + ITEM_COST;
         if (at >= end)
             return false;
-        unit = 0;
         if (++item == seq.tiles * a.kv_heads) {
             item = 0;
             do {
@@ -376,7 +409,10 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         uint32_t phase = 0;
         bool ok = true;
         do {
-            const int units_here = int(min(int64_t(seq.units - unit), end - at));
+            int unit;
+            const int units_here = segment(unit);
+            if (units_here <= 0)
+                continue;
             const int head = item % a.kv_heads;
             const int first = seq.start + unit * UNIT + 32 * producer + lane, t_end = min(seq.len, seq.start + (unit + units_here) * UNIT);
             const int32_t *const table = a.table + int64_t(b) * a.max_pages;
@@ -449,7 +485,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 if (++stage == STAGES)
                     stage = 0, phase ^= 1;
             }
-        } while (ok && next_segment(int(min(int64_t(seq.units - unit), end - at))));
+        } while (ok && next_segment());
         asm volatile("cp.async.wait_all;" ::: "memory");
         return;
     }
@@ -458,8 +494,15 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::REGS));
     int stage = 0;
     uint32_t phase = 0;
+    Part parts[2] = {};  // of an item that began before, and of one that goes on behind, this CTA's run
     while (true) {
-        const int units_here = int(min(int64_t(seq.units - unit), end - at));
+        int unit;
+        const int units_here = segment(unit);
+        if (units_here <= 0) {
+            if (!next_segment())
+                break;
+            continue;
+        }
         const int tile = item / a.kv_heads, head = item - tile * a.kv_heads;
         const int rows = min(ROWS, seq.n * a.group - tile * ROWS);
         const int t_begin = seq.start + unit * UNIT;
@@ -496,7 +539,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
             // a power of two brings the row's largest value to 2^10 .. 2^11, clear of fp16's ends
             const int exponent = int(__float_as_uint(top) >> 23);
             const int k = (exponent == 255 || top == 0.0f) ? 0 : 10 - (exponent - 127);
-            const float f1 = ldexpf(1.0f, k / 2), f2 = ldexpf(1.0f, k - k / 2);
+            const float f1 = power_of_two(k / 2), f2 = power_of_two(k - k / 2);
 #pragma unroll
             for (int i = 0; i < GROUPS; i++) {
                 const int c = (j + 8 * i) >> 2;
@@ -524,7 +567,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                     q_sum[c * ROWS + r] = -sum;  // K's accumulators start at zero times this
             }
             if (j == 0)
-                q_factor[r] = ldexpf(a.scale_log2e, (S::SUBNORMAL ? 24 : 0) - k);
+                q_factor[r] = a.scale_log2e * power_of_two(-(k / 2)) * power_of_two((S::SUBNORMAL ? 24 : 0) - (k - k / 2));
         }
         consumers_sync<CONSUMERS>();
         uint4 bq[S::Q_REGS ? PARTS : 1][S::Q_REGS ? NT : 1][S::Q_REGS ? NCH : 1];
@@ -892,8 +935,8 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
             consumers_sync<CONSUMERS>();
         }
         const bool whole = unit == 0 && units_here == seq.units;
-        const int which = unit == 0 ? 1 : 0;  // a partial result that begins an item, or goes on with one
-        float *const slot = a.partial + (int64_t(blockIdx.x) * 2 + which) * S::SLOT;
+        // a CTA has at most two parts: one that goes on with an item (slot 0), one that begins an item (slot 1)
+        float *const slot = a.partial + (int64_t(blockIdx.x) * 2 + (unit == 0 ? 1 : 0)) * S::SLOT;
         for (int i = tid; i < rows * (D / 4); i += CONSUMERS) {
             const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
             float most = NONE, sum = 0.0f;
@@ -910,97 +953,74 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
             }
             if (whole) {
-                const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const int row = row0 + r, token = row / a.group;
-                T *dst = static_cast<T *>(a.out) + int64_t(seq.first + token) * a.o_token +
-                         (int64_t(head) * a.group + (row - token * a.group)) * a.o_head + d;
-                if constexpr (sizeof(T) == 4)
-                    *reinterpret_cast<float4 *>(dst) = make_float4(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
-                else
-                    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_halves(v.x * inverse, v.y * inverse),
-                                                                 pack_halves(v.z * inverse, v.w * inverse));
+                write_out<T>(a, seq.first, row0 + r, head, d, v, sum);
             } else {
                 *reinterpret_cast<float4 *>(slot + r * D + d) = v;
-                if (d == 0) {
-                    slot[ROWS * D + 2 * r] = most;
-                    slot[ROWS * D + 2 * r + 1] = sum;
-                }
+                if (d == 0)
+                    *reinterpret_cast<float2 *>(slot + ROWS * D + 2 * r) = make_float2(most, sum);
             }
         }
-        if (!whole && which == 1 && tid == 0) {
-            // the CTAs that hold the rest of this item: the last is the one with its last unit
-            const int64_t last_unit = at - unit + seq.units - 1;
-            a.meta[blockIdx.x] = make_int4(int(shares.holder(last_unit)) + 1 - int(blockIdx.x), b, tile, head);
+        if (!whole) {
+            // the CTAs that hold this item: from the one that has its first unit to the one that has its last
+            Part &part = parts[unit == 0 ? 1 : 0];
+            part.first_cta = int(shares.holder(item_at + ITEM_COST));
+            part.count = int(shares.holder(item_at + ITEM_COST + seq.units - 1)) - part.first_cta + 1;
+            part.first_row = seq.first, part.row0 = row0, part.rows = rows, part.head = head;
         }
-        if (!next_segment(units_here))
+        if (!next_segment())
             break;
     }
-}
 
-// Joins the partial results of items that lie in several CTAs: block (cta, row) takes the item that
-// begins in `cta` and goes on behind it, if there is one, and adds its parts in CTA order.
-constexpr int JOIN_THREADS = 256;
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(JOIN_THREADS) attention_kv4_join_kernel(const __grid_constant__ Kv4Args a)
-{
-    constexpr int LANES = D / 4, GROUPS = JOIN_THREADS / LANES, SLOT = ROWS * (D + 2);
-    __shared__ float4 sums[GROUPS][LANES];
-    __shared__ float tops[JOIN_THREADS / 32], group_sum[GROUPS];
-    OVK_PDL_WAIT();
-    const int4 meta = a.meta[blockIdx.x];
-    const int count = meta.x, b = meta.y, tile = meta.z, head = meta.w, r = blockIdx.y;
-    if (count == 0)
-        return;
-    const int first = a.cu[b], n = a.cu[b + 1] - first;
-    const int row = tile * ROWS + r;
-    if (row >= n * a.group)
-        return;
-    const int tid = threadIdx.x;
-    auto part = [&](int i) { return a.partial + (int64_t(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * SLOT; };
-    float most = NONE;
-    for (int i = tid; i < count; i += JOIN_THREADS)
-        most = fmaxf(most, part(i)[ROWS * D + 2 * r]);
+    // ------------------------------------------- join items, where this CTA is the last to have left its part
+#pragma unroll 1
+    for (int which = 0; which < 2; which++) {
+        const Part part = parts[which];
+        if (part.count == 0)
+            continue;
+        __threadfence();
+        consumers_sync<CONSUMERS>();
+        if (tid == 0) {
+            last_part = atomicAdd(&a.counters[part.first_cta], 1u) == unsigned(part.count - 1);
+            if (last_part)
+                a.counters[part.first_cta] = 0;
+        }
+        consumers_sync<CONSUMERS>();
+        if (!last_part)
+            continue;
+        __threadfence();
+        // a lane of sixteen fetches the maximum and sum of one part, and all of them their elements of sixteen parts
+        const uint32_t half = (lane & 16) ? 0xffff0000u : 0x0000ffffu;
+        for (int i = tid; i < part.rows * (D / 4); i += CONSUMERS) {
+            const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+            float top = NONE, sum = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int base = 0; base < part.count; base += 16) {
+                auto slot_of = [&](int k) { return a.partial + (int64_t(part.first_cta + k) * 2 + (k == 0 ? 1 : 0)) * S::SLOT; };
+                float2 ml = make_float2(NONE, 0.0f);
+                if (base + (lane & 15) < part.count)
+                    ml = __ldcg(reinterpret_cast<const float2 *>(slot_of(base + (lane & 15)) + ROWS * D + 2 * r));
+                float4 u[16];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if ((tid & 31) == 0)
-        tops[tid >> 5] = most;
-    __syncthreads();
+                for (int k = 0; k < 16; k++)
+                    u[k] = base + k < part.count ? __ldcg(reinterpret_cast<const float4 *>(slot_of(base + k) + r * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float most = ml.x;
 #pragma unroll
-    for (int w = 0; w < JOIN_THREADS / 32; w++)
-        most = fmaxf(most, tops[w]);
-    const int lane = tid % LANES, group = tid / LANES;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-#pragma unroll 4
-    for (int i = group; i < count; i += GROUPS) {
-        const float *p = part(i);
-        const float4 u = reinterpret_cast<const float4 *>(p + r * D)[lane];
-        const float w = exp2_approx(p[ROWS * D + 2 * r] - most);
-        sum = fmaf(w, p[ROWS * D + 2 * r + 1], sum);
-        v.x = fmaf(w, u.x, v.x), v.y = fmaf(w, u.y, v.y), v.z = fmaf(w, u.z, v.z), v.w = fmaf(w, u.w, v.w);
+                for (int o = 1; o < 16; o <<= 1)
+                    most = fmaxf(most, __shfl_xor_sync(half, most, o));
+                const float to = fmaxf(top, most), f = exp2_approx(top - to), mine = exp2_approx(ml.x - to);
+                top = to;
+                sum *= f;
+                v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const float w = __shfl_sync(half, mine, k, 16);
+                    sum = fmaf(w, __shfl_sync(half, ml.y, k, 16), sum);
+                    v.x = fmaf(w, u[k].x, v.x), v.y = fmaf(w, u[k].y, v.y), v.z = fmaf(w, u[k].z, v.z), v.w = fmaf(w, u[k].w, v.w);
+                }
+            }
+            write_out<T>(a, part.first_row, part.row0 + r, part.head, d, v, sum);
+        }
     }
-    sums[group][lane] = v;
-    if (lane == 0)
-        group_sum[group] = sum;
-    __syncthreads();
-    if (group != 0)
-        return;
-    sum = group_sum[0];
-#pragma unroll
-    for (int i = 1; i < GROUPS; i++) {
-        const float4 u = sums[i][lane];
-        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-        sum += group_sum[i];
-    }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int token = row / a.group;
-    T *dst = static_cast<T *>(a.out) + int64_t(first + token) * a.o_token +
-             (int64_t(head) * a.group + (row - token * a.group)) * a.o_head + 4 * lane;
-    if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<float4 *>(dst) = make_float4(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
-    else
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_halves(v.x * inverse, v.y * inverse), pack_halves(v.z * inverse, v.w * inverse));
 }
 
 template <typename T, int D, int NT> int32_t launch(ovk_ctx *ctx, const Kv4Args &a, int ctas)
@@ -1008,13 +1028,8 @@ template <typename T, int D, int NT> int32_t launch(ovk_ctx *ctx, const Kv4Args 
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     using S = Shape<D, NT, PARTS>;
     OVK_CUDA(ctx, ovk_allow_smem(attention_kv4_kernel<T, D, NT, PARTS>, S::SMEM, ctx->device));
-    attention_kv4_kernel<T, D, NT, PARTS><<<ctas, S::THREADS, S::SMEM, ctx->stream>>>(a);
+    OVK_CUDA(ctx, ovk_launch_pdl(attention_kv4_kernel<T, D, NT, PARTS>, dim3(unsigned(ctas)), dim3(S::THREADS), S::SMEM, ctx->stream, a));
     OVK_LAUNCHED(ctx, NT == 1 ? "attention_kv4" : "attention_kv4_rows16");
-    if (ctas > 1) {
-        OVK_CUDA(ctx, ovk_launch_pdl(attention_kv4_join_kernel<T, D, S::ROWS>, dim3(unsigned(ctas - 1), S::ROWS), dim3(JOIN_THREADS), 0,
-                                     ctx->stream, a));
-        ctx->launches++;
-    }
     return OVK_OK;
 }
 

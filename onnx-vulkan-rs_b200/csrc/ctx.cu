@@ -84,6 +84,8 @@ int32_t ovk_ctx_create(int32_t device, void *stream, ovk_ctx **out)
     }
     CTX_CUDA(cudaMalloc(&ctx->range_slot, 256));
     CTX_CUDA(cudaMalloc(&ctx->dev_status, 256));
+    CTX_CUDA(cudaMalloc(&ctx->kv4_counters, OVK_KV4_COUNTERS * sizeof(uint32_t)));
+    CTX_CUDA(cudaMemset(ctx->kv4_counters, 0, OVK_KV4_COUNTERS * sizeof(uint32_t)));
     CTX_CUDA(cudaMalloc(&ctx->params, OVK_PARAM_FLOATS * sizeof(float)));
     CTX_CUDA(cudaMemset(ctx->dev_status, 0, 256));
     CTX_CUDA(cudaMemset(ctx->range_slot, 0, 256));  // DynamicQuantizeLinear leaves it zeroed after every call
@@ -108,6 +110,7 @@ void ovk_ctx_destroy(ovk_ctx *ctx)
     cudaFree(ctx->dev_status);
     cudaFree(ctx->params);
     cudaFree(ctx->tile_counters);
+    cudaFree(ctx->kv4_counters);
     cudaFreeHost(ctx->host_status);
     cudaEventDestroy(ctx->t0);
     cudaEventDestroy(ctx->t1);
@@ -134,6 +137,7 @@ int32_t ovk_flush(ovk_ctx *ctx)
     if (st != OVK_DEV_OK) {
         OVK_CUDA(ctx, cudaMemsetAsync(ctx->dev_status, 0, sizeof(int), ctx->stream));
         OVK_CUDA(ctx, cudaMemsetAsync(ctx->range_slot, 0, 256, ctx->stream));  // a launch that gave up may have left counts
+        OVK_CUDA(ctx, cudaMemsetAsync(ctx->kv4_counters, 0, OVK_KV4_COUNTERS * sizeof(uint32_t), ctx->stream));
         if (st == OVK_DEV_BAD_INDEX)
             return ovk_fail(ctx, OVK_INVALID_ARGUMENT,
                             "GatherBlockQuantized: an index read on the device fell outside the table "

@@ -58,10 +58,12 @@ struct ovk_ctx {
     // MatMulNBits prefill with K ranges shared between CTAs: one arrival counter per output tile,
     // zero between launches (the CTA that arrives last at a tile resets it)
     uint32_t *tile_counters = nullptr;
+    uint32_t *kv4_counters = nullptr;  // attention over the 4-bit cache: OVK_KV4_COUNTERS arrival counters, zero between launches
     int mmi_pairs = -1;    // the same for the 256-row MatMulInteger kernel
     int nbits_pairs = -1;  // pairs of CTAs the MatMulNBits prefill kernel can run at once (-1: not asked yet)
 };
 constexpr int OVK_TILE_COUNTERS = 65536;
+constexpr int OVK_KV4_COUNTERS = 1024;
 
 constexpr int OVK_PARAM_FLOATS = 16384;
 

@@ -766,6 +766,7 @@ class Context:
             self.check(lib().ovk_attention_kv4_workspace(self.h, cache.params, h, max_tokens, code, C.byref(size)))
             need = size.value
             space = torch.empty(need, dtype=torch.uint8, device=q.device)
+            space[:4096].zero_()
         self.check(self._fast.ovk_attention_kv4(self.h, cache.packed, b, _PACK_HEADS(*hq), _PACK_HEADS(*ho), code, max_tokens,
                                                 cache.head_dim ** -0.5 if scale is None else scale, window,
                                                 None if space is None else space.data_ptr(), need))
