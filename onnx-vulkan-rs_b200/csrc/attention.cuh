@@ -83,10 +83,14 @@ int32_t ovk_check_kv4(ovk_ctx *ctx, const char *op, const ovk_kv4_cache *c);
 int32_t ovk_check_kv4_batch(ovk_ctx *ctx, const char *op, const ovk_kv4_batch *b);
 
 #ifdef __CUDACC__
-// The index of the sequence that holds packed row `token`, or -1: the last b with cu[b] <= token, if
-// its end lies behind it (empty sequences share their start with the next one).
-__device__ __forceinline__ int sequence_of(const int32_t *__restrict__ cu, int batch, int token)
+// The index of the sequence that holds packed row `token` of `tokens`, or -1: the last b with cu[b] <= token,
+// if its end lies behind it (empty sequences share their start with the next one).  Where the sequences bring
+// about as many rows each - one in decode - the first place looked at is the right one.
+__device__ __forceinline__ int sequence_of(const int32_t *__restrict__ cu, int batch, int token, int tokens)
 {
+    const int guess = int(int64_t(token) * batch / tokens);  // batch < 2^24
+    if (guess < batch && cu[guess] <= token && token < cu[guess + 1])
+        return guess;
     int lo = 0, hi = batch;  // cu[lo] <= token < cu[hi] once both are inside
     if (token < cu[0] || token >= cu[batch])
         return -1;

@@ -4,16 +4,20 @@
 //   x[i][j] = scale * q[i] . k[j],  out[i] = sum_j 2^(x log2 e - m) v[j] / sum_j 2^(x log2 e - m),
 //
 // one pass over the keys with the running maximum m and sum of each row.  A block
-// of 256 threads holds 64 query rows of one head and walks 64 keys at a time; a
-// thread computes 4 x 4 scores, then 4 rows x head_dim / 16 columns of the result.
-// All of it is f32 arithmetic on the CUDA cores: with Q and K transposed in shared
-// memory a step over d is two 16-byte loads for 16 multiply-adds, so the adders
-// and not shared memory bound it.
+// holds 64 query rows of one head and walks 64 keys at a time; a thread computes 8
+// (256-wide heads: 4) x 4 scores, then as many rows x head_dim / 16 columns of the
+// result.  All of it is f32 arithmetic on the CUDA cores: with Q and K transposed in
+// shared memory a step over d is three 16-byte loads for 32 multiply-adds, so the
+// adders and not shared memory bound it.
 #include "attention_prompt.cuh"
 
 namespace {
 
-constexpr int BM = 64, BN = 64, THREADS = 256, PITCH = BM + 4;
+constexpr int BM = 64, BN = 64, PITCH = BM + 4;
+
+// rows of a thread: eight (128 threads) where the registers hold their results
+template <int DMAX> constexpr int rows_of() { return DMAX == 256 ? 4 : 8; }
+template <int DMAX> constexpr int threads_of() { return BM / rows_of<DMAX>() * 16; }
 
 template <int DMAX> constexpr size_t simt_smem() { return size_t(2 * DMAX * PITCH + BN * DMAX + BN * PITCH) * 4; }
 
@@ -21,10 +25,11 @@ template <int DMAX> constexpr size_t simt_smem() { return size_t(2 * DMAX * PITC
 template <typename T, int DMAX>
 __device__ __forceinline__ void load_transposed(float *t, const T *base, int64_t stride, int rows, int d, bool vec)
 {
-    const int r = threadIdx.x >> 2, part = threadIdx.x & 3;
+    constexpr int V = 16 / sizeof(T), PARTS = threads_of<DMAX>() / BM;  // threads of a row
+    const int r = threadIdx.x / PARTS, part = threadIdx.x % PARTS;
     const T *src = base + int64_t(r) * stride;
-    constexpr int V = 16 / sizeof(T);
-    for (int e = part * V; e < DMAX; e += 4 * V) {
+#pragma unroll 4
+    for (int e = part * V; e < DMAX; e += PARTS * V) {
         float v[V];
         if (r < rows && vec && e + V <= d) {
             load_row<T, V, true>(src + e, v);
@@ -40,8 +45,9 @@ __device__ __forceinline__ void load_transposed(float *t, const T *base, int64_t
 }
 
 template <typename T, int DMAX>
-__global__ void __launch_bounds__(THREADS) attention_prompt_simt_kernel(const PromptArgs a)
+__global__ void __launch_bounds__(threads_of<DMAX>()) attention_prompt_simt_kernel(const PromptArgs a)
 {
+    constexpr int RT = rows_of<DMAX>(), THREADS = threads_of<DMAX>();
     extern __shared__ __align__(16) float sm[];
     float *const qt = sm, *const kt = qt + DMAX * PITCH, *const vs = kt + DMAX * PITCH, *const pt = vs + BN * DMAX;
     __shared__ PromptTile where;
@@ -62,9 +68,9 @@ __global__ void __launch_bounds__(THREADS) attention_prompt_simt_kernel(const Pr
     load_transposed<T, DMAX>(qt, q, a.q_token, rows, D, a.vec);
 
     constexpr int OC = DMAX / 64;
-    float o[4][OC][4], m[4], l[4];
+    float o[RT][OC][4], m[RT], l[RT];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < RT; i++) {
         m[i] = -1e30f, l[i] = 0.0f;
 #pragma unroll
         for (int c = 0; c < OC; c++)
@@ -96,25 +102,30 @@ __global__ void __launch_bounds__(THREADS) attention_prompt_simt_kernel(const Pr
             }
         }
         odd_value = __syncthreads_or(odd_value);
-        float s[4][4];
+        float s[RT][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < RT; i++)
             s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
 #pragma unroll 8
         for (int d = 0; d < DMAX; d++) {
-            const float4 x = *reinterpret_cast<const float4 *>(qt + d * PITCH + ty * 4);
-            const float4 y = *reinterpret_cast<const float4 *>(kt + d * PITCH + tx * 4);
-            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+            float xs[RT];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < RT; i += 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(qt + d * PITCH + ty * RT + i);
+                xs[i] = x.x, xs[i + 1] = x.y, xs[i + 2] = x.z, xs[i + 3] = x.w;
+            }
+            const float4 y = *reinterpret_cast<const float4 *>(kt + d * PITCH + tx * 4);
+            const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < RT; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     s[i][j] = fmaf(xs[i], ys[j], s[i][j]);
         }
         const bool masked = keys < BN || (a.causal && j0 + BN - 1 > first) || (a.window > 0 && j0 <= first + rows - 1 - a.window);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int64_t p = first + ty * 4 + i;
+        for (int i = 0; i < RT; i++) {
+            const int64_t p = first + ty * RT + i;
             float most = -1e30f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -143,15 +154,17 @@ __global__ void __launch_bounds__(THREADS) attention_prompt_simt_kernel(const Pr
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            *reinterpret_cast<float4 *>(pt + (tx * 4 + j) * PITCH + ty * 4) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+#pragma unroll
+            for (int i = 0; i < RT; i += 4)
+                *reinterpret_cast<float4 *>(pt + (tx * 4 + j) * PITCH + ty * RT + i) = make_float4(s[i][j], s[i + 1][j], s[i + 2][j], s[i + 3][j]);
         __syncthreads();
         if (masked && odd_value) {
             // 0 times an infinity is NaN: rows that do not read a key skip it
             for (int n = 0; n < keys; n++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float p = pt[n * PITCH + ty * 4 + i];
-                    const int64_t key = j0 + n, at = first + ty * 4 + i;
+                for (int i = 0; i < RT; i++) {
+                    const float p = pt[n * PITCH + ty * RT + i];
+                    const int64_t key = j0 + n, at = first + ty * RT + i;
                     if ((a.causal && key > at) || (a.window > 0 && key <= at - a.window))
                         continue;
 #pragma unroll
@@ -164,13 +177,17 @@ __global__ void __launch_bounds__(THREADS) attention_prompt_simt_kernel(const Pr
         }
 #pragma unroll 4
         for (int n = 0; n < BN; n++) {
-            const float4 x = *reinterpret_cast<const float4 *>(pt + n * PITCH + ty * 4);
-            const float xs[4] = {x.x, x.y, x.z, x.w};
+            float xs[RT];
+#pragma unroll
+            for (int i = 0; i < RT; i += 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(pt + n * PITCH + ty * RT + i);
+                xs[i] = x.x, xs[i + 1] = x.y, xs[i + 2] = x.z, xs[i + 3] = x.w;
+            }
 #pragma unroll
             for (int c = 0; c < OC; c++) {
                 const float4 y = *reinterpret_cast<const float4 *>(vs + n * DMAX + c * 64 + tx * 4);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < RT; i++) {
                     o[i][c][0] = fmaf(xs[i], y.x, o[i][c][0]);
                     o[i][c][1] = fmaf(xs[i], y.y, o[i][c][1]);
                     o[i][c][2] = fmaf(xs[i], y.z, o[i][c][2]);
@@ -180,8 +197,8 @@ __global__ void __launch_bounds__(THREADS) attention_prompt_simt_kernel(const Pr
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = ty * 4 + i;
+    for (int i = 0; i < RT; i++) {
+        const int r = ty * RT + i;
         float sum = l[i];
 #pragma unroll
         for (int x = 1; x < 16; x <<= 1)
@@ -205,7 +222,7 @@ template <typename T, int DMAX> int32_t launch_simt(ovk_ctx *ctx, const PromptAr
 {
     constexpr size_t smem = simt_smem<DMAX>();
     OVK_CUDA(ctx, ovk_allow_smem(attention_prompt_simt_kernel<T, DMAX>, smem, ctx->device));
-    attention_prompt_simt_kernel<T, DMAX><<<dim3(tiles, unsigned(a.heads)), THREADS, smem, ctx->stream>>>(a);
+    attention_prompt_simt_kernel<T, DMAX><<<dim3(tiles, unsigned(a.heads)), threads_of<DMAX>(), smem, ctx->stream>>>(a);
     OVK_LAUNCHED(ctx, sizeof(T) == 4 ? "attention_prompt_f32" : "attention_prompt_simt");
     return OVK_OK;
 }

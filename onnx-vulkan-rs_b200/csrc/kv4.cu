@@ -6,10 +6,11 @@
 // of a row go through the same thread, so its place in the cache is found once.
 //
 // The quotients are rounded exactly without dividing: for an fp16 scale s and an
-// integer n <= 16, (n + 1/2) s has at most 16 significant bits, so the sign of
-// fma(-(n + 1/2), s, x) is the sign of x / s - (n + 1/2), and a first guess
-// n = rint(x * (1 / s)), off by at most one, is set right by the two borders
-// around it.  The scale itself is one f64 quotient a block.
+// integer n <= 16, n s has at most 16 significant bits, and the rest r = x - n s of
+// a value within a step of n s is a whole number of units of its last place that
+// fits 24 bits - so fma(-n, s, x) is r exactly, and a first guess n = rint(x * (1 /
+// s)), off by at most one, is set right by comparing |r| with s / 2.  The scale
+// itself is one f64 quotient a block, keys' on the even lanes and values' on the odd.
 #include "attention.cuh"
 
 int32_t ovk_check_kv4(ovk_ctx *ctx, const char *op, const ovk_kv4_cache *c)
@@ -57,20 +58,19 @@ struct AppendArgs {
     uint8_t *zero_points[2];
     const int32_t *cu, *lens, *table;
     int64_t items;  // tokens * heads * head_dim / 8
-    int batch, heads, head_dim, block_size, page_size, pages;
+    int tokens, batch, heads, head_dim, word_shift, block_size, page_size, pages;
     int64_t max_pages;
     int *status;
 };
 
-// round-to-nearest-even of x / s for an fp16 value s > 0, clamped to +-16; inv is about 1 / s
-__device__ __forceinline__ int quotient(float x, float s, float inv)
+// x / s rounded to the nearest integer, ties to even, as a float; inv is about 1 / s, half is s / 2 (infinity where s is 0:
+// then the quotient counts as 0).  Beyond +-2^22 the result is only large.
+__device__ __forceinline__ float quotient(float x, float s, float inv, float half)
 {
-    const float guess = fminf(fmaxf(rintf(x * inv), -16.0f), 16.0f);
-    const float above = fmaf(-(guess + 0.5f), s, x);  // > 0: x / s lies above the upper border
-    const float below = fmaf(-(guess - 0.5f), s, x);  // < 0: below the lower one
-    const int n = int(guess);
-    const bool odd = n & 1;
-    return n + (above > 0.0f || (above == 0.0f && odd) ? 1 : 0) - (below < 0.0f || (below == 0.0f && odd) ? 1 : 0);
+    const float magic = 12582912.0f;  // 1.5 * 2^23: the sum's last bits are the integer
+    const float t = fmaf(x, inv, magic), n = t - magic, rest = fmaf(-n, s, x), off = fabsf(rest);
+    const bool moves = off > half || (off == half && (__float_as_uint(t) & 1u));
+    return moves ? n + copysignf(1.0f, rest) : n;
 }
 
 template <typename T, bool VEC>
@@ -78,12 +78,13 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
 {
     const int64_t item = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
     const int words = a.head_dim / 8;  // a power of two up to 32: a row lies inside a warp
-    const int64_t at = item / words;
-    const int word = int(item - at * words);
-    const int token = int(at / a.heads), head = int(at - int64_t(token) * a.heads);
+    // tokens x heads < 2^31
+    const uint32_t at = uint32_t(item >> a.word_shift);
+    const int word = int(item & (words - 1));
+    const int token = int(at / uint32_t(a.heads)), head = int(at - uint32_t(token) * a.heads);
     int64_t row = -1;
     if (item < a.items) {
-        const int b = sequence_of(a.cu, a.batch, token);
+        const int b = sequence_of(a.cu, a.batch, token, a.tokens);
         if (b >= 0) {
             const int64_t position = int64_t(a.lens[b]) - (int64_t(a.cu[b + 1]) - token);
             const int64_t page = position < 0 ? a.max_pages : position / a.page_size;
@@ -107,29 +108,36 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
                 x[j][e] = 0.0f;
         }
     }
+    float lo[2] = {0.0f, 0.0f}, hi[2] = {0.0f, 0.0f};  // fminf and fmaxf drop a NaN
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-        float lo = 0.0f, hi = 0.0f;  // fminf and fmaxf drop a NaN
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            lo = fminf(lo, x[j][e]), hi = fmaxf(hi, x[j][e]);
+            lo[j] = fminf(lo[j], x[j][e]), hi[j] = fmaxf(hi[j], x[j][e]);
         for (int o = 1; o < lanes; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            lo[j] = fminf(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], o));
+            hi[j] = fmaxf(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], o));
         }
-        const double step = a.zero_points[j] ? (double(hi) - double(lo)) / 15.0 : fmax(double(hi) / 7.0, -double(lo) / 8.0);
-        const __half scale = __float2half_rn(fminf(float(step), 65504.0f));
+    }
+    const int mine = threadIdx.x & 1;
+    const double top = mine ? hi[1] : hi[0], low = mine ? lo[1] : lo[0];
+    const double step = a.zero_points[0] ? (top - low) / 15.0 : fmax(top / 7.0, -low / 8.0);
+    const float my_scale = fminf(float(step), 65504.0f), other_scale = __shfl_xor_sync(0xffffffffu, my_scale, 1);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const __half scale = __float2half_rn(mine == j ? my_scale : other_scale);
         const float s = __half2float(scale);
-        const float inv = s > 0.0f ? 1.0f / s : 0.0f;  // a scale is at least 2^-24: finite
-        int zero = 8;
+        const float inv = s > 0.0f ? 1.0f / s : 0.0f, half = s > 0.0f ? 0.5f * s : INFINITY;  // a scale is at least 2^-24: finite
+        float zero_f = 8.0f;
         if (a.zero_points[j])
-            zero = s > 0.0f ? max(0, min(15, quotient(-lo, s, inv))) : 0;
+            zero_f = fminf(fmaxf(quotient(-lo[j], s, inv, half), 0.0f), 15.0f);
+        const int zero = int(zero_f);
         uint32_t codes = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float v = x[j][e] == x[j][e] ? x[j][e] : 0.0f;
-            const int q = s > 0.0f ? quotient(v, s, inv) : 0;
-            codes |= uint32_t(max(0, min(15, q + zero))) << (4 * e);
+            const float q = fminf(fmaxf(quotient(v, s, inv, half) + zero_f, 0.0f), 15.0f) + 8388608.0f;  // 2^23: the last bits are the code
+            codes |= (__float_as_uint(q) & 15u) << (4 * e);
         }
         // the block to the right shares this block's byte of zero points
         const int next = __shfl_down_sync(0xffffffffu, zero, lanes);
@@ -165,7 +173,7 @@ extern "C" int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, cons
     OVK_REQUIRE(ctx, k->heads == cache->kv_heads && v->heads == cache->kv_heads, "%s: %lld and %lld heads for a cache of %lld", op,
                 (long long)k->heads, (long long)v->heads, (long long)cache->kv_heads);
     const int64_t items = batch->tokens * cache->kv_heads * (cache->head_dim / 8);
-    OVK_REQUIRE(ctx, ceil_div64(items, 256) < (int64_t(1) << 31), "%s: %lld tokens of %lld heads are too many for one call", op,
+    OVK_REQUIRE(ctx, batch->tokens * cache->kv_heads < (int64_t(1) << 31) && ceil_div64(items, 256) < (int64_t(1) << 31), "%s: %lld tokens of %lld heads are too many for one call", op,
                 (long long)batch->tokens, (long long)cache->kv_heads);
     OVK_REQUIRE(ctx, ctx, "%s: null context", op);
     if (items == 0 || batch->batch == 0)
@@ -180,6 +188,8 @@ extern "C" int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, cons
     a.zero_points[0] = static_cast<uint8_t *>(cache->k_zero_points), a.zero_points[1] = static_cast<uint8_t *>(cache->v_zero_points);
     a.cu = batch->cu_tokens, a.lens = batch->lens, a.table = batch->block_table;
     a.items = items;
+    a.tokens = int(batch->tokens);
+    a.word_shift = cache->head_dim == 64 ? 3 : cache->head_dim == 128 ? 4 : 5;
     a.batch = int(batch->batch), a.heads = int(cache->kv_heads), a.head_dim = int(cache->head_dim), a.block_size = int(cache->block_size);
     a.page_size = int(cache->page_size), a.pages = int(cache->pages), a.max_pages = batch->max_pages;
     a.status = ctx->dev_status;

@@ -23,7 +23,8 @@ gather_block_quantized_kernel(const uint32_t *__restrict__ table, const void *__
     const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= count_words)
         return;
-    const int64_t j = i / words_per_row;
+    // (a 64-bit division costs more than the rest of the thread's work)
+    const int64_t j = count_words >> 32 ? i / words_per_row : int64_t(uint32_t(i) / uint32_t(words_per_row));
     const int word = int(i - j * words_per_row);
     int64_t row = IDX64 ? static_cast<const int64_t *>(indices)[j] : int64_t(static_cast<const int32_t *>(indices)[j]);
     if (row < 0)
