@@ -4,70 +4,100 @@
 //   x[i][j] = scale * q[i] . k[j],  out[i] = sum_j 2^(x log2 e - m) v[j] / sum_j 2^(x log2 e - m),
 //
 // one pass over the keys with the running maximum m and sum of each row.  A block
-// holds 64 query rows of one head and walks 64 keys at a time; a thread computes 8
-// (256-wide heads: 4) x 4 scores, then as many rows x head_dim / 16 columns of the
-// result.  All of it is f32 arithmetic on the CUDA cores: with Q and K transposed in
-// shared memory a step over d is three 16-byte loads for 32 multiply-adds, so the
+// holds 64 query rows of one head and walks 64 or 32 keys at a time; a thread
+// computes 8 (256-wide heads: 4) x 4 or 2 scores, then as many rows x head_dim / 16
+// columns of the result.  All of it is f32 arithmetic on the CUDA cores: a step over
+// four d is twelve 16-byte loads of shared memory for 128 multiply-adds, so the
 // adders and not shared memory bound it.
 #include "attention_prompt.cuh"
 
 namespace {
 
-constexpr int BM = 64, BN = 64, PITCH = BM + 4;
+constexpr int BM = 64;
 
-// rows of a thread: eight (128 threads) where the registers hold their results
-template <int DMAX> constexpr int rows_of() { return DMAX == 256 ? 4 : 8; }
-template <int DMAX> constexpr int threads_of() { return BM / rows_of<DMAX>() * 16; }
+// Per padded head_dim: rows of a thread (eight where the registers hold their results) and keys of a tile (so that two
+// blocks or more fit an SM).  Rows in shared memory are four floats apart beyond their length, which spreads the eight
+// rows that a quarter of a warp reads at once over all banks.
+template <int DMAX> struct Simt {
+    static constexpr int RT = DMAX == 256 ? 4 : 8, THREADS = BM / RT * 16, BN = DMAX == 64 ? 64 : 32, CT = BN / 16;
+    static constexpr int PITCH = DMAX + 4, P_PITCH = BM + 4, OC = DMAX / 64;
+    static constexpr size_t SMEM = size_t(BM * PITCH + BN * PITCH + BN * DMAX + BN * P_PITCH) * 4;
+};
 
-template <int DMAX> constexpr size_t simt_smem() { return size_t(2 * DMAX * PITCH + BN * DMAX + BN * PITCH) * 4; }
-
-// rows of a [tokens, heads, d] tensor as columns of `t`: t[d][row], zeros outside
-template <typename T, int DMAX>
-__device__ __forceinline__ void load_transposed(float *t, const T *base, int64_t stride, int rows, int d, bool vec)
+// ROWS rows of a [tokens, heads, d] tensor into shared memory as f32, zeros outside.  f32 rows on 16-byte boundaries are
+// copied asynchronously (wait_copies makes them visible to the thread that copied them).
+template <typename T, int DMAX, int ROWS, int PITCH>
+__device__ __forceinline__ void load_rows(float *dst, const T *base, int64_t stride, int rows, int d, bool vec)
 {
-    constexpr int V = 16 / sizeof(T), PARTS = threads_of<DMAX>() / BM;  // threads of a row
-    const int r = threadIdx.x / PARTS, part = threadIdx.x % PARTS;
-    const T *src = base + int64_t(r) * stride;
+    constexpr int V = 16 / sizeof(T), PER = DMAX / V;
 #pragma unroll 4
-    for (int e = part * V; e < DMAX; e += PARTS * V) {
+    for (int i = threadIdx.x; i < ROWS * PER; i += Simt<DMAX>::THREADS) {
+        const int r = i / PER, e = (i - r * PER) * V;
+        const T *src = base + int64_t(r) * stride + e;
+        float *to = dst + r * PITCH + e;
+        if constexpr (sizeof(T) == 4) {
+            if (vec && (e + V <= d || e >= d)) {
+                const int bytes = r < rows && e < d ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(to))),
+                             "l"(bytes ? static_cast<const void *>(src) : static_cast<const void *>(base)), "r"(bytes)
+                             : "memory");
+                continue;
+            }
+        }
         float v[V];
         if (r < rows && vec && e + V <= d) {
-            load_row<T, V, true>(src + e, v);
+            load_row<T, V, true>(src, v);
         } else {
 #pragma unroll
-            for (int i = 0; i < V; i++)
-                v[i] = r < rows && e + i < d ? to_f32<T>(src[e + i]) : 0.0f;
+            for (int u = 0; u < V; u++)
+                v[u] = r < rows && e + u < d ? to_f32<T>(src[u]) : 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            t[(e + i) * PITCH + r] = v[i];
+        for (int u = 0; u < V; u += 4)
+            *reinterpret_cast<float4 *>(to + u) = make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]);
     }
 }
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <typename T, int DMAX>
-__global__ void __launch_bounds__(threads_of<DMAX>()) attention_prompt_simt_kernel(const PromptArgs a)
+__global__ void __launch_bounds__(Simt<DMAX>::THREADS) attention_prompt_simt_kernel(const PromptArgs a)
 {
-    constexpr int RT = rows_of<DMAX>(), THREADS = threads_of<DMAX>();
+    using C = Simt<DMAX>;
+    constexpr int RT = C::RT, CT = C::CT, BN = C::BN, PITCH = C::PITCH, P_PITCH = C::P_PITCH, OC = C::OC, THREADS = C::THREADS;
     extern __shared__ __align__(16) float sm[];
-    float *const qt = sm, *const kt = qt + DMAX * PITCH, *const vs = kt + DMAX * PITCH, *const pt = vs + BN * DMAX;
+    float *const qs = sm, *const ks = qs + BM * PITCH, *const vs = ks + BN * PITCH, *const pt = vs + BN * DMAX;
     __shared__ PromptTile where;
     const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
     if (tid < 32)
-        find_prompt_tile<BM>(a, blockIdx.x, where);
+        find_prompt_tile<BM>(a, blockIdx.x / a.heads, where);  // the heads of a tile together, the long tiles first
     __syncthreads();
     const PromptTile w = where;
     if (w.b < 0)
         return;
-    const int head = blockIdx.y, kv_head = head / a.group, D = a.head_dim;
+    const int head = blockIdx.x % a.heads, kv_head = head / a.group, D = a.head_dim;
     const int rows = min(BM, w.n_q - w.row0);
     const int64_t first = int64_t(w.n_k) - w.n_q + w.row0;  // position of the tile's first row
     const KeyRange range = key_range(a, w, rows);
     const T *q = static_cast<const T *>(a.q) + int64_t(w.first_q + w.row0) * a.q_token + int64_t(head) * a.q_head;
     const T *k = static_cast<const T *>(a.k) + int64_t(w.first_k) * a.k_token + int64_t(kv_head) * a.k_head;
     const T *v = static_cast<const T *>(a.v) + int64_t(w.first_k) * a.v_token + int64_t(kv_head) * a.v_head;
-    load_transposed<T, DMAX>(qt, q, a.q_token, rows, D, a.vec);
+    // K and V have one buffer each: the next K comes while the weights are computed and used, the next V beside the
+    // next scores
+    auto fetch_k = [&](int64_t j0) {
+        if (j0 < range.end)
+            load_rows<T, DMAX, BN, PITCH>(ks, k + j0 * a.k_token, a.k_token, int(min(int64_t(BN), range.end - j0)), D, a.vec);
+        commit_copies();
+    };
+    auto fetch_v = [&](int64_t j0) {
+        if (j0 < range.end)
+            load_rows<T, DMAX, BN, DMAX>(vs, v + j0 * a.v_token, a.v_token, int(min(int64_t(BN), range.end - j0)), D, a.vec);
+        commit_copies();
+    };
+    load_rows<T, DMAX, BM, PITCH>(qs, q, a.q_token, rows, D, a.vec);
+    fetch_k(range.begin);
+    fetch_v(range.begin);
 
-    constexpr int OC = DMAX / 64;
     float o[RT][OC][4], m[RT], l[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) {
@@ -78,49 +108,27 @@ __global__ void __launch_bounds__(threads_of<DMAX>()) attention_prompt_simt_kern
     }
     for (int64_t j0 = range.begin; j0 < range.end; j0 += BN) {
         const int keys = int(min(int64_t(BN), range.end - j0));
+        wait_copies<1>();  // K, and the first time Q; V may still be on its way
         __syncthreads();
-        load_transposed<T, DMAX>(kt, k + j0 * a.k_token, a.k_token, keys, D, a.vec);
-        bool odd_value = false;  // an infinity or NaN among the values
-        {
-            constexpr int V = 16 / sizeof(T), PER = DMAX / V;
-            for (int i = tid; i < BN * PER; i += THREADS) {
-                const int r = i / PER, e = (i - r * PER) * V;
-                const T *src = v + (j0 + r) * a.v_token + e;
-                float x[V];
-                if (r < keys && a.vec && e + V <= D) {
-                    load_row<T, V, true>(src, x);
-                } else {
-#pragma unroll
-                    for (int u = 0; u < V; u++)
-                        x[u] = r < keys && e + u < D ? to_f32<T>(src[u]) : 0.0f;
-                }
-#pragma unroll
-                for (int u = 0; u < V; u++) {
-                    odd_value |= !(x[u] - x[u] == 0.0f);
-                    vs[r * DMAX + e + u] = x[u];
-                }
-            }
-        }
-        odd_value = __syncthreads_or(odd_value);
-        float s[RT][4];
+        float s[RT][CT];
 #pragma unroll
         for (int i = 0; i < RT; i++)
-            s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
-#pragma unroll 8
-        for (int d = 0; d < DMAX; d++) {
-            float xs[RT];
 #pragma unroll
-            for (int i = 0; i < RT; i += 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(qt + d * PITCH + ty * RT + i);
-                xs[i] = x.x, xs[i + 1] = x.y, xs[i + 2] = x.z, xs[i + 3] = x.w;
+            for (int j = 0; j < CT; j++)
+                s[i][j] = 0.0f;
+#pragma unroll 2
+        for (int d = 0; d < DMAX; d += 4) {
+            float4 y[CT];
+#pragma unroll
+            for (int j = 0; j < CT; j++)
+                y[j] = *reinterpret_cast<const float4 *>(ks + (tx + 16 * j) * PITCH + d);
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                const float4 x = *reinterpret_cast<const float4 *>(qs + (ty * RT + i) * PITCH + d);
+#pragma unroll
+                for (int j = 0; j < CT; j++)
+                    s[i][j] = fmaf(x.x, y[j].x, fmaf(x.y, y[j].y, fmaf(x.z, y[j].z, fmaf(x.w, y[j].w, s[i][j]))));
             }
-            const float4 y = *reinterpret_cast<const float4 *>(kt + d * PITCH + tx * 4);
-            const float ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    s[i][j] = fmaf(xs[i], ys[j], s[i][j]);
         }
         const bool masked = keys < BN || (a.causal && j0 + BN - 1 > first) || (a.window > 0 && j0 <= first + rows - 1 - a.window);
 #pragma unroll
@@ -128,8 +136,8 @@ __global__ void __launch_bounds__(threads_of<DMAX>()) attention_prompt_simt_kern
             const int64_t p = first + ty * RT + i;
             float most = -1e30f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int64_t key = j0 + tx * 4 + j;
+            for (int j = 0; j < CT; j++) {
+                const int64_t key = j0 + tx + 16 * j;
                 s[i][j] *= a.scale_log2e;
                 if (masked && (key >= w.n_k || (a.causal && key > p) || (a.window > 0 && key <= p - a.window)))
                     s[i][j] = -INFINITY;
@@ -147,23 +155,33 @@ __global__ void __launch_bounds__(threads_of<DMAX>()) attention_prompt_simt_kern
                 for (int e = 0; e < 4; e++)
                     o[i][c][e] *= f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < CT; j++) {
                 s[i][j] = exp2_approx(s[i][j] - to);
                 l[i] += s[i][j];
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int j = 0; j < CT; j++)
 #pragma unroll
             for (int i = 0; i < RT; i += 4)
-                *reinterpret_cast<float4 *>(pt + (tx * 4 + j) * PITCH + ty * RT + i) = make_float4(s[i][j], s[i + 1][j], s[i + 2][j], s[i + 3][j]);
+                *reinterpret_cast<float4 *>(pt + (tx + 16 * j) * P_PITCH + ty * RT + i) = make_float4(s[i][j], s[i + 1][j], s[i + 2][j], s[i + 3][j]);
+        wait_copies<0>();
+        // an infinity or NaN among values that some row must not read: 0 times it is NaN, so such rows skip it
+        bool odd_value = false;
         __syncthreads();
-        if (masked && odd_value) {
-            // 0 times an infinity is NaN: rows that do not read a key skip it
+        fetch_k(j0 + BN);
+        if (masked) {
+            for (int i = tid; i < BN * DMAX / 4; i += THREADS) {
+                const float4 x = reinterpret_cast<const float4 *>(vs)[i];
+                odd_value |= !((x.x - x.x) + (x.y - x.y) + (x.z - x.z) + (x.w - x.w) == 0.0f);
+            }
+            odd_value = __syncthreads_or(odd_value);
+        }
+        if (odd_value) {
             for (int n = 0; n < keys; n++)
 #pragma unroll
                 for (int i = 0; i < RT; i++) {
-                    const float p = pt[n * PITCH + ty * RT + i];
+                    const float p = pt[n * P_PITCH + ty * RT + i];
                     const int64_t key = j0 + n, at = first + ty * RT + i;
                     if ((a.causal && key > at) || (a.window > 0 && key <= at - a.window))
                         continue;
@@ -173,29 +191,32 @@ __global__ void __launch_bounds__(threads_of<DMAX>()) attention_prompt_simt_kern
                         for (int e = 0; e < 4; e++)
                             o[i][c][e] = fmaf(p, vs[n * DMAX + c * 64 + tx * 4 + e], o[i][c][e]);
                 }
-            continue;
-        }
+        } else {
 #pragma unroll 4
-        for (int n = 0; n < BN; n++) {
-            float xs[RT];
+            for (int n = 0; n < BN; n++) {
+                float xs[RT];
 #pragma unroll
-            for (int i = 0; i < RT; i += 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(pt + n * PITCH + ty * RT + i);
-                xs[i] = x.x, xs[i + 1] = x.y, xs[i + 2] = x.z, xs[i + 3] = x.w;
-            }
+                for (int i = 0; i < RT; i += 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(pt + n * P_PITCH + ty * RT + i);
+                    xs[i] = x.x, xs[i + 1] = x.y, xs[i + 2] = x.z, xs[i + 3] = x.w;
+                }
 #pragma unroll
-            for (int c = 0; c < OC; c++) {
-                const float4 y = *reinterpret_cast<const float4 *>(vs + n * DMAX + c * 64 + tx * 4);
+                for (int c = 0; c < OC; c++) {
+                    const float4 y = *reinterpret_cast<const float4 *>(vs + n * DMAX + c * 64 + tx * 4);
 #pragma unroll
-                for (int i = 0; i < RT; i++) {
-                    o[i][c][0] = fmaf(xs[i], y.x, o[i][c][0]);
-                    o[i][c][1] = fmaf(xs[i], y.y, o[i][c][1]);
-                    o[i][c][2] = fmaf(xs[i], y.z, o[i][c][2]);
-                    o[i][c][3] = fmaf(xs[i], y.w, o[i][c][3]);
+                    for (int i = 0; i < RT; i++) {
+                        o[i][c][0] = fmaf(xs[i], y.x, o[i][c][0]);
+                        o[i][c][1] = fmaf(xs[i], y.y, o[i][c][1]);
+                        o[i][c][2] = fmaf(xs[i], y.z, o[i][c][2]);
+                        o[i][c][3] = fmaf(xs[i], y.w, o[i][c][3]);
+                    }
                 }
             }
         }
+        __syncthreads();
+        fetch_v(j0 + BN);
     }
+    wait_copies<0>();
 #pragma unroll
     for (int i = 0; i < RT; i++) {
         const int r = ty * RT + i;
@@ -218,11 +239,11 @@ __global__ void __launch_bounds__(threads_of<DMAX>()) attention_prompt_simt_kern
     }
 }
 
-template <typename T, int DMAX> int32_t launch_simt(ovk_ctx *ctx, const PromptArgs &a, unsigned tiles)
+template <typename T, int DMAX> int32_t launch_simt(ovk_ctx *ctx, const PromptArgs &a, unsigned blocks)
 {
-    constexpr size_t smem = simt_smem<DMAX>();
-    OVK_CUDA(ctx, ovk_allow_smem(attention_prompt_simt_kernel<T, DMAX>, smem, ctx->device));
-    attention_prompt_simt_kernel<T, DMAX><<<dim3(tiles, unsigned(a.heads)), threads_of<DMAX>(), smem, ctx->stream>>>(a);
+    using C = Simt<DMAX>;
+    OVK_CUDA(ctx, ovk_allow_smem(attention_prompt_simt_kernel<T, DMAX>, C::SMEM, ctx->device));
+    attention_prompt_simt_kernel<T, DMAX><<<blocks, C::THREADS, C::SMEM, ctx->stream>>>(a);
     OVK_LAUNCHED(ctx, sizeof(T) == 4 ? "attention_prompt_f32" : "attention_prompt_simt");
     return OVK_OK;
 }
@@ -260,7 +281,6 @@ extern "C" int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p
     OVK_REQUIRE(ctx, ctx, "%s: null context", op);
     if (p->q_tokens == 0 || p->batch == 0)
         return OVK_OK;
-    OVK_REQUIRE(ctx, q->heads <= 65535, "%s: %lld query heads", op, (long long)q->heads);
     DeviceGuard guard(ctx->device);
     PromptArgs a = {};
     a.q = q->data, a.k = k->data, a.v = v->data, a.out = out->data;
@@ -273,16 +293,18 @@ extern "C" int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p
     a.max_q = p->max_q;
     a.vec = ovk_rows_aligned(q, elem) && ovk_rows_aligned(k, elem) && ovk_rows_aligned(v, elem);
     a.status = ctx->dev_status;
-    const unsigned tiles = unsigned(prompt_tiles(a, BM));
+    const int64_t tiles = prompt_tiles(a, BM) * a.heads;
+    OVK_REQUIRE(ctx, tiles < (int64_t(1) << 31), "%s: %lld query rows of %d heads are too many for one call", op, (long long)p->q_tokens, a.heads);
+    const unsigned blocks = unsigned(tiles);
     if (p->dtype == OVK_FLOAT)
-        return p->head_dim <= 64    ? launch_simt<float, 64>(ctx, a, tiles)
-               : p->head_dim <= 128 ? launch_simt<float, 128>(ctx, a, tiles)
-                                    : launch_simt<float, 256>(ctx, a, tiles);
+        return p->head_dim <= 64    ? launch_simt<float, 64>(ctx, a, blocks)
+               : p->head_dim <= 128 ? launch_simt<float, 128>(ctx, a, blocks)
+                                    : launch_simt<float, 256>(ctx, a, blocks);
     bool taken = false;
     rc = ovk_prompt_tc(ctx, a, &taken);
     if (taken || rc != OVK_OK)
         return rc;
-    return p->head_dim <= 64    ? launch_simt<__half, 64>(ctx, a, tiles)
-           : p->head_dim <= 128 ? launch_simt<__half, 128>(ctx, a, tiles)
-                                : launch_simt<__half, 256>(ctx, a, tiles);
+    return p->head_dim <= 64    ? launch_simt<__half, 64>(ctx, a, blocks)
+           : p->head_dim <= 128 ? launch_simt<__half, 128>(ctx, a, blocks)
+                                : launch_simt<__half, 256>(ctx, a, blocks);
 }
