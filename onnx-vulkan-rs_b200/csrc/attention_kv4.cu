@@ -95,9 +95,11 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
     DeviceGuard guard(ctx->device);
 
     Kv4Args a = {};
-    a.codes[0] = static_cast<const uint8_t *>(cache->k), a.codes[1] = static_cast<const uint8_t *>(cache->v);
-    a.scales[0] = static_cast<const uint8_t *>(cache->k_scales), a.scales[1] = static_cast<const uint8_t *>(cache->v_scales);
-    a.zero_points[0] = static_cast<const uint8_t *>(cache->k_zero_points), a.zero_points[1] = static_cast<const uint8_t *>(cache->v_zero_points);
+    // a cache without pages may come without data: copies of no bytes still name an address
+    auto data = [&](const void *p) { return static_cast<const uint8_t *>(cache->pages ? p : ctx->dev_status); };
+    a.codes[0] = data(cache->k), a.codes[1] = data(cache->v), a.scales[0] = data(cache->k_scales), a.scales[1] = data(cache->v_scales);
+    if (cache->k_zero_points)
+        a.zero_points[0] = data(cache->k_zero_points), a.zero_points[1] = data(cache->v_zero_points);
     a.cu = batch->cu_tokens, a.lens = batch->lens, a.table = batch->block_table;
     a.q = q->data, a.out = out->data;
     a.q_token = q->token_stride, a.q_head = q->head_stride, a.o_token = out->token_stride, a.o_head = out->head_stride;

@@ -230,10 +230,15 @@ def _ptr(t):
     return t.data_ptr()
 
 
-def _dtype_code(t) -> int:
+@functools.cache
+def _dtype_codes() -> dict:
     import torch
     return {torch.float32: FLOAT, torch.float16: FLOAT16, torch.uint8: UINT8, torch.int8: INT8,
-            torch.int32: INT32, torch.int64: INT64}[t.dtype]
+            torch.int32: INT32, torch.int64: INT64}
+
+
+def _dtype_code(t) -> int:
+    return _dtype_codes()[t.dtype]
 
 
 class Context:
@@ -590,21 +595,22 @@ class Context:
     def gather_block_quantized(self, table, indices, scales, zero_points, block_size, out_dtype=None, out=None):
         """interp::gather_block_quantized (interp.rs:2874).  `indices`: a torch CUDA tensor (read on the
         device), or a CPU tensor / numpy array / list (checked on the host first, as the reference does)."""
-        import numpy as np
         import torch
-        rows, cols = int(table.shape[0]), int(table.shape[1]) * 2
+        rows, half = table.shape
+        cols = half * 2
         on_host = not (isinstance(indices, torch.Tensor) and indices.is_cuda)
         if on_host:
+            import numpy as np
             idx = np.ascontiguousarray(np.asarray(indices, dtype=np.int64))
             shape, count, ptr, code = idx.shape, idx.size, idx.ctypes.data, INT64
         else:
-            idx = indices.contiguous()
-            shape, count, ptr, code = tuple(idx.shape), idx.numel(), _ptr(idx), _dtype_code(idx)
+            idx = indices if indices.is_contiguous() else indices.contiguous()
+            shape, count, ptr, code = idx.shape, idx.numel(), idx.data_ptr(), _dtype_code(idx)
         if out is None:
-            out = torch.empty(tuple(shape) + (cols,), dtype=out_dtype or torch.float32, device=table.device)
+            out = torch.empty((*shape, cols), dtype=out_dtype or torch.float32, device=table.device)
         self.check(lib().ovk_gather_block_quantized(self.h, _ptr(table), _ptr(scales), _dtype_code(scales),
                                                     _ptr(zero_points), rows, cols, 4, int(block_size), ptr, code,
-                                                    int(on_host), count, _ptr(out), _dtype_code(out)))
+                                                    1 if on_host else 0, count, _ptr(out), _dtype_code(out)))
         return out
 
     def argmax(self, x, axis=-1, out=None):
@@ -692,10 +698,14 @@ class Context:
             x += self._activation("Rotary: k", k, n, None, d, kind)
             if k_out is None:
                 k_out = self._new(k, stream)
-            y_k = self._activation("Rotary: k_out", k_out, n, x[5], d, kind)
+                y_k = (k_out.data_ptr(), x[5], x[5] * d, d)
+            else:
+                y_k = self._activation("Rotary: k_out", k_out, n, x[5], d, kind)
         if out is None:
             out = self._new(q, stream)
-        y = self._activation("Rotary: out", out, n, h, d, kind)
+            y = (out.data_ptr(), h, h * d, d)
+        else:
+            y = self._activation("Rotary: out", out, n, h, d, kind)
         self._keep(stream, q, k, cos, sin, positions, out, k_out)
         p = _PACK_ROTARY(n, d, 2 * pairs, rows, codes[kind], codes[cos.dtype], _index_codes()[positions.dtype], 1 if interleaved else 0, axes,
                          *sections, *(0,) * (4 - axes))
@@ -755,7 +765,9 @@ class Context:
         stream = self._foreign_stream()
         if out is None:
             out = self._new(q, stream)
-        ho = self._activation("AttentionKV4: out", out, n, h, d, q.dtype)
+            ho = (out.data_ptr(), h, h * d, d)
+        else:
+            ho = self._activation("AttentionKV4: out", out, n, h, d, q.dtype)
         space, need = None, 0
         if stream is not None:
             self._keep(stream, q, block_table, cu_tokens, lens, out, *cache.tensors)
@@ -788,7 +800,9 @@ class Context:
         stream = self._foreign_stream()
         if out is None:
             out = self._new(q, stream)
-        ho = self._activation("AttentionPrompt: out", out, n, h, d, kind)
+            ho = (out.data_ptr(), h, h * d, d)
+        else:
+            ho = self._activation("AttentionPrompt: out", out, n, h, d, kind)
         self._keep(stream, q, k, v, cu_q, cu_k, out)
         p = _PACK_PROMPT(n, k.shape[0], batch, d, _activation_codes()[kind], 1 if causal else 0, window, d ** -0.5 if scale is None else scale,
                          int(max_q or 0))

@@ -290,6 +290,65 @@ def test_attention_kv4_many_sequences():
     check_kv4(cache, table, q, new, lens, 64 ** -0.5, 0, got.cpu())
 
 
+def test_attention_kv4_far_more_sequences_than_threads():
+    """The shares of the work are found by a scan over the batch that takes several passes."""
+    rng = np.random.default_rng(4)
+    lens = [int(v) for v in rng.integers(0, 9, 1100)]
+    lens[700], new = 3000, [int(v) for v in rng.integers(0, 2, 1100)]
+    new[700] = 1
+    cache, table = filled_cache(lens, 1, 64, 64, 8, True, 7)
+    q = randn((sum(new), 2, 64), 9, F16, 1.5)
+    got = ctx().attention_kv4(cache, q.cuda(), dev(table), starts(new), i32(lens))
+    ctx().flush()
+    check_kv4(cache, table, q, new, lens, 64 ** -0.5, 0, got.cpu())
+
+
+def test_cache_offsets_beyond_32_bits():
+    """Pages at the end of a cache whose codes, and scales, lie more than 2^32 bytes from their tensors' starts."""
+    page, d, pages = 64, 128, 8_600_000 // 8 + 10  # 68.8 million rows: codes of 4.4 GB each
+    make = lambda last, dtype: torch.empty((pages, 1, page, last), dtype=dtype, device="cuda")  # noqa: E731
+    cache = ovk_b200.KV4Cache(make(64, torch.uint8), make(64, torch.uint8), make(4, F16), make(4, F16), make(2, torch.uint8), make(2, torch.uint8))
+    assert cache.k.numel() > 2 ** 32
+    lens, table = [150], np.array([[pages - 1, 3, pages - 2]], dtype=np.int32)
+    k, v, q = randn((150, 1, d), 1, F16), randn((150, 1, d), 2, F16), randn((1, 8, d), 3, F16)
+    ctx().kv4_append(cache, k.cuda(), v.cuda(), dev(table), starts(lens), i32(lens))
+    got = ctx().attention_kv4(cache, q.cuda(), dev(table), starts([1]), i32(lens))
+    ctx().flush()
+    rows = {w: ref.dequantize(*ref.quantize(x, 32, True))[:, 0] for w, x in (("k", k), ("v", v))}
+    sizes = ref.row_sizes(*ref.quantize(k, 32, True))[:, 0]
+    for h in range(8):
+        want, bound = ref.attend(q[:, h].double(), rows["k"], rows["v"], d ** -0.5, True, 0, 2.0 ** -11, 0.0, sizes)
+        ref.check(got[:, h], want, bound, f"head {h}")
+
+
+def test_attention_kv4_without_pages_or_sequences():
+    q = randn((2, 4, 128), 1, F16).cuda()
+    cache = ctx().kv4_cache(0, 2, 16, 128)
+    none = torch.zeros((2, 0), dtype=torch.int32, device="cuda")
+    got = ctx().attention_kv4(cache, q, none, i32([0, 1, 2]), i32([0, 0]), out=torch.full_like(q, 3.0))
+    ctx().flush()
+    assert bool((got == 0).all())
+    got = ctx().attention_kv4(cache, q, torch.zeros((0, 4), dtype=torch.int32, device="cuda"), i32([0]), i32([]), out=torch.full_like(q, 3.0))
+    ctx().flush()
+    assert bool((got == 3).all())
+    assert ctx().attention_kv4(cache, q[:0], none, i32([0, 0, 0]), i32([0, 0])).shape == (0, 4, 128)
+    ctx().kv4_append(cache, q[:0, :2], q[:0, :2], none, i32([0, 0, 0]), i32([0, 0]))
+    ctx().flush()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.11, 3.0])
+def test_scales_of_any_sign(scale):
+    cache, table = filled_cache([70], 1, 128, 32, 16, True, 3)
+    q = randn((1, 4, 128), 1, F16)
+    got = ctx().attention_kv4(cache, q.cuda(), dev(table), starts([1]), i32([70]), scale=scale)
+    ctx().flush()
+    check_kv4(cache, table, q, [1], [70], scale, 0, got.cpu())
+    q, k, v = (randn((140, 2, 128), s, F16) for s in (1, 2, 3))
+    got = ctx().attention_prompt(q.cuda(), k.cuda(), v.cuda(), starts([140]), scale=scale)
+    ctx().flush()
+    check_prompt(q, k, v, [0, 140], [0, 140], scale, True, 0, got.cpu(), False)
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_attention_kv4_extreme_queries_and_scales(dtype):
     lens = [90]
@@ -461,6 +520,29 @@ def test_attention_prompt_large_scores_and_lowest_values():
     got = ctx().attention_prompt(lowest.cuda(), lowest.cuda(), randn((130, 1, 64), 3, F16).cuda(), starts([130]), 130)
     ctx().flush()
     assert bool(torch.isfinite(got).all())
+
+
+def test_attention_prompt_longer_than_promised_is_left_out_and_reported():
+    q, k = randn((300, 2, 64), 1, F16).cuda(), randn((300, 1, 64), 2, F16).cuda()
+    out = ctx().attention_prompt(q, k, k, i32([0, 100, 300]), 150, out=torch.full_like(q, 3.0))
+    with pytest.raises(ovk_b200.OvkError) as e:
+        ctx().flush()
+    assert "bounds" in e.value.message and bool((out[100:] == 3).all()) and bool((out[:100] != 3).all())
+    want = ctx().attention_prompt(q, k, k, i32([0, 100, 300]))
+    assert torch.equal(ctx().attention_prompt(q, k, k, i32([0, 100, 300]), 200), want)
+    ctx().flush()
+
+
+def test_attention_prompt_broadcast_keys_and_no_keys():
+    q, k = randn((90, 4, 128), 1, F16).cuda(), randn((90, 1, 128), 2, F16).cuda()
+    wide = k.expand(90, 2, 128)  # one head's rows under two names
+    got = ctx().attention_prompt(q, wide, wide, starts([90]))
+    want = ctx().attention_prompt(q, wide.contiguous(), wide.contiguous(), starts([90]))
+    none = ctx().attention_prompt(q, k[:0], k[:0], starts([90]), cu_k=i32([0, 0]), out=torch.full_like(q, 3.0))
+    ctx().flush()
+    assert bool((none == 0).all())
+    # the two calls take different kernels: both are within half a step and the weights' rounding of the exact result
+    assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -10 * float(k.float().abs().max())
 
 
 def test_attention_prompt_bad_bounds_are_left_out_and_reported():
