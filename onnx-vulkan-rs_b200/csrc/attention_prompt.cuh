@@ -35,10 +35,11 @@ template <int BM> __device__ __forceinline__ void find_prompt_tile(const PromptA
     PromptTile w = {-1, 0, 0, 0, 0, 0};
     for (int base = a.batch - 1; base >= 0; base -= 32) {
         const int b = base - lane;
-        int first = 0, n = 0;
+        int first = 0, n = 0, first_k = 0, end_k = 0;
         if (b >= 0) {
             first = a.cu_q[b];
             const int end = a.cu_q[b + 1];
+            first_k = a.cu_k[b], end_k = a.cu_k[b + 1];  // fetched with the others: one way to memory, not two
             n = end - first;
             if (first < 0 || end < first || end > a.q_tokens || (a.max_q > 0 && n > a.max_q)) {
                 n = 0;
@@ -58,10 +59,9 @@ template <int BM> __device__ __forceinline__ void find_prompt_tile(const PromptA
         if (mine) {
             w.b = b, w.first_q = first, w.n_q = n;
             w.row0 = (before + sum - 1 - index) * BM;
-            w.first_k = a.cu_k[b];
-            const int end = a.cu_k[b + 1];
-            w.n_k = end - w.first_k;
-            if (w.first_k < 0 || end < w.first_k || end > a.k_tokens) {
+            w.first_k = first_k;
+            w.n_k = end_k - first_k;
+            if (first_k < 0 || end_k < first_k || end_k > a.k_tokens) {
                 w.n_k = w.first_k = 0;
                 atomicExch(a.status, OVK_DEV_BAD_SEQUENCE);
             }

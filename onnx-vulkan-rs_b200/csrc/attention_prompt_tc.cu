@@ -120,6 +120,13 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
 
     const int index = blockIdx.x / p.pairs, pair = blockIdx.x - index * p.pairs;
     const bool rows_split = NS == 2 && !p.by_heads;
+    OVK_PDL_LAUNCH_DEPENDENTS();
+    if (tid == 32) {
+        umma::prefetch_tmap(&tm_q);
+        umma::prefetch_tmap(&tm_k);
+        umma::prefetch_tmap(&tm_v);
+    }
+    OVK_PDL_WAIT();
     if (warp == 0) {
         if (rows_split)
             find_prompt_tile<2 * BM>(a, index, sh.tile);
@@ -617,7 +624,7 @@ template <int DP> int32_t launch(ovk_ctx *ctx, const PromptArgs &a, bool *taken)
     if (grid >= (int64_t(1) << 31))
         return OVK_OK;
     OVK_CUDA(ctx, ovk_allow_smem(attention_prompt_tc_kernel<DP>, C::SMEM, ctx->device));
-    attention_prompt_tc_kernel<DP><<<unsigned(grid), C::THREADS, C::SMEM, ctx->stream>>>(q, k, v, p);
+    OVK_CUDA(ctx, ovk_launch_pdl(attention_prompt_tc_kernel<DP>, dim3(unsigned(grid)), dim3(C::THREADS), C::SMEM, ctx->stream, q, k, v, p));
     *taken = true;
     OVK_LAUNCHED(ctx, "attention_prompt_tc");
     return OVK_OK;

@@ -82,6 +82,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
     const uint32_t at = uint32_t(item >> a.word_shift);
     const int word = int(item & (words - 1));
     const int token = int(at / uint32_t(a.heads)), head = int(at - uint32_t(token) * a.heads);
+    OVK_PDL_LAUNCH_DEPENDENTS();
+    OVK_PDL_WAIT();
     int64_t row = -1;
     if (item < a.items) {
         const int b = sequence_of(a.cu, a.batch, token, a.tokens);
@@ -195,13 +197,9 @@ extern "C" int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, cons
     a.status = ctx->dev_status;
     const unsigned grid = unsigned(ceil_div64(items, 256));
     const bool vec = ovk_rows_aligned(k, elem) && ovk_rows_aligned(v, elem);
-    if (dtype == OVK_FLOAT) {
-        if (vec) kv4_append_kernel<float, true><<<grid, 256, 0, ctx->stream>>>(a);
-        else kv4_append_kernel<float, false><<<grid, 256, 0, ctx->stream>>>(a);
-    } else {
-        if (vec) kv4_append_kernel<__half, true><<<grid, 256, 0, ctx->stream>>>(a);
-        else kv4_append_kernel<__half, false><<<grid, 256, 0, ctx->stream>>>(a);
-    }
+    void (*kernel)(AppendArgs) = dtype == OVK_FLOAT ? (vec ? kv4_append_kernel<float, true> : kv4_append_kernel<float, false>)
+                                                    : (vec ? kv4_append_kernel<__half, true> : kv4_append_kernel<__half, false>);
+    OVK_CUDA(ctx, ovk_launch_pdl(kernel, dim3(grid), dim3(256), 0, ctx->stream, a));
     OVK_LAUNCHED(ctx, vec ? "kv4_append" : "kv4_append_scalar");
     return OVK_OK;
 }

@@ -46,6 +46,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a)
     const int vec = int(item - row * a.items_per_row);
     const int64_t token = row / a.slots;
     const int slot = int(row - token * a.slots);
+    OVK_PDL_LAUNCH_DEPENDENTS();
+    OVK_PDL_WAIT();
     if (token >= a.tokens)
         return;
     // a position outside the tables: the token's rows are zeros and the next flush reports it
@@ -149,8 +151,7 @@ template <typename T> cudaError_t launch(const RotaryArgs &a, bool il, bool vec,
 {
     void (*kernel)(RotaryArgs) = il ? (vec ? rotary_kernel<T, true, true> : rotary_kernel<T, true, false>)
                                     : (vec ? rotary_kernel<T, false, true> : rotary_kernel<T, false, false>);
-    kernel<<<grid, 256, 0, stream>>>(a);
-    return cudaSuccess;
+    return ovk_launch_pdl(kernel, dim3(grid), dim3(256), 0, stream, a);
 }
 
 }  // namespace
@@ -236,10 +237,7 @@ extern "C" int32_t ovk_rotary(ovk_ctx *ctx, const ovk_rotary_params *p, int32_t 
     OVK_REQUIRE(ctx, ceil_div64(items, 256) < (int64_t(1) << 31), "Rotary: %lld tokens of %d heads are too many for one call",
                 (long long)p->tokens, a.heads_total);
     const unsigned grid = unsigned(ceil_div64(items, 256));
-    if (p->dtype == OVK_FLOAT)
-        launch<float>(a, il, vec, grid, ctx->stream);
-    else
-        launch<__half>(a, il, vec, grid, ctx->stream);
+    OVK_CUDA(ctx, p->dtype == OVK_FLOAT ? launch<float>(a, il, vec, grid, ctx->stream) : launch<__half>(a, il, vec, grid, ctx->stream));
     OVK_LAUNCHED(ctx, vec ? "rotary" : "rotary_scalar");
     return OVK_OK;
 }
