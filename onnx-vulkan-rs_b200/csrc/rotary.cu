@@ -201,7 +201,6 @@ extern "C" int32_t ovk_rotary(ovk_ctx *ctx, const ovk_rotary_params *p, int32_t 
     const bool il = p->interleaved != 0;
     const int v16 = int(16 / elem);
     bool vec = (il ? p->rotary_dim : pairs) % v16 == 0 && (p->head_dim - p->rotary_dim) % v16 == 0;
-    bool in_place = true;
     for (int j = 0; j < count; j++) {
         a.t.x[j] = x[j].data, a.t.out[j] = out[j].data;
         a.t.x_token[j] = x[j].token_stride, a.t.x_head[j] = x[j].head_stride;
@@ -209,7 +208,6 @@ extern "C" int32_t ovk_rotary(ovk_ctx *ctx, const ovk_rotary_params *p, int32_t 
         a.t.heads[j] = int(x[j].heads);
         a.heads_total += a.t.heads[j];
         vec = vec && ovk_rows_aligned(&x[j], elem) && ovk_rows_aligned(&out[j], elem);
-        in_place = in_place && x[j].data == out[j].data;
     }
     const int v = vec ? v16 : (il ? 2 : 1), np = il ? v / 2 : v;
     // an element outside every pair; odd counts need single elements, which the vector of two does not give
@@ -220,7 +218,6 @@ extern "C" int32_t ovk_rotary(ovk_ctx *ctx, const ovk_rotary_params *p, int32_t 
     a.turned = int(pairs / np);
     // a bad token's copied elements become zeros, so they are visited in place too
     a.items_per_row = a.turned + int(rest / v);
-    (void)in_place;
     a.pairs = int(pairs), a.rotary_dim = int(p->rotary_dim);
     a.axes = p->axes;
     for (int k = 0, end = 0; k < p->axes; k++)
