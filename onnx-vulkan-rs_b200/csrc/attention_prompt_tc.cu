@@ -183,19 +183,23 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
             umma::tmem_alloc(&sh.tmem, 512);
             umma::tmem_relinquish();
         }
-        umma::tc_fence_before();
-        asm volatile("bar.sync 1, %0;" ::"n"(C::THREADS) : "memory");
-        umma::tc_fence_after();
-        const uint32_t tmem = sh.tmem;
+        uint32_t tmem = 0;
+        if (role != 0) {  // the loads need no tensor memory
+            umma::tc_fence_before();
+            asm volatile("bar.sync 1, %0;" ::"n"(C::THREADS - 32) : "memory");
+            umma::tc_fence_after();
+            tmem = sh.tmem;
+        }
         if (role == 0) {
             // ------------------------------------------------------------ loads
             if (lane == 0 && tiles > 0) {
-                for (int s = 0; s < streams; s++) {
+                auto load_q = [&](int s) {
                     umma::mbar_expect_tx(&sh.q_full[s], C::Q_BYTES);
                     for (int x = 0; x < C::ATOMS; x++)
                         umma::tma_load_3d(smem + s * C::Q_BYTES + x * BM * 128, &tm_q, &sh.q_full[s], 64 * x,
                                           rows_split ? head0 : head0 + s, w.first_q + w.row0 + (rows_split ? s * BM : 0));
-                }
+                };
+                load_q(0);
                 int stage = 0, issued = 0;
                 uint32_t phase = 0;
                 uint32_t in_raw = 0, raw_phase = 0;  // a bit per stage: its last copy is counted at `raw`; uses of `raw` so far
@@ -225,8 +229,11 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                             stage = 0, phase ^= 1;
                     }
                 };
-                for (int j = 0; j < SB && j < tiles; j++)
-                    load(false, j);
+                load(false, 0);
+                if (streams == 2)
+                    load_q(1);
+                if (tiles > 1)
+                    load(false, 1);
                 for (int i = 0; i < tiles && ok; i++) {
                     load(true, i);
                     if (i + SB < tiles)
@@ -378,37 +385,40 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                     ok = wait_warp(&sh.raw[stage], (raw_phase >> stage) & 1, dead, status, OVK_DEV_TIMEOUT_TMA);
                     raw_phase ^= 1u << stage;
                     // in each 128-byte column the chunk's rows lie one after the other, eight 16-byte words a row
-                    constexpr int KEYS = BN / CH;
+                    constexpr int KEYS = BN / CH, STEP = 32 * C::GUARDS, WORDS = C::STAGE / 16 / STEP;
                     const int left = min(KEYS, max(0, key_end - (key_begin + i * BN + c * KEYS)));  // rows before the end
                     const int self = guard * 32 + lane;
-                    for (int x = 0; x < C::ATOMS && ok; x++) {
-                        uint4 *const words = reinterpret_cast<uint4 *>(ring + stage * C::STAGE) + x * KEYS * 8;
+                    if (ok) {
+                        uint4 *const words = reinterpret_cast<uint4 *>(ring + stage * C::STAGE) + self;
+                        bool wrote = false;
+                        if (left < KEYS)
+                            for (int k = 0; k < WORDS; k++)
+                                if ((((self + STEP * k) >> 3) & (KEYS - 1)) >= left)
+                                    words[STEP * k] = make_uint4(0, 0, 0, 0), wrote = true;
                         uint32_t bad = 0;
-#pragma unroll
-                        for (int k = 0; k < KEYS * 8 / (32 * C::GUARDS); k++) {
-                            const int at = self + 32 * C::GUARDS * k;
-                            if (at < left * 8) {
-                                const uint4 v = words[at];  // a carry into the sign bit marks an exponent of ones
-                                bad |= ((v.x & 0x7c007c00u) + 0x04000400u) | ((v.y & 0x7c007c00u) + 0x04000400u) |
-                                       ((v.z & 0x7c007c00u) + 0x04000400u) | ((v.w & 0x7c007c00u) + 0x04000400u);
-                            } else {
-                                words[at] = make_uint4(0, 0, 0, 0);
+#pragma unroll 8
+                        for (int k = 0; k < WORDS; k++) {
+                            const uint4 v = words[STEP * k];  // a carry into the sign bit marks an exponent of ones
+                            bad |= ((v.x & 0x7c007c00u) + 0x04000400u) | ((v.y & 0x7c007c00u) + 0x04000400u) |
+                                   ((v.z & 0x7c007c00u) + 0x04000400u) | ((v.w & 0x7c007c00u) + 0x04000400u);
+                        }
+                        if (bad & 0x80008000u) {
+                            wrote = true;
+#pragma unroll 1
+                            for (int k = 0; k < WORDS; k++) {
+                                const int at = self + STEP * k;
+                                const int col = at / (KEYS * 8) * 64 + (((at & 7) ^ ((at >> 3) & 7)) << 3);  // of the word's first element
+                                __half *const z = reinterpret_cast<__half *>(&words[STEP * k]);
+                                for (int e = 0; e < 8; e++)
+                                    if ((__half_as_ushort(z[e]) & 0x7c00u) == 0x7c00u) {
+                                        z[e] = __ushort_as_half(0);
+                                        atomicOr(&sh.odd[(col + e) >> 5], 1u << ((col + e) & 31));
+                                    }
                             }
                         }
-                        if (!(bad & 0x80008000u))
-                            continue;
-                        for (int at = self; at < left * 8; at += 32 * C::GUARDS) {
-                            const int col = x * 64 + (((at & 7) ^ ((at >> 3) & 7)) << 3);  // of the word's first element
-                            uint32_t z[4] = {words[at].x, words[at].y, words[at].z, words[at].w};
-                            for (int e = 0; e < 8; e++)
-                                if ((z[e >> 1] >> (16 * (e & 1)) & 0x7c00u) == 0x7c00u) {
-                                    z[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-                                    atomicOr(&sh.odd[(col + e) >> 5], 1u << ((col + e) & 31));
-                                }
-                            words[at] = make_uint4(z[0], z[1], z[2], z[3]);
-                        }
+                        if (wrote)
+                            umma::fence_proxy_async();
                     }
-                    umma::fence_proxy_async();
                     // all of them, also after a wait that gave up: then all leave
                     uint32_t all;
                     asm volatile(
@@ -430,7 +440,7 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
         // ---------------------------------------------------------------- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
         umma::tc_fence_before();
-        asm volatile("bar.sync 1, %0;" ::"n"(C::THREADS) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(C::THREADS - 32) : "memory");
         umma::tc_fence_after();
         const uint32_t tmem = sh.tmem;
         const int s = group;
@@ -454,16 +464,24 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                 for (int c = 0; c < BN / 32; c++)
                     umma::tmem_ld_32x32(t_s + 32 * c, x[c]);
                 umma::tmem_ld_wait();
-                if (partial(i, first, first + rows - 1)) {
-                    const int j0 = key_begin + i * BN;
+                const int j0 = key_begin + i * BN;
+                if (j0 + BN > w.n_k || (a.causal && j0 + BN - 1 > first)) {
                     const int hi = (a.causal ? min(pos, w.n_k - 1) : w.n_k - 1) - j0;
-                    const int lo = p.window > 0 ? pos - p.window + 1 - j0 : 0;
 #pragma unroll
                     for (int c = 0; c < BN / 32; c++)
 #pragma unroll
                         for (int e = 0; e < 32; e++)
-                            if (32 * c + e > hi || 32 * c + e < lo)
+                            if (32 * c + e > hi)
                                 x[c][e] = 0xff800000u;  // -infinity
+                }
+                if (p.window > 0 && j0 <= first + rows - 1 - p.window) {
+                    const int lo = pos - p.window + 1 - j0;
+#pragma unroll
+                    for (int c = 0; c < BN / 32; c++)
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (32 * c + e < lo)
+                                x[c][e] = 0xff800000u;
                 }
                 float most[4];
 #pragma unroll
@@ -522,61 +540,77 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                 umma::tc_fence_after();
             }
             if (ok) {
+                // By way of the queries' place in shared memory, which no product reads any more: a warp lays its 32 rows
+                // there, 16-byte words exchanged by row so that neither side meets in a bank, and stores them row by row.
+                // (Straight from registers a store touched 32 lines: 6300 cycles a tile of 256-wide rows, now XXXX.)
                 const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-                __half *const out = static_cast<__half *>(a.out) +
-                                    int64_t(w.first_q + w.row0 + (rows_split ? s * BM : 0) + r) * a.o_token +
-                                    int64_t(rows_split ? head0 : head0 + s) * a.o_head;
+                uint8_t *const stage = smem + s * C::Q_BYTES;
                 bool any_odd = false;
                 for (int i = 0; i < DP / 32; i++)
                     any_odd |= sh.odd[i] != 0;
 #pragma unroll
-                for (int c = 0; c < DP / 32; c++) {
-                    uint32_t o[32];
+                for (int c = 0; c < DP / 64; c++) {
+                    uint32_t o[2][32];
                     if (tiles > 0) {
-                        umma::tmem_ld_32x32(t_o + 32 * c, o);
+                        umma::tmem_ld_32x32(t_o + 64 * c, o[0]);
+                        umma::tmem_ld_32x32(t_o + 64 * c + 32, o[1]);
                         umma::tmem_ld_wait();
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            o[e] = 0;
+                        for (int e = 0; e < 64; e++)
+                            o[e >> 5][e & 31] = 0;
                     }
-                    if (r >= rows || 32 * c >= a.head_dim)
-                        continue;
-                    if (any_odd && sh.odd[c]) {
+                    if (any_odd && (sh.odd[2 * c] | sh.odd[2 * c + 1])) {
                         // elements that the guards took out, of the keys that this row reads
                         for (int i = 0; i < tiles; i++) {
-                            if (!partial(i, pos0, pos_last))
+                            if (r >= rows || !partial(i, pos0, pos_last))
                                 continue;
                             const int j0 = key_begin + i * BN;
                             const int from = p.window > 0 ? max(j0, pos - p.window + 1) : j0;
                             const int to = min(j0 + BN, a.causal ? min(w.n_k, pos + 1) : w.n_k);
                             for (int j = from; j < to; j++) {
                                 const __half *v = static_cast<const __half *>(a.v) + int64_t(w.first_k + j) * a.v_token +
-                                                  int64_t(kv_head) * a.v_head + 32 * c;
+                                                  int64_t(kv_head) * a.v_head + 64 * c;
 #pragma unroll
-                                for (int e = 0; e < 32; e++)
-                                    if ((sh.odd[c] >> e) & 1) {
+                                for (int e = 0; e < 64; e++)
+                                    if ((sh.odd[2 * c + (e >> 5)] >> (e & 31)) & 1) {
                                         const float x = __half2float(v[e]);
                                         if (!(x - x == 0.0f))
-                                            o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                                            o[e >> 5][e & 31] = __float_as_uint(__uint_as_float(o[e >> 5][e & 31]) + x);
                                     }
                             }
                         }
                     }
-                    if (p.vec_out && 32 * c + 32 <= a.head_dim) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint32_t h[4];
+                    for (int e = 0; e < 8; e++) {
+                        uint32_t h[4];
 #pragma unroll
-                            for (int u = 0; u < 4; u++)
-                                h[u] = pack_halves(__uint_as_float(o[e + 2 * u]) * inverse, __uint_as_float(o[e + 2 * u + 1]) * inverse);
-                            *reinterpret_cast<uint4 *>(out + 32 * c + e) = make_uint4(h[0], h[1], h[2], h[3]);
-                        }
-                    } else {
+                        for (int u = 0; u < 4; u++)
+                            h[u] = pack_halves(__uint_as_float(o[e >> 2][8 * (e & 3) + 2 * u]) * inverse,
+                                               __uint_as_float(o[e >> 2][8 * (e & 3) + 2 * u + 1]) * inverse);
+                        *reinterpret_cast<uint4 *>(stage + r * (DP * 2) + c * 128 + ((e ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    }
+                }
+                __syncwarp();
+                constexpr int WORDS = DP / 8;  // of a row
+                const int word = lane % WORDS, r0 = (warp & 3) * 32;
+                __half *const out = static_cast<__half *>(a.out) +
+                                    int64_t(w.first_q + w.row0 + (rows_split ? s * BM : 0)) * a.o_token +
+                                    int64_t(rows_split ? head0 : head0 + s) * a.o_head + 8 * word;
+                if (8 * word < a.head_dim) {
+#pragma unroll 8
+                    for (int k = 0; k < WORDS; k++) {
+                        const int row = r0 + k * (32 / WORDS) + lane / WORDS;
+                        if (row >= rows)
+                            break;
+                        const uint4 h = *reinterpret_cast<const uint4 *>(stage + row * (DP * 2) + ((word ^ (row & 7)) << 4));
+                        __half *const to = out + int64_t(row) * a.o_token;
+                        if (p.vec_out)
+                            *reinterpret_cast<uint4 *>(to) = h;
+                        else
 #pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (32 * c + e < a.head_dim)
-                                out[32 * c + e] = __float2half_rn(__uint_as_float(o[e]) * inverse);
+                            for (int e = 0; e < 8; e++)
+                                to[e] = reinterpret_cast<const __half *>(&h)[e];
                     }
                 }
             }
