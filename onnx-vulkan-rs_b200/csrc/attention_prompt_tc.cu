@@ -548,7 +548,7 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                 bool any_odd = false;
                 for (int i = 0; i < DP / 32; i++)
                     any_odd |= sh.odd[i] != 0;
-#pragma unroll
+#pragma unroll 1  // run once a tile, so what it costs is fetching its instructions
                 for (int c = 0; c < DP / 64; c++) {
                     uint32_t o[2][32];
                     if (tiles > 0) {
