@@ -43,7 +43,7 @@ template <typename... A> static inline cudaError_t ovk_allow_smem(void (*kernel)
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
 }
 
-constexpr int64_t OVK_MAX_HEADS = 1 << 16;
+constexpr int64_t OVK_MAX_HEADS = (1 << 16) - 1;  // heads are a grid dimension
 
 // A [tokens, heads, head_dim] tensor with contiguous heads; `what` names it in the message.  Strides
 // may have any order (a [heads, tokens] tensor is one too); an output's rows must not overlap.
@@ -88,7 +88,7 @@ int32_t ovk_check_kv4_batch(ovk_ctx *ctx, const char *op, const ovk_kv4_batch *b
 // about as many rows each - one in decode - the first place looked at is the right one.
 __device__ __forceinline__ int sequence_of(const int32_t *__restrict__ cu, int batch, int token, int tokens)
 {
-    const int guess = int(int64_t(token) * batch / tokens);  // batch < 2^24
+    const int guess = int(float(token) * (float(batch) / float(tokens)));  // any will do; batch < 2^24
     if (guess < batch && cu[guess] <= token && token < cu[guess + 1])
         return guess;
     int lo = 0, hi = batch;  // cu[lo] <= token < cu[hi] once both are inside

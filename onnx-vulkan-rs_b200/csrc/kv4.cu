@@ -1,16 +1,24 @@
 // The 4-bit key / value cache: argument checks and the write of new tokens.
 //
-// Bytes bound the write: 2 or 4 bytes are read per value and about 0.6 stored.
+// Bytes ought to bound the write: 2 or 4 bytes are read per value and about 0.6
+// stored.  What does is issue: 21784 tokens in f32, one head of 256, keys and values,
+// 50 MB, take 19.6 us (2.6 TB/s) at 74 % of the issue slots, a third of them for the
+// values and the rest for places, ranges and scales.
 // A thread holds eight values of a row - one 32-bit word of codes - and the
 // block_size / 8 threads of a block find its range with shuffles; keys and values
 // of a row go through the same thread, so its place in the cache is found once.
 //
-// The quotients are rounded exactly without dividing: for an fp16 scale s and an
-// integer n <= 16, n s has at most 16 significant bits, and the rest r = x - n s of
-// a value within a step of n s is a whole number of units of its last place that
-// fits 24 bits - so fma(-n, s, x) is r exactly, and a first guess n = rint(x * (1 /
-// s)), off by at most one, is set right by comparing |r| with s / 2.  The scale
-// itself is one f64 quotient a block, keys' on the even lanes and values' on the odd.
+// The quotients are rounded exactly without dividing.  x * (1 / s), the reciprocal
+// good to two units of its last place, is within 2^-17 of x / s up to 32 (beyond, the
+// code is 0 or 15 either way), so n = rint(x * (1 / s)) is right wherever the product
+// lies farther than 2^-16 from a border - all eight values of a
+// word but for one word in some thousands, seven operations a value.  Elsewhere (and
+// where a value is not finite): for an fp16 scale s and an integer n <= 16, n s has
+// at most 16 significant bits, and the rest r = x - n s of a value within a step of n
+// s is a whole number of units of its last place that fits 24 bits - so fma(-n, s, x)
+// is r exactly, and n, off by at most one, is set right by comparing |r| with s / 2.
+// The scale itself is one f64 quotient a block, keys' on the even lanes and values'
+// on the odd.
 #include "attention.cuh"
 
 int32_t ovk_check_kv4(ovk_ctx *ctx, const char *op, const ovk_kv4_cache *c)
@@ -57,8 +65,9 @@ struct AppendArgs {
     __half *scales[2];
     uint8_t *zero_points[2];
     const int32_t *cu, *lens, *table;
-    int64_t items;  // tokens * heads * head_dim / 8
-    int tokens, batch, heads, head_dim, word_shift, block_size, page_size, pages;
+    int tokens, batch, heads, page_size, pages;
+    int word_shift, lane_shift, block_shift;  // log2 of the words of a row, the words of a block, the blocks of a row
+    int page_shift;                           // log2 of page_size, or -1
     int64_t max_pages;
     int *status;
 };
@@ -73,32 +82,48 @@ __device__ __forceinline__ float quotient(float x, float s, float inv, float hal
     return moves ? n + copysignf(1.0f, rest) : n;
 }
 
+// x / N to its exact rounding: the rest of the rounded product with a rounded reciprocal corrects it (Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990).  x is finite.
+template <int N> __device__ __forceinline__ double divided(double x)
+{
+    constexpr double inverse = 1.0 / N;
+    const double q = x * inverse;
+    return fma(fma(-double(N), q, x), inverse, q);
+}
+
+// The larger of the two, NaN where one of them is.
+__device__ __forceinline__ float max_or_nan(float a, float b)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
 {
-    const int64_t item = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int words = a.head_dim / 8;  // a power of two up to 32: a row lies inside a warp
-    // tokens x heads < 2^31
-    const uint32_t at = uint32_t(item >> a.word_shift);
-    const int word = int(item & (words - 1));
-    const int token = int(at / uint32_t(a.heads)), head = int(at - uint32_t(token) * a.heads);
+    // a block's threads: the words (up to 32, a row lies inside a warp) of 256 / words tokens; its head is blockIdx.y
+    const int word = threadIdx.x & ((1 << a.word_shift) - 1), head = blockIdx.y;
+    const int64_t first = int64_t(blockIdx.x) << (8 - a.word_shift);  // below 2^31 but for the last block's end
+    const int token = int(min(first + (threadIdx.x >> a.word_shift), int64_t(a.tokens)));
     OVK_PDL_LAUNCH_DEPENDENTS();
     OVK_PDL_WAIT();
-    int64_t row = -1;
-    if (item < a.items) {
+    int row = -1;  // rows of the cache are fewer than 2^31
+    if (token < a.tokens) {
         const int b = sequence_of(a.cu, a.batch, token, a.tokens);
         if (b >= 0) {
-            const int64_t position = int64_t(a.lens[b]) - (int64_t(a.cu[b + 1]) - token);
-            const int64_t page = position < 0 ? a.max_pages : position / a.page_size;
-            const int where = page < a.max_pages ? a.table[int64_t(b) * a.max_pages + page] : -1;
+            const int length = a.lens[b], from_end = a.cu[b + 1] - token;
+            const uint32_t position = uint32_t(length) - uint32_t(from_end);
+            const uint32_t page = a.page_shift >= 0 ? position >> a.page_shift : position / uint32_t(a.page_size);
+            const int where = length >= from_end && page < a.max_pages ? a.table[b * a.max_pages + page] : -1;
             if (where >= 0 && where < a.pages)
-                row = (int64_t(where) * a.heads + head) * a.page_size + (position - page * a.page_size);
+                row = (where * a.heads + head) * a.page_size + int(position - page * a.page_size);
             else if (word == 0)
                 atomicExch(a.status, OVK_DEV_BAD_PAGE);
         }
     }
-    const int lanes = a.block_size / 8, blocks = a.head_dim / a.block_size;
-    const int block = word / lanes;
+    const int lanes = 1 << a.lane_shift, blocks = 1 << a.block_shift;
+    const int block = word >> a.lane_shift;
     float x[2][8];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
@@ -122,33 +147,48 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
         }
     }
     const int mine = threadIdx.x & 1;
-    const double top = mine ? hi[1] : hi[0], low = mine ? lo[1] : lo[0];
-    const double step = a.zero_points[0] ? (top - low) / 15.0 : fmax(top / 7.0, -low / 8.0);
+    const float most = 3.4e38f;  // an infinity's scale is 65504, and this one's
+    const double top = fminf(mine ? hi[1] : hi[0], most), low = fmaxf(mine ? lo[1] : lo[0], -most);
+    const double step = a.zero_points[0] ? divided<15>(top - low) : fmax(divided<7>(top), -low * 0.125);
     const float my_scale = fminf(float(step), 65504.0f), other_scale = __shfl_xor_sync(0xffffffffu, my_scale, 1);
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         const __half scale = __float2half_rn(mine == j ? my_scale : other_scale);
         const float s = __half2float(scale);
-        const float inv = s > 0.0f ? 1.0f / s : 0.0f, half = s > 0.0f ? 0.5f * s : INFINITY;  // a scale is at least 2^-24: finite
+        const float inv = s > 0.0f ? __fdividef(1.0f, s) : 0.0f, half = s > 0.0f ? 0.5f * s : INFINITY;  // a scale is at least 2^-24: finite
         float zero_f = 8.0f;
         if (a.zero_points[j])
             zero_f = fminf(fmaxf(quotient(-lo[j], s, inv, half), 0.0f), 15.0f);
         const int zero = int(zero_f);
+        // 1.5 * 2^23 + n has the integer in its last bits, and each word so shifted in leaves its leading ones behind
+        const float magic = 12582912.0f, to_zero = magic + zero_f;
+        constexpr uint32_t left_over = 0x4b400000u * 0x11111111u;
         uint32_t codes = 0;
+        float off = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float v = x[j][e] == x[j][e] ? x[j][e] : 0.0f;
-            const float q = fminf(fmaxf(quotient(v, s, inv, half) + zero_f, 0.0f), 15.0f) + 8388608.0f;  // 2^23: the last bits are the code
-            codes |= (__float_as_uint(q) & 15u) << (4 * e);
+        for (int e = 7; e >= 0; e--) {
+            const float t = fmaf(x[j][e], inv, to_zero);
+            off = max_or_nan(off, fabsf(fmaf(x[j][e], inv, to_zero - t)));
+            codes = (codes << 4) + __float_as_uint(fminf(fmaxf(t, magic), magic + 15.0f));
+        }
+        codes -= left_over;
+        if (!(off < 0.5f - 0x1p-16f)) {
+            codes = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = x[j][e] == x[j][e] ? x[j][e] : 0.0f;
+                codes |= uint32_t(fminf(fmaxf(quotient(v, s, inv, half) + zero_f, 0.0f), 15.0f)) << (4 * e);
+            }
         }
         // the block to the right shares this block's byte of zero points
         const int next = __shfl_down_sync(0xffffffffu, zero, lanes);
         if (row >= 0) {
-            reinterpret_cast<uint32_t *>(a.codes[j])[row * words + word] = codes;
-            if (word % lanes == 0) {
-                a.scales[j][row * blocks + block] = scale;
+            const int64_t at = row;
+            reinterpret_cast<uint32_t *>(a.codes[j])[(at << a.word_shift) + word] = codes;
+            if ((word & (lanes - 1)) == 0) {
+                a.scales[j][(at << a.block_shift) + block] = scale;
                 if (a.zero_points[j] && block % 2 == 0)
-                    a.zero_points[j][row * ((blocks + 1) / 2) + block / 2] = uint8_t(zero | (block + 1 < blocks ? next << 4 : 0));
+                    a.zero_points[j][(at << max(a.block_shift - 1, 0)) + block / 2] = uint8_t(zero | (block + 1 < blocks ? next << 4 : 0));
             }
         }
     }
@@ -174,11 +214,8 @@ extern "C" int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, cons
         return rc;
     OVK_REQUIRE(ctx, k->heads == cache->kv_heads && v->heads == cache->kv_heads, "%s: %lld and %lld heads for a cache of %lld", op,
                 (long long)k->heads, (long long)v->heads, (long long)cache->kv_heads);
-    const int64_t items = batch->tokens * cache->kv_heads * (cache->head_dim / 8);
-    OVK_REQUIRE(ctx, batch->tokens * cache->kv_heads < (int64_t(1) << 31) && ceil_div64(items, 256) < (int64_t(1) << 31), "%s: %lld tokens of %lld heads are too many for one call", op,
-                (long long)batch->tokens, (long long)cache->kv_heads);
     OVK_REQUIRE(ctx, ctx, "%s: null context", op);
-    if (items == 0 || batch->batch == 0)
+    if (batch->tokens == 0 || batch->batch == 0)
         return OVK_OK;
     DeviceGuard guard(ctx->device);
     AppendArgs a = {};
@@ -189,17 +226,23 @@ extern "C" int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, cons
     a.scales[0] = static_cast<__half *>(cache->k_scales), a.scales[1] = static_cast<__half *>(cache->v_scales);
     a.zero_points[0] = static_cast<uint8_t *>(cache->k_zero_points), a.zero_points[1] = static_cast<uint8_t *>(cache->v_zero_points);
     a.cu = batch->cu_tokens, a.lens = batch->lens, a.table = batch->block_table;
-    a.items = items;
     a.tokens = int(batch->tokens);
-    a.word_shift = cache->head_dim == 64 ? 3 : cache->head_dim == 128 ? 4 : 5;
-    a.batch = int(batch->batch), a.heads = int(cache->kv_heads), a.head_dim = int(cache->head_dim), a.block_size = int(cache->block_size);
+    auto log2_of = [](int64_t n) {  // of a power of two, -1 of any other number
+        int shift = 0;
+        while (int64_t(1) << shift < n)
+            shift++;
+        return int64_t(1) << shift == n ? shift : -1;
+    };
+    a.word_shift = log2_of(cache->head_dim / 8), a.lane_shift = log2_of(cache->block_size / 8);
+    a.block_shift = log2_of(cache->head_dim / cache->block_size), a.page_shift = log2_of(cache->page_size);
+    a.batch = int(batch->batch), a.heads = int(cache->kv_heads);
     a.page_size = int(cache->page_size), a.pages = int(cache->pages), a.max_pages = batch->max_pages;
     a.status = ctx->dev_status;
-    const unsigned grid = unsigned(ceil_div64(items, 256));
+    const dim3 grid(unsigned(ceil_div64(batch->tokens, 256 >> a.word_shift)), unsigned(cache->kv_heads));
     const bool vec = ovk_rows_aligned(k, elem) && ovk_rows_aligned(v, elem);
     void (*kernel)(AppendArgs) = dtype == OVK_FLOAT ? (vec ? kv4_append_kernel<float, true> : kv4_append_kernel<float, false>)
                                                     : (vec ? kv4_append_kernel<__half, true> : kv4_append_kernel<__half, false>);
-    OVK_CUDA(ctx, ovk_launch_pdl(kernel, dim3(grid), dim3(256), 0, ctx->stream, a));
+    OVK_CUDA(ctx, ovk_launch_pdl(kernel, grid, dim3(256), 0, ctx->stream, a));
     OVK_LAUNCHED(ctx, vec ? "kv4_append" : "kv4_append_scalar");
     return OVK_OK;
 }
