@@ -43,6 +43,11 @@
 // sequence leaves a partial result, and the CTA that is the last to leave one of a
 // sequence joins them, always in CTA order, so results do not depend on timing.  (A
 // second kernel for that cost 5 us a call.)
+//
+// f16, 16 query heads on 2 key heads of 128, block 32: eight contexts of up to 100000
+// tokens take 66 us (3.1 TB/s of 6.5 that a copy reaches; the loads alone take 49, the
+// arithmetic alone 59), 48 contexts of up to 4000 31 us (1.8 TB/s), one context of 900
+// 11 us, which is the way through an empty pipeline and back.
 #pragma once
 
 #include <type_traits>

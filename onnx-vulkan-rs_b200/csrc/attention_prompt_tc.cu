@@ -1,31 +1,40 @@
 // f16 attention over packed prompts on the 5th-generation tensor cores.
 //
-//   S = Q K^T (128 query rows x 128 keys, f32 in tensor memory),
+//   S = Q K^T (128 query rows x 64 or 128 keys, f32 in tensor memory),
 //   P = 2^(scale' S - m) (f16, written back over S),  O = O + P V (f32 in tensor memory),
 //
 // m a per-row reference that follows the running maximum, out = O / sum of P.
 // The two products are 4 head_dim operations per score, the exponential one of 16
-// a cycle and SM: at head_dim 128 both pipes need the same 1024 cycles a tile, so
-// the point of the layout is that neither waits for the other.
+// a cycle and SM: at head_dim 128 both pipes need the same 1024 cycles for 128 x 128
+// scores, so the point of the layout is that neither waits for the other.
 //
 //   softmax groups of four warps   a thread owns a row: tcgen05.ld, maximum, exp2,
 //                                  tcgen05.st, and at the end its row of the result
 //   control group: warp 0          TMA: Q once, then K and V tiles into one ring in
 //                                  the order the products use them
-//                  warps 1, 2      issue tcgen05.mma, one thread each
+//                  warps 1, 2      issue tcgen05.mma
 //   guards                         look through V tiles that some row of the block
 //                                  does not read entirely (below): warp 3 of the
 //                                  control group, or a group of their own
 //
 // Up to 128 elements a head two independent query tiles share each K and V tile
 // (two heads of a group, or neighbouring rows where the group is odd), each with
-// its own issuing thread: while one tile's softmax runs, the tensor core works for
-// the other.  (The core's queue is short - a thread that issues runs at the core's
-// pace - and a wait costs some 300 cycles even where nothing is to be waited for:
-// one thread for both tiles left the core idle for half of the time, 308 us for
-// 8192 tokens of 16 heads.)  256-wide heads fill tensor memory with one tile's O, so
-// there one tile has two S buffers, one thread issues Q K^T and the other P V, and
-// the next scores are computed before the last weights are used.
+// its own issuing warp and two S buffers of 64 keys: while the one half of a tile's
+// softmax runs, the tensor core works for the other half and for the other tile.
+// (The core's queue is short - a warp that issues runs at the core's pace - and a
+// wait costs some 300 cycles even where nothing is to be waited for: one issuer for
+// both tiles took 308 us for 8192 tokens of 16 heads, two 294, with two buffers 280:
+// 982 TFLOP/s.  What is left is the softmax's own latency: 128 rows are four warps,
+// one to a scheduler, and the two tiles run in step.)  256-wide heads fill tensor
+// memory with one tile's O, so there one tile has two S buffers of 128 keys, one warp
+// issues Q K^T and the other P V, and the next scores are computed before the last
+// weights are used: 1340 TFLOP/s for 8192 tokens of 16 heads.
+//
+// A block is one query tile (or two) from its first load to its last store, one on
+// an SM at a time: some 15000 cycles pass outside the products (lookup 1200, first
+// tiles 4000, store 3800, the next block's start 1700, half of the first and last
+// softmax), which is what short prompts and windows cost: 8192 tokens of 16 heads
+// of 256 run at 695 TFLOP/s with a window of 1024.
 //
 // The reference m moves only when a row's maximum passes it by 2^8 (P is then at
 // most 256, sums are f32), so O is rarely rescaled; the softmax group does it
@@ -542,7 +551,7 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
             if (ok) {
                 // By way of the queries' place in shared memory, which no product reads any more: a warp lays its 32 rows
                 // there, 16-byte words exchanged by row so that neither side meets in a bank, and stores them row by row.
-                // (Straight from registers a store touched 32 lines: 6300 cycles a tile of 256-wide rows, now XXXX.)
+                // (Straight from registers a store touched 32 lines: 6300 cycles a tile of 256-wide rows, now 3800.)
                 const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
                 uint8_t *const stage = smem + s * C::Q_BYTES;
                 bool any_odd = false;

@@ -4,6 +4,8 @@
 // that axis's angle: out[a] = x[a] c - x[b] s, out[b] = x[b] c + x[a] s with
 // c, s read from tables of cosines and sines.  Bytes bound it: every element is
 // read and written once, three flops each; the tables are small and stay in L2.
+// 16411 f16 tokens of 16 + 2 heads of 128 take 31.7 us (4.9 TB/s of 6.5 that a copy
+// reaches), 33.8 when the launch waits for the whole of the kernel before.
 //
 // A thread owns the same few pairs (16 bytes of elements) of several heads of one
 // token, so the table entries and positions are loaded once and kept in registers
