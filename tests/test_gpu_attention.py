@@ -652,3 +652,41 @@ def test_two_contexts_at_once_do_not_share_results():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     for c in cs:
         c.close()
+
+
+# ------------------------------------------------------------- rows as they are stored
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,hq,hk,lens,window", [(64, 2, 1, [130, 5], 0), (80, 3, 3, [129, 257], 0), (128, 4, 2, [1, 200], 0), (200, 2, 1, [140], 64),
+                                                 (256, 1, 1, [129, 127], 0), (8, 2, 2, [131], 0)])
+def test_attention_prompt_results_at_any_alignment_have_the_same_bits(dtype, d, hq, hk, lens, window):
+    n = sum(lens)
+    q, k, v = (randn((n, h, d), s, dtype).cuda() for s, h in ((1, hq), (2, hk), (3, hk)))
+    want = ctx().attention_prompt(q, k, v, starts(lens), max(lens), window=window)
+    buffer = torch.full((n * hq * (d + 2) + 9,), 7.0, dtype=dtype, device="cuda")
+    out = buffer[1:1 + n * hq * (d + 2)].view(n, hq, d + 2)[..., :d]  # odd start, a gap of two elements behind each row
+    ctx().attention_prompt(q, k, v, starts(lens), max(lens), window=window, out=out)
+    ctx().flush()
+    assert torch.equal(out, want)
+    assert int((buffer == 7).sum()) >= buffer.numel() - n * hq * d, "elements between the rows were written"
+    assert bool((buffer[1:1 + n * hq * (d + 2)].view(n, hq, d + 2)[..., d:] == 7).all()) and bool((buffer[-8:] == 7).all())
+
+
+@pytest.mark.parametrize("zero_points", [True, False])
+def test_append_of_the_largest_values_and_many_heads(zero_points):
+    top = torch.finfo(F32).max
+    lens, heads = [5, 2], 300
+    k = randn((7, heads, 64), 1, F32)
+    v = randn((7, heads, 64), 2, F32)
+    k[0, 0, 1], k[0, 0, 2], k[0, 1, 3], v[1, 2, 3] = top, -top, -top, top
+    v[2, 299] = torch.linspace(-1e-8, 1e-8, 64)
+    v[3, 298, :32] = 65504.0 * 15
+    v[3, 297, :32] = -65504.0 * 15.5
+    cache = ctx().kv4_cache(4, heads, 3, 64, 32, zero_points)
+    table = [[2, 0], [3, 1]]
+    ctx().kv4_append(cache, k.cuda(), v.cuda(), i32(table), starts(lens), i32(lens))
+    ctx().flush()
+    for which, x in (("k", k), ("v", v)):
+        got, want = cache_rows(cache, which), ref.quantize(x, 32, zero_points)
+        for i, (p, o) in enumerate(place(cache, table, lens, lens)):
+            for a, b, name in zip(got, want, ("codes", "scales", "zero points")):
+                assert torch.equal(a[p, :, o], b[i]), (which, name, i)
