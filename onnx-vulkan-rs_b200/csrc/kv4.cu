@@ -2,17 +2,18 @@
 //
 // Bytes ought to bound the write: 2 or 4 bytes are read per value and about 0.6
 // stored.  What does is issue: 21784 tokens in f32, one head of 256, keys and values,
-// 50 MB, take 19.6 us (2.6 TB/s) at 74 % of the issue slots, a third of them for the
-// values and the rest for places, ranges and scales.
-// A thread holds eight values of a row - one 32-bit word of codes - and the
-// block_size / 8 threads of a block find its range with shuffles; keys and values
+// 50 MB, take some 17.6 us (2.9 TB/s); with eight values a thread 19.6 at 74 % of the
+// issue slots, of which a third went into the values and the rest into places, ranges
+// and scales.
+// A thread holds sixteen values of a row - two 32-bit words of codes - and the
+// block_size / 16 threads of a block find its range with shuffles; keys and values
 // of a row go through the same thread, so its place in the cache is found once.
 //
 // The quotients are rounded exactly without dividing.  x * (1 / s), the reciprocal
 // good to two units of its last place, is within 2^-17 of x / s up to 32 (beyond, the
 // code is 0 or 15 either way), so n = rint(x * (1 / s)) is right wherever the product
-// lies farther than 2^-16 from a border - all eight values of a
-// word but for one word in some thousands, seven operations a value.  Elsewhere (and
+// lies farther than 2^-16 from a border - all sixteen of a
+// thread but for one thread in some thousands, seven operations a value.  Elsewhere (and
 // where a value is not finite): for an fp16 scale s and an integer n <= 16, n s has
 // at most 16 significant bits, and the rest r = x - n s of a value within a step of n
 // s is a whole number of units of its last place that fits 24 bits - so fma(-n, s, x)
@@ -66,7 +67,7 @@ struct AppendArgs {
     uint8_t *zero_points[2];
     const int32_t *cu, *lens, *table;
     int tokens, batch, heads, page_size, pages;
-    int word_shift, lane_shift, block_shift;  // log2 of the words of a row, the words of a block, the blocks of a row
+    int pair_shift, lane_shift, block_shift;  // log2 of the pairs of words of a row and of a block, and the blocks of a row
     int page_shift;                           // log2 of page_size, or -1
     int64_t max_pages;
     int *status;
@@ -102,10 +103,10 @@ __device__ __forceinline__ float max_or_nan(float a, float b)
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
 {
-    // a block's threads: the words (up to 32, a row lies inside a warp) of 256 / words tokens; its head is blockIdx.y
-    const int word = threadIdx.x & ((1 << a.word_shift) - 1), head = blockIdx.y;
-    const int64_t first = int64_t(blockIdx.x) << (8 - a.word_shift);  // below 2^31 but for the last block's end
-    const int token = int(min(first + (threadIdx.x >> a.word_shift), int64_t(a.tokens)));
+    // a block's threads: the pairs of words (up to 16, a row lies inside a warp) of 256 / pairs tokens; its head is blockIdx.y
+    const int pair = threadIdx.x & ((1 << a.pair_shift) - 1), head = blockIdx.y;
+    const int64_t first = int64_t(blockIdx.x) << (8 - a.pair_shift);  // below 2^31 but for the last block's end
+    const int token = int(min(first + (threadIdx.x >> a.pair_shift), int64_t(a.tokens)));
     OVK_PDL_LAUNCH_DEPENDENTS();
     OVK_PDL_WAIT();
     int row = -1;  // rows of the cache are fewer than 2^31
@@ -118,20 +119,20 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
             const int where = length >= from_end && page < a.max_pages ? a.table[b * a.max_pages + page] : -1;
             if (where >= 0 && where < a.pages)
                 row = (where * a.heads + head) * a.page_size + int(position - page * a.page_size);
-            else if (word == 0)
+            else if (pair == 0)
                 atomicExch(a.status, OVK_DEV_BAD_PAGE);
         }
     }
     const int lanes = 1 << a.lane_shift, blocks = 1 << a.block_shift;
-    const int block = word >> a.lane_shift;
-    float x[2][8];
+    const int block = pair >> a.lane_shift;
+    float x[2][16];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         if (row >= 0) {
-            load_row<T, 8, VEC>(static_cast<const T *>(a.x[j]) + token * a.token_stride[j] + head * a.head_stride[j] + 8 * word, x[j]);
+            load_row<T, 16, VEC>(static_cast<const T *>(a.x[j]) + token * a.token_stride[j] + head * a.head_stride[j] + 16 * pair, x[j]);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
+            for (int e = 0; e < 16; e++)
                 x[j][e] = 0.0f;
         }
     }
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
 #pragma unroll
     for (int j = 0; j < 2; j++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++)
+        for (int e = 0; e < 16; e++)
             lo[j] = fminf(lo[j], x[j][e]), hi[j] = fmaxf(hi[j], x[j][e]);
         for (int o = 1; o < lanes; o <<= 1) {
             lo[j] = fminf(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], o));
@@ -163,29 +164,29 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
         // 1.5 * 2^23 + n has the integer in its last bits, and each word so shifted in leaves its leading ones behind
         const float magic = 12582912.0f, to_zero = magic + zero_f;
         constexpr uint32_t left_over = 0x4b400000u * 0x11111111u;
-        uint32_t codes = 0;
+        uint32_t codes[2] = {0, 0};
         float off = 0.0f;
 #pragma unroll
-        for (int e = 7; e >= 0; e--) {
+        for (int e = 15; e >= 0; e--) {
             const float t = fmaf(x[j][e], inv, to_zero);
             off = max_or_nan(off, fabsf(fmaf(x[j][e], inv, to_zero - t)));
-            codes = (codes << 4) + __float_as_uint(fminf(fmaxf(t, magic), magic + 15.0f));
+            codes[e / 8] = (codes[e / 8] << 4) + __float_as_uint(fminf(fmaxf(t, magic), magic + 15.0f));
         }
-        codes -= left_over;
+        codes[0] -= left_over, codes[1] -= left_over;
         if (!(off < 0.5f - 0x1p-16f)) {
-            codes = 0;
+            codes[0] = codes[1] = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
+            for (int e = 0; e < 16; e++) {
                 const float v = x[j][e] == x[j][e] ? x[j][e] : 0.0f;
-                codes |= uint32_t(fminf(fmaxf(quotient(v, s, inv, half) + zero_f, 0.0f), 15.0f)) << (4 * e);
+                codes[e / 8] |= uint32_t(fminf(fmaxf(quotient(v, s, inv, half) + zero_f, 0.0f), 15.0f)) << (4 * (e % 8));
             }
         }
         // the block to the right shares this block's byte of zero points
         const int next = __shfl_down_sync(0xffffffffu, zero, lanes);
         if (row >= 0) {
             const int64_t at = row;
-            reinterpret_cast<uint32_t *>(a.codes[j])[(at << a.word_shift) + word] = codes;
-            if ((word & (lanes - 1)) == 0) {
+            reinterpret_cast<uint2 *>(a.codes[j])[(at << a.pair_shift) + pair] = make_uint2(codes[0], codes[1]);
+            if ((pair & (lanes - 1)) == 0) {
                 a.scales[j][(at << a.block_shift) + block] = scale;
                 if (a.zero_points[j] && block % 2 == 0)
                     a.zero_points[j][(at << max(a.block_shift - 1, 0)) + block / 2] = uint8_t(zero | (block + 1 < blocks ? next << 4 : 0));
@@ -233,12 +234,12 @@ extern "C" int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, cons
             shift++;
         return int64_t(1) << shift == n ? shift : -1;
     };
-    a.word_shift = log2_of(cache->head_dim / 8), a.lane_shift = log2_of(cache->block_size / 8);
+    a.pair_shift = log2_of(cache->head_dim / 16), a.lane_shift = log2_of(cache->block_size / 16);
     a.block_shift = log2_of(cache->head_dim / cache->block_size), a.page_shift = log2_of(cache->page_size);
     a.batch = int(batch->batch), a.heads = int(cache->kv_heads);
     a.page_size = int(cache->page_size), a.pages = int(cache->pages), a.max_pages = batch->max_pages;
     a.status = ctx->dev_status;
-    const dim3 grid(unsigned(ceil_div64(batch->tokens, 256 >> a.word_shift)), unsigned(cache->kv_heads));
+    const dim3 grid(unsigned(ceil_div64(batch->tokens, 256 >> a.pair_shift)), unsigned(cache->kv_heads));
     const bool vec = ovk_rows_aligned(k, elem) && ovk_rows_aligned(v, elem);
     void (*kernel)(AppendArgs) = dtype == OVK_FLOAT ? (vec ? kv4_append_kernel<float, true> : kv4_append_kernel<float, false>)
                                                     : (vec ? kv4_append_kernel<__half, true> : kv4_append_kernel<__half, false>);
