@@ -611,7 +611,7 @@ OVK_API int32_t ovk_attention_kv4_workspace(ovk_ctx *ctx, const ovk_kv4_cache *c
  * so query i has position p = n_k - n_q + i.  causal: it reads keys up to p;
  * window > 0: keys from p - window + 1; a row that reads nothing gives zeros.
  * Scores, softmax and sums are f32.  head_dim 1 to 256.  The f16 tensor-core
- * kernel takes 16-byte aligned rows (head_dim a multiple of 8); other layouts
+ * kernel takes q, k and v with 16-byte aligned rows of any width; other layouts
  * and f32 run on the CUDA cores. */
 typedef struct ovk_prompt_params {
     int64_t q_tokens, k_tokens, batch, head_dim;
