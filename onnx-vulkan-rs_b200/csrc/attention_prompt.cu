@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(Simt<DMAX>::THREADS) attention_prompt_simt_ker
     __shared__ PromptTile where;
     const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
     if (tid < 32)
-        find_prompt_tile<BM>(a, blockIdx.x / a.heads, where);  // the heads of a tile together, the long tiles first
+        find_prompt_tile<BM>(a, blockIdx.x / a.heads, gridDim.x / a.heads, where);  // the heads of a tile together, the long tiles first
     __syncthreads();
     const PromptTile w = where;
     if (w.b < 0)

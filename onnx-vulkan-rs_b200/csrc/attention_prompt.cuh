@@ -27,11 +27,13 @@ struct KeyRange {
 #ifdef __CUDACC__
 // The index-th tile of BM query rows of the batch, counted from the last one (under a causal mask the
 // last tiles are the long ones, which go first).  One warp; the bounds are read 32 sequences at a time,
-// back to front.  Bounds that leave the tensors make the sequence one without rows (or without keys).
-template <int BM> __device__ __forceinline__ void find_prompt_tile(const PromptArgs &a, int index, PromptTile &out)
+// back to front.  Bounds that leave the tensors make the sequence one without rows (or without keys); who
+// reads such bounds reports them, and the last block of `blocks` reads those of the whole batch.
+template <int BM> __device__ __forceinline__ void find_prompt_tile(const PromptArgs &a, int index, int blocks, PromptTile &out)
 {
     const int lane = threadIdx.x & 31;
     int before = 0;
+    bool found = false;
     PromptTile w = {-1, 0, 0, 0, 0, 0};
     for (int base = a.batch - 1; base >= 0; base -= 32) {
         const int b = base - lane;
@@ -43,8 +45,7 @@ template <int BM> __device__ __forceinline__ void find_prompt_tile(const PromptA
             n = end - first;
             if (first < 0 || end < first || end > a.q_tokens || (a.max_q > 0 && n > a.max_q)) {
                 n = 0;
-                if (index == 0)
-                    atomicExch(a.status, OVK_DEV_BAD_SEQUENCE);
+                atomicExch(a.status, OVK_DEV_BAD_SEQUENCE);
             }
         }
         const int tiles = (n + BM - 1) / BM;
@@ -67,11 +68,12 @@ template <int BM> __device__ __forceinline__ void find_prompt_tile(const PromptA
             }
             out = w;
         }
-        if (__any_sync(0xffffffffu, mine))
+        found |= __any_sync(0xffffffffu, mine);
+        if (found && index < blocks - 1)
             return;
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0)
+    if (lane == 0 && !found)
         out = w;
 }
 

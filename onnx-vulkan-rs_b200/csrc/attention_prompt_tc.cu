@@ -138,9 +138,9 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
     OVK_PDL_WAIT();
     if (warp == 0) {
         if (rows_split)
-            find_prompt_tile<2 * BM>(a, index, sh.tile);
+            find_prompt_tile<2 * BM>(a, index, gridDim.x / p.pairs, sh.tile);
         else
-            find_prompt_tile<BM>(a, index, sh.tile);
+            find_prompt_tile<BM>(a, index, gridDim.x / p.pairs, sh.tile);
         __syncwarp();
         if (lane == 0) {
             // how many threads give a ring stage back: one for each query tile that there is

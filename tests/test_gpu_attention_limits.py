@@ -40,3 +40,32 @@ def test_prompt_heads_that_end_inside_a_word(d, wide, gap, shift):
     if gap is not None:
         rows = buffer[shift:shift + n * hq * pitch].view(n, hq, pitch)
         assert bool((rows[..., d:] == 7).all()) and bool((buffer[:shift] == 7).all()) and bool((buffer[shift + n * hq * pitch:] == 7).all())
+
+
+# ------------------------------------------------------- bounds that disagree with the call
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("bad", [0, 30, 69])
+@pytest.mark.parametrize("kind", ["long", "before", "behind"])
+def test_prompt_reports_bad_sequences_of_large_batches(dtype, bad, kind):
+    """A sequence that is left out is reported wherever it lies in the batch."""
+    lens = [3] * 70
+    lens[bad] = 9 if kind == "long" else 3
+    n = sum(lens)
+    q, k = randn((n, 2, 64), 1, dtype).cuda(), randn((n, 1, 64), 2, dtype).cuda()
+    cu = [sum(lens[:i]) for i in range(71)]
+    if kind == "before":  # the sequence before this one ends in front of its own start
+        cu[bad + 1] = -1 if bad == 0 else cu[bad] - 1
+    elif kind == "behind":
+        cu[bad + 1] = n + 5
+    out = ctx().attention_prompt(q, k, k, i32(cu), 8, cu_k=i32([sum(lens[:i]) for i in range(71)]), out=torch.full_like(q, 3.0))
+    with pytest.raises(ovk_b200.OvkError) as e:
+        ctx().flush()
+    assert e.value.status == ovk_b200.INVALID_ARGUMENT and "bounds" in e.value.message
+    if kind == "long":
+        keep = torch.ones(n, dtype=torch.bool)
+        keep[cu[bad]:cu[bad + 1]] = False
+        assert bool((out[~keep.cuda()] == 3).all()) and bool((out[keep.cuda()] != 3).any(-1).all())
+    ctx().attention_prompt(q, k, k, starts(lens), 9)
+    ctx().flush()
+
+
