@@ -150,7 +150,7 @@ int32_t ovk_flush(ovk_ctx *ctx)
                             "4-bit cache: a position or page number read on the device fell outside the cache (it was left out)");
         if (st == OVK_DEV_BAD_SEQUENCE)
             return ovk_fail(ctx, OVK_INVALID_ARGUMENT,
-                            "Attention: sequence bounds read on the device disagree with the call (the sequence was left out)");
+                            "Packed sequences: bounds read on the device disagree with the call (the sequence was left out)");
         return ovk_fail(ctx, OVK_TIMEOUT, "a device-side wait gave up (code %d: %s)", st,
                         st == OVK_DEV_TIMEOUT_TMA    ? "bulk copy never arrived"
                         : st == OVK_DEV_TIMEOUT_MMA  ? "tensor core never signalled"

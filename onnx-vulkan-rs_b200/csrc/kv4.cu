@@ -109,10 +109,15 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
     const int token = int(min(first + (threadIdx.x >> a.pair_shift), int64_t(a.tokens)));
     OVK_PDL_LAUNCH_DEPENDENTS();
     OVK_PDL_WAIT();
+    // bounds that leave the tensors: reported here for the whole batch, left out below
+    if (head == 0)
+        for (int64_t b = int64_t(blockIdx.x) * 256 + threadIdx.x; b < a.batch; b += int64_t(gridDim.x) * 256)
+            if (a.cu[b] < 0 || a.cu[b + 1] < a.cu[b] || a.cu[b + 1] > a.tokens)
+                atomicExch(a.status, OVK_DEV_BAD_SEQUENCE);
     int row = -1;  // rows of the cache are fewer than 2^31
     if (token < a.tokens) {
         const int b = sequence_of(a.cu, a.batch, token, a.tokens);
-        if (b >= 0) {
+        if (b >= 0 && a.cu[b] >= 0 && a.cu[b + 1] <= a.tokens) {
             const int length = a.lens[b], from_end = a.cu[b + 1] - token;
             const uint32_t position = uint32_t(length) - uint32_t(from_end);
             const uint32_t page = a.page_shift >= 0 ? position >> a.page_shift : position / uint32_t(a.page_size);

@@ -69,3 +69,32 @@ def test_prompt_reports_bad_sequences_of_large_batches(dtype, bad, kind):
     ctx().flush()
 
 
+@pytest.mark.parametrize("cu,kept", [([0, 9], []), ([-1, 2], []), ([0, 1, 5], [0]), ([-3, 1, 3], [1, 2]), ([0, 2, 1], None)])
+def test_append_of_bad_bounds_is_left_out_and_reported(cu, kept):
+    """Sequences whose rows lie outside the tensors store nothing; the others store their rows."""
+    batch = len(cu) - 1
+    cache = ctx().kv4_cache(2 * batch, 1, 8, 64, 32)
+    k = torch.ones((3, 1, 64), dtype=F16, device="cuda")
+    table, lens = [[2 * b, 2 * b + 1] for b in range(batch)], [max(cu[b + 1] - cu[b], 0) for b in range(batch)]
+    ctx().kv4_append(cache, k, k, i32(table), i32(cu), i32(lens))
+    with pytest.raises(ovk_b200.OvkError) as e:
+        ctx().flush()
+    assert e.value.status == ovk_b200.INVALID_ARGUMENT and "bounds" in e.value.message
+    # (which sequence rows belong to that two claim is not said)
+    assert kept is None or int((cache.k_scales != 0).any(-1).sum()) == len(kept)
+    ctx().flush()
+
+
+def test_append_reports_bad_bounds_of_a_large_batch():
+    """Bounds that no row falls into, far from the rows there are."""
+    cu = [0] * 2000 + [1]
+    cu[700] = -4
+    cache = ctx().kv4_cache(2, 1, 8, 64, 32)
+    k = torch.ones((1, 1, 64), dtype=F16, device="cuda")
+    ctx().kv4_append(cache, k, k, i32([[0]] * 2000), i32(cu), i32([1] * 2000))
+    with pytest.raises(ovk_b200.OvkError) as e:
+        ctx().flush()
+    assert "bounds" in e.value.message and int((cache.k_scales != 0).any(-1).sum()) == 1
+    ctx().flush()
+
+
