@@ -519,10 +519,11 @@ OVK_API int32_t ovk_qlinear_global_average_pool(ovk_ctx *ctx, const void *x, int
  * stay as they are, and nothing of it is stored to the cache), nothing outside
  * the tensors is touched, and the next ovk_flush returns OVK_INVALID_ARGUMENT.
  *
- * Like every operator these only enqueue on the context's stream.  They keep no
- * state in the context, so calls on several contexts and replays of captured
- * graphs do not disturb one another as long as their outputs, caches and
- * workspaces differ. */
+ * Like every operator these only enqueue on the context's stream.  What they keep
+ * in the context is for the time of a call (ovk_attention_kv4 without a workspace:
+ * partial results and counters that it leaves zero), so calls on several contexts
+ * and replays of captured graphs do not disturb one another as long as their
+ * outputs, caches and workspaces differ. */
 /* One [tokens, heads, head_dim] tensor; elements of a head are contiguous, the
  * strides count elements.  A slice of a fused q | k | v product is one of these. */
 typedef struct ovk_heads {
@@ -587,10 +588,14 @@ OVK_API int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, const o
 /* Causal attention of the new tokens over the cache, their own rows included:
  *   out = softmax(scale q K^T) V,  K and V = (code - zero) * scale of the rows,
  * a token at position p reads positions max(0, p - window + 1) .. p (window 0: no
- * lower limit); one that reads nothing gives zeros.  Scores, softmax and sums are
- * f32.  q and out are [tokens, q_heads, head_dim] of `dtype`, 16-byte aligned rows.
- * max_tokens: the most new tokens a sequence brings (1 in decode); a sequence
- * that brings more is left out as described above.
+ * lower limit); one that reads nothing gives zeros.  Scores, maxima and sums are
+ * f32; what enters the products is fp16 (the tensor cores take nothing wider): the
+ * queries, for OVK_FLOAT as two parts of 22 bits together, and each weight times a
+ * value's scale, rounded alike.  Scores of OVK_FLOAT16 queries are good to 2^-17 of the
+ * largest product in them.  q and out are [tokens, q_heads, head_dim] of `dtype`,
+ * 16-byte aligned rows.
+ * max_tokens: the most new tokens a sequence is expected to bring (1 in decode); it
+ * chooses how many rows are computed together, results hold for any number.
  * workspace: partial results of sequences that several CTAs share, 16-byte
  * aligned, ovk_attention_kv4_workspace() bytes; NULL takes the context's own
  * workspace, which grows on demand.  A call that is being captured into a graph
@@ -610,7 +615,8 @@ OVK_API int32_t ovk_attention_kv4_workspace(ovk_ctx *ctx, const ovk_kv4_cache *c
  * queries are the LAST tokens of the keys' sequence (a chunk after earlier ones),
  * so query i has position p = n_k - n_q + i.  causal: it reads keys up to p;
  * window > 0: keys from p - window + 1; a row that reads nothing gives zeros.
- * Scores, softmax and sums are f32.  head_dim 1 to 256.  The f16 tensor-core
+ * Scores, maxima and sums are f32; OVK_FLOAT16 weights enter the second product as
+ * fp16, the sum of them as f32.  head_dim 1 to 256.  The f16 tensor-core
  * kernel takes q, k and v with 16-byte aligned rows of any width; other layouts
  * and f32 run on the CUDA cores. */
 typedef struct ovk_prompt_params {

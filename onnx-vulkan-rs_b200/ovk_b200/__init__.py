@@ -756,8 +756,9 @@ class Context:
 
     def attention_kv4(self, cache: "KV4Cache", q, block_table, cu_tokens, lens, max_tokens=1, scale=None, window=0, out=None):
         """Causal attention of the new tokens q [tokens, q_heads, head_dim] over the cache, which holds their own rows already.
-        max_tokens: the most new tokens a sequence brings; scale: 1 / sqrt(head_dim) unless given; window: positions a
-        token reads, its own included (0: all before it)."""
+        max_tokens: the most new tokens a sequence is expected to bring (it chooses how many rows are computed together;
+        results hold for any number); scale: 1 / sqrt(head_dim) unless given; window: positions a token reads, its own
+        included (0: all before it)."""
         hq = self._activation("AttentionKV4: q", q, None, None, cache.head_dim)
         n, h, d = q.shape
         b = self._kv4_batch("AttentionKV4", cache, n, block_table, cu_tokens, lens)

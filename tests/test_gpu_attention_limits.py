@@ -98,3 +98,15 @@ def test_append_reports_bad_bounds_of_a_large_batch():
     ctx().flush()
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,hq,hk,new,lens", [(128, 8, 1, [5, 1], [77, 4]), (64, 12, 4, [1, 9], [3, 40]), (256, 4, 1, [70], [90])])
+def test_kv4_more_new_tokens_than_promised(dtype, d, hq, hk, new, lens):
+    """max_tokens chooses a variant; results hold for any number of new tokens."""
+    cache, table = filled_cache(lens, hk, d, 32, 16, True, d)
+    q = randn((sum(new), hq, d), 9, F32, 1.5).to(dtype)
+    for most in (1, 2, max(new), 1000):
+        got = ctx().attention_kv4(cache, q.cuda(), dev(table), starts(new), i32(lens), max_tokens=most)
+        ctx().flush()
+        check_kv4(cache, table, q, new, lens, d ** -0.5, 0, got.cpu())
+
+
