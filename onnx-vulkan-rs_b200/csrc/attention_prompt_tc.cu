@@ -607,23 +607,30 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                                     int64_t(w.first_q + w.row0 + (rows_split ? s * BM : 0)) * a.o_token +
                                     int64_t(rows_split ? head0 : head0 + s) * a.o_head + 8 * word;
                 const int left = a.head_dim - 8 * word;  // elements of the row from this word on: it may end inside the word
-                if (left > 0) {
-                    const bool whole = p.vec_out && left >= 8;
+                auto store = [&](int k, bool whole) {
+                    const int row = r0 + k * (32 / WORDS) + lane / WORDS;
+                    if (row >= rows)
+                        return false;
+                    const uint8_t *const from = stage + row * (DP * 2) + ((word ^ (row & 7)) << 4);
+                    __half *const to = out + int64_t(row) * a.o_token;
+                    if (whole)
+                        *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
+                    else
+#pragma unroll 1
+                        for (int e = 0; e < min(left, 8); e++)
+                            to[e] = reinterpret_cast<const __half *>(from)[e];
+                    return true;
+                };
+                if (p.vec_out && left >= 8) {
 #pragma unroll 8
-                    for (int k = 0; k < WORDS; k++) {
-                        const int row = r0 + k * (32 / WORDS) + lane / WORDS;
-                        if (row >= rows)
+                    for (int k = 0; k < WORDS; k++)
+                        if (!store(k, true))
                             break;
-                        const uint4 h = *reinterpret_cast<const uint4 *>(stage + row * (DP * 2) + ((word ^ (row & 7)) << 4));
-                        __half *const to = out + int64_t(row) * a.o_token;
-                        if (whole)
-                            *reinterpret_cast<uint4 *>(to) = h;
-                        else
-#pragma unroll
-                            for (int e = 0; e < 8; e++)
-                                if (e < left)
-                                    to[e] = reinterpret_cast<const __half *>(&h)[e];
-                    }
+                } else if (left > 0) {
+#pragma unroll 1
+                    for (int k = 0; k < WORDS; k++)
+                        if (!store(k, false))
+                            break;
                 }
             }
         }
