@@ -111,6 +111,10 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// The running maximum of a row that has seen nothing.  Finite, so that a masked score (-infinity) less it is -infinity and
+// not NaN; no score is lower but one that has overflowed.
+constexpr float NO_SCORE = -3.402823466e38f;
+
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float y;

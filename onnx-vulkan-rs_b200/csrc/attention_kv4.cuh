@@ -75,7 +75,7 @@ struct Kv4Args {
 namespace kv4 {
 
 constexpr int STEP = 32;  // tokens of a warp at a time: two products' rows, independent until they meet in the sums
-constexpr float NONE = -1e30f;  // the maximum of a row that has seen nothing (in powers of two)
+constexpr float NONE = NO_SCORE;  // (scores are in powers of two)
 
 template <int D_, int NT_, int PARTS_> struct Shape {
     static constexpr int D = D_, NT = NT_, PARTS = PARTS_;
@@ -312,7 +312,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
     uint8_t *const qf = reinterpret_cast<uint8_t *>(merge) + S::MERGE;
     float *const q_sum = reinterpret_cast<float *>(qf + S::QF);       // [NCH][ROWS]
     float *const q_factor = q_sum + ROWS * NCH;                       // [ROWS]
-    float *const stat = q_factor + ROWS;                              // [WARPS][ROWS] references, then sums
+    float *const stat = q_factor + ROWS;                              // [WARPS][ROWS] maxima, then sums
     const uint32_t sz = ring + S::RING + warp * S::SZ;
 
     OVK_PDL_LAUNCH_DEPENDENTS();
@@ -623,10 +623,12 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         const uint32_t row_at = ring + 2 * S::CODES + 2 * (S::SCALES + S::ZEROS) + place * 4;
 
         float o[NCH][2][NT][4];
-        float m[NT][2], l[NT][2], reference[NT][2];  // reference: m and the scale's exponent, what p is relative to
+        // p = 2^(x - m - lower): the maximum and the scale's exponent are taken off one after the other, since beside a large
+        // maximum the exponent would be rounded away
+        float m[NT][2], l[NT][2], lower = 0.0f;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            m[n][0] = m[n][1] = reference[n][0] = reference[n][1] = NONE;
+            m[n][0] = m[n][1] = NONE;
             l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
             for (int c = 0; c < NCH; c++)
@@ -799,14 +801,15 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    moves |= x[0][n][e] > m[n][e & 1] + 6.0f || x[1][n][e] > m[n][e & 1] + 6.0f;
+                    moves |= x[0][n][e] - m[n][e & 1] > 6.0f || x[1][n][e] - m[n][e & 1] > 6.0f;
             if (__any_sync(0xffffffffu, moves)) {
                 // sums and accumulators so far are brought to the new maximum and the new scale's exponent
                 high = __reduce_max_sync(0xffffffffu, high);
                 const uint32_t new_scale = max(top_scale, min(high, 0x7800u) & 0x7c00u);
                 top_scale = new_scale;
                 // p is smaller by the exponent of the largest scale, less 6
-                const float lower = float(int(new_scale >> 10) - 21);
+                const float lower_before = lower;
+                lower = float(int(new_scale >> 10) - 21);
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -816,9 +819,8 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                         for (int o_ = 4; o_ < 32; o_ <<= 1)
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o_));
                         const float to = fmaxf(m[n][e], most);
-                        const float f = exp2_approx(reference[n][e] - (to + lower));
+                        const float f = exp2_approx((m[n][e] - to) + (lower_before - lower));
                         m[n][e] = to;
-                        reference[n][e] = to + lower;
                         l[n][e] *= f;
 #pragma unroll
                         for (int c = 0; c < NCH; c++) {
@@ -834,7 +836,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        p[h][n][e] = exp2_approx(x[h][n][e] - reference[n][e & 1]);
+                        p[h][n][e] = exp2_approx((x[h][n][e] - m[n][e & 1]) - lower);
                     l[n][0] += p[h][n][0] + p[h][n][2];
                     l[n][1] += p[h][n][1] + p[h][n][3];
                 }
@@ -896,6 +898,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         }
 
         // ------------------------------------------------ join the warps
+        const float unit_weight = power_of_two(int(lower));  // p back to what is relative to the maximum alone
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -904,13 +907,13 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 for (int o_ = 4; o_ < 32; o_ <<= 1)
                     l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o_);
                 if (g == 0) {
-                    stat[warp * ROWS + n * 8 + 2 * t + e] = reference[n][e];
-                    stat[(WARPS + warp) * ROWS + n * 8 + 2 * t + e] = l[n][e];
+                    stat[warp * ROWS + n * 8 + 2 * t + e] = m[n][e];
+                    stat[(WARPS + warp) * ROWS + n * 8 + 2 * t + e] = l[n][e] * unit_weight;
                 }
             }
         if (!consumers_all<CONSUMERS>(ok))
             return;
-        // groups of SLOTS warps add their sums, relative to the largest reference of all, one group after the other
+        // groups of SLOTS warps add their sums, relative to the largest maximum of all, one group after the other
         constexpr float first = S::SUBNORMAL ? 0x1p24f : 1.0f, second = S::SUBNORMAL ? 0x1p20f : 1.0f;
 #pragma unroll
         for (int round = 0; round < WARPS / S::SLOTS; round++) {
@@ -924,7 +927,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
 #pragma unroll
                         for (int w = 0; w < WARPS; w++)
                             most = fmaxf(most, stat[w * ROWS + r]);
-                        const float f = exp2_approx(reference[n][e] - most), f1 = f * first, f2 = f * second;
+                        const float f = exp2_approx(m[n][e] - most) * unit_weight, f1 = f * first, f2 = f * second;
                         float *dst = merge + (warp % S::SLOTS * ROWS + r) * (D + 4) + 4 * g;
 #pragma unroll
                         for (int c = 0; c < NCH; c++) {

@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(Simt<DMAX>::THREADS) attention_prompt_simt_ker
     float o[RT][OC][4], m[RT], l[RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) {
-        m[i] = -1e30f, l[i] = 0.0f;
+        m[i] = NO_SCORE, l[i] = 0.0f;
 #pragma unroll
         for (int c = 0; c < OC; c++)
             o[i][c][0] = o[i][c][1] = o[i][c][2] = o[i][c][3] = 0.0f;
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(Simt<DMAX>::THREADS) attention_prompt_simt_ker
 #pragma unroll
         for (int i = 0; i < RT; i++) {
             const int64_t p = first + ty * RT + i;
-            float most = -1e30f;
+            float most = NO_SCORE;
 #pragma unroll
             for (int j = 0; j < CT; j++) {
                 const int64_t key = j0 + tx + 16 * j;

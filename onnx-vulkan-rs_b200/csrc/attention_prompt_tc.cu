@@ -459,7 +459,8 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
             const uint32_t lanes = uint32_t(warp & 3) << 21;  // 32 lanes a warp
             const uint32_t t_o = tmem + lanes + C::O_COL + s * DP;
             const float scale = a.scale_log2e;
-            float m = -1e30f, l = 0.0f;
+            float m = NO_SCORE, l = 0.0f;
+            float ahead = 8.0f;  // how far a score may pass m; less than any where m is so large that scores have to be rounded (below)
             bool ok = true;
             for (int i = 0; i < tiles; i++) {
                 const int buffer = 2 * s + (i & 1);
@@ -500,9 +501,20 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                 for (int e = 4; e < BN; e++)
                     most[e & 3] = fmaxf(most[e & 3], __uint_as_float(x[e >> 5][e & 31]));
                 const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * scale;
-                if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                float factor = scale;
+                if (__any_sync(0xffffffffu, top - m > ahead)) {  // the difference is exact where it matters
                     const float to = fmaxf(m, top), f = exp2_approx(m - to);
                     m = to;
+                    // m is a rounded product, off by up to 2^-25 |m|; the multiply-add below uses unrounded ones.  That is a
+                    // factor common to all of a row's weights, but far from zero it passes fp16's range: there scores are
+                    // rounded too.
+                    ahead = fabsf(m) > 0x1p22f && m != NO_SCORE ? -INFINITY : 8.0f;
+                    if (__any_sync(0xffffffffu, ahead < 0.0f)) {
+                        factor = 1.0f;
+#pragma unroll
+                        for (int e = 0; e < BN; e++)
+                            x[e >> 5][e & 31] = __float_as_uint(__uint_as_float(x[e >> 5][e & 31]) * scale);
+                    }
                     l *= f;
                     if (i > 0) {
                         // the product before this one may still be writing O
@@ -529,8 +541,8 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
                         const int at = 64 * c + 2 * e;
-                        const float p0 = exp2_approx(fmaf(__uint_as_float(x[at >> 5][at & 31]), scale, -m));
-                        const float p1 = exp2_approx(fmaf(__uint_as_float(x[at >> 5][(at & 31) + 1]), scale, -m));
+                        const float p0 = exp2_approx(fmaf(__uint_as_float(x[at >> 5][at & 31]), factor, -m));
+                        const float p1 = exp2_approx(fmaf(__uint_as_float(x[at >> 5][(at & 31) + 1]), factor, -m));
                         sum[(2 * e) & 3] += p0;
                         sum[(2 * e + 1) & 3] += p1;
                         out[e] = pack_halves(p0, p1);

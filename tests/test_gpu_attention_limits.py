@@ -110,3 +110,68 @@ def test_kv4_more_new_tokens_than_promised(dtype, d, hq, hk, new, lens):
         check_kv4(cache, table, q, new, lens, d ** -0.5, 0, got.cpu())
 
 
+# --------------------------------------------------- scores and weights far from one another
+@pytest.mark.parametrize("score", [-1e31, -3e37, 1e37])
+@pytest.mark.parametrize("d,split", [(64, 8), (128, 16), (256, 8), (33, 4)])
+def test_prompt_f32_scores_of_any_size(score, d, split):
+    """A row with one key gives that key's value, however low its score; of several keys the highest score takes all."""
+    n = 70
+    q, k = torch.zeros(n, 2, d), torch.zeros(n, 1, d)
+    v = randn((n, 1, d), 3)
+    root = math.sqrt(abs(score))
+    q[..., 1], k[..., 1] = root, math.copysign(root, score)
+    k[:, 0, 1] *= 1 + torch.arange(n) / n  # farther from zero with each key
+    cu = [0, 1, split, n]
+    got = ctx().attention_prompt(q.cuda(), k.cuda(), v.cuda(), i32(cu), scale=1.0)
+    ctx().flush()
+    for a, b in zip(cu, cu[1:]):
+        for i in range(a, b):  # scores are in steps of more than a weight's whole range
+            want = v[a if score < 0 else i]
+            assert bool(((got[i].cpu() - want).abs() <= 2.0 ** -21 * want.abs()).all()), (i, float(got[i].abs().max()))
+
+
+SIZES = [1.0, 37.3, 300.7, 5.1e3, 1.03e6, 1e27]  # scales that bring a score of a million to 2^20 .. 2^110
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("scale", SIZES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_f16_scores_of_any_size(d, scale, sign):
+    """Equal scores, however large: the mean of the values that a row reads."""
+    q, k = torch.zeros(250, 2, d, dtype=F16), torch.zeros(250, 1, d, dtype=F16)
+    q[..., 0], k[..., 0] = 1000.0, sign * 1000.0
+    q[..., 1], k[..., 1] = 3.0, 3.0
+    v = randn((250, 1, d), 3, F16)
+    got = ctx().attention_prompt(q.cuda(), k.cuda(), v.cuda(), starts([1] * 50 + [200]), scale=scale)
+    ctx().flush()
+    assert bool(((got[:50].cpu() - v[:50]).abs() <= 2.0 ** -11 * v[:50].abs()).all())
+    x, count = v[50:].double(), torch.arange(1, 201)[:, None, None]
+    # a weight is one fp16 number (2^-11), sums are f32
+    ref.check(got[50:], (x.cumsum(0) / count).expand(200, 2, d), (x.abs().cumsum(0) / count * (2.0 ** -11 + 210 * 2.0 ** -23)).expand(200, 2, d), "mean")
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("scale", SIZES)
+@pytest.mark.parametrize("d,lens", [(64, [1]), (128, [1, 1]), (256, [1, 40]), (128, [700])])
+def test_kv4_scores_of_any_size(dtype, d, lens, scale, sign):
+    """Equal scores, however large: the mean of the cached values."""
+    table, pages = make_table(lens, 16, 1)
+    cache = ctx().kv4_cache(pages, 1, 16, d, 32)
+    total = sum(lens)
+    k, v = torch.zeros(total, 1, d), randn((total, 1, d), 2, F32, 3e-4)
+    k[..., 0] = sign * 1000.0
+    ctx().kv4_append(cache, k.cuda(), v.cuda(), dev(table), starts(lens), i32(lens))
+    q = torch.zeros(len(lens), 4, d, dtype=dtype)
+    q[..., 0] = 1000.0
+    got = ctx().attention_kv4(cache, q.cuda(), dev(table), starts([1] * len(lens)), i32(lens), scale=scale)
+    ctx().flush()
+    values = ref.dequantize(*cache_rows(cache, "v"))
+    for b, n in enumerate(lens):
+        at = torch.arange(n)
+        rows = values[torch.as_tensor(table[b])[at // 16].long(), 0, at % 16]
+        # a weight times a value's scale is one fp16 number (f16) or two (f32)
+        p_error = 2.0 ** -11 if dtype == F16 else 2.0 ** -21
+        ref.check(got[b], rows.mean(0).expand(4, d), (rows.abs().mean(0) * (p_error + (n + 8) * 2.0 ** -23)).expand(4, d), f"sequence {b}")
+
+
