@@ -616,7 +616,8 @@ OVK_API int32_t ovk_attention_kv4_workspace(ovk_ctx *ctx, const ovk_kv4_cache *c
  * so query i has position p = n_k - n_q + i.  causal: it reads keys up to p;
  * window > 0: keys from p - window + 1; a row that reads nothing gives zeros.
  * Scores, maxima and sums are f32; OVK_FLOAT16 weights enter the second product as
- * fp16, the sum of them as f32.  head_dim 1 to 256.  The f16 tensor-core
+ * fp16 (off by 2^-11 of themselves or 2^-32 of the row's largest, if that is more),
+ * the sum of them as f32.  head_dim 1 to 256.  The f16 tensor-core
  * kernel takes q, k and v with 16-byte aligned rows of any width; other layouts
  * and f32 run on the CUDA cores. */
 typedef struct ovk_prompt_params {

@@ -36,9 +36,10 @@
 // softmax), which is what short prompts and windows cost: 8192 tokens of 16 heads
 // of 256 run at 695 TFLOP/s with a window of 1024.
 //
-// The reference m moves only when a row's maximum passes it by 2^8 (P is then at
-// most 256, sums are f32), so O is rarely rescaled; the softmax group does it
-// itself, between the products that write O.
+// The reference m lies 7 below the row's maximum and moves only when that passes it by 15, so O is rarely rescaled;
+// the softmax group does it itself, between the products that write O.  P then has 2^7 to 2^15 where the row's largest
+// score is: fp16 holds weights down to 2^-21 of that in full and counts what is below in steps of 2^-31, so that a long
+// flat tail is not lost (sums are f32).
 //
 // Masked weights are exactly 0, and 0 times an infinity is NaN: in tiles that are
 // not read whole, the guards zero the V rows behind the sequence's end and every
@@ -460,7 +461,7 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
             const uint32_t t_o = tmem + lanes + C::O_COL + s * DP;
             const float scale = a.scale_log2e;
             float m = NO_SCORE, l = 0.0f;
-            float ahead = 8.0f;  // how far a score may pass m; less than any where m is so large that scores have to be rounded (below)
+            float ahead = 15.0f;  // how far a score may pass m; less than any where m is so large that scores have to be rounded (below)
             bool ok = true;
             for (int i = 0; i < tiles; i++) {
                 const int buffer = 2 * s + (i & 1);
@@ -503,12 +504,12 @@ attention_prompt_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __gri
                 const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * scale;
                 float factor = scale;
                 if (__any_sync(0xffffffffu, top - m > ahead)) {  // the difference is exact where it matters
-                    const float to = fmaxf(m, top), f = exp2_approx(m - to);
+                    const float to = fmaxf(m, top - 7.0f), f = exp2_approx(m - to);
                     m = to;
                     // m is a rounded product, off by up to 2^-25 |m|; the multiply-add below uses unrounded ones.  That is a
                     // factor common to all of a row's weights, but far from zero it passes fp16's range: there scores are
                     // rounded too.
-                    ahead = fabsf(m) > 0x1p22f && m != NO_SCORE ? -INFINITY : 8.0f;
+                    ahead = fabsf(m) > 0x1p22f && m != NO_SCORE ? -INFINITY : 15.0f;
                     if (__any_sync(0xffffffffu, ahead < 0.0f)) {
                         factor = 1.0f;
 #pragma unroll

@@ -175,3 +175,31 @@ def test_kv4_scores_of_any_size(dtype, d, lens, scale, sign):
         ref.check(got[b], rows.mean(0).expand(4, d), (rows.abs().mean(0) * (p_error + (n + 8) * 2.0 ** -23)).expand(4, d), f"sequence {b}")
 
 
+@pytest.mark.parametrize("d,heads", [(64, 1), (128, 2), (256, 1)])
+@pytest.mark.parametrize("peak", ["first", "last"])
+def test_prompt_f16_long_flat_tail(d, heads, peak):
+    """One key outweighs each of thousands by 2^26, which together are half a thousandth of it: weights are f16, off by 2^-11 of
+    themselves or 2^-32 of the largest, whichever is more."""
+    n, m = 32768, 128  # keys; queries, the last m tokens
+    q = torch.zeros(m, heads, d, dtype=F16)
+    k, v = torch.zeros(n, 1, d, dtype=F16), torch.zeros(n, 1, d, dtype=F16)
+    q[..., 0] = 8.0
+    k[..., 0] = -2.25  # scores of -18: e^-18 = 2^-25.97
+    v[..., 0], v[:, 0, 1] = 1.0, torch.linspace(-1, 1, n).half()
+    at = 0 if peak == "first" else n - m
+    k[at, 0, 0], v[at, 0, :2] = 0.0, 0.0
+    v[at, 0, 2] = 1.0
+    got = ctx().attention_prompt(q.cuda(), k.cuda(), v.cuda(), i32([0, m]), m, cu_k=i32([0, n]), scale=1.0).double().cpu()
+    ctx().flush()
+    w = math.exp(-18.0)
+    for i in (0, 1, m // 2, m - 1):
+        reads = n - m + i + 1
+        below = (reads - 1) * w
+        total = 1 + below
+        # each weight's rounding, 2^-11 of it or (reads - 1) of 2^-32 in all; f32 sums; the result's half step
+        slack = below * 2.0 ** -11 + reads * 2.0 ** -32 + below * reads * 2.0 ** -23
+        want = torch.tensor([below, float(v[:reads, 0, 1].double().sum()) * w, 1.0]) / total
+        for e, tol in ((0, slack), (1, slack), (2, 2.0 ** -11)):
+            assert float((got[i, :, e] - want[e]).abs().max()) <= tol + 2.0 ** -11 * abs(float(want[e])), (i, e, got[i, :, e], want[e])
+
+
