@@ -623,20 +623,21 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         const uint32_t row_at = ring + 2 * S::CODES + 2 * (S::SCALES + S::ZEROS) + place * 4;
 
         float o[NCH][2][NT][4];
-        // p = 2^(x - m - lower): the maximum and the scale's exponent are taken off one after the other, since beside a large
-        // maximum the exponent would be rounded away
-        float m[NT][2], l[NT][2], lower = 0.0f;
+        // p = 2^(x - m - lower): the maximum and the exponent of the largest scale that the row has read are taken off one
+        // after the other, since beside a large maximum the exponent would be rounded away
+        float m[NT][2], l[NT][2], lower[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             m[n][0] = m[n][1] = NONE;
             l[n][0] = l[n][1] = 0.0f;
+            lower[n][0] = lower[n][1] = -21.0f;
 #pragma unroll
             for (int c = 0; c < NCH; c++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     o[c][0][n][e] = o[c][1][n][e] = 0.0f;
         }
-        uint32_t top_scale = 0;  // fp16 bits of the V scale that the maximum allows for
+        uint32_t top_scale = 0;  // fp16 bits of the V scale that every row's `lower` allows for
         bool ok = true;
         for (int u = 0; u < units_here; u++) {
             ok = wait(&full[stage], phase, dead, a.status, OVK_DEV_TIMEOUT_TMA);
@@ -803,13 +804,35 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 for (int e = 0; e < 4; e++)
                     moves |= x[0][n][e] - m[n][e & 1] > 6.0f || x[1][n][e] - m[n][e & 1] > 6.0f;
             if (__any_sync(0xffffffffu, moves)) {
-                // sums and accumulators so far are brought to the new maximum and the new scale's exponent
-                high = __reduce_max_sync(0xffffffffu, high);
-                const uint32_t new_scale = max(top_scale, min(high, 0x7800u) & 0x7c00u);
-                top_scale = new_scale;
-                // p is smaller by the exponent of the largest scale, less 6
-                const float lower_before = lower;
-                lower = float(int(new_scale >> 10) - 21);
+                // Sums and accumulators so far are brought to the new maximum and the new scale's exponent, less 6.  A scale
+                // counts for the rows that read its token: elsewhere it may be anything, and p would sink below fp16's range.
+                auto exponent_of = [](uint32_t scale) { return float(int(min(scale, 0x7800u) >> 10) - 21); };
+                float next[NT][2];
+                if (masked) {
+                    const bool there = (present >> lane) & 1u;
+                    const int token = token0 + lane;
+                    uint32_t least = 0x7fffu;
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const int p = __shfl_sync(0xffffffffu, pos[n][i & 1], i >> 1);  // column i belongs to lanes of t = i / 2
+                            const bool reads = p < 0 || (there && token <= p && !(window > 0 && token <= p - window));
+                            const uint32_t scale = __reduce_max_sync(0xffffffffu, reads ? high : 0u);
+                            const float own = exponent_of(scale);
+                            if (i >> 1 == t)
+                                next[n][i & 1] = fmaxf(lower[n][i & 1], own);
+                            least = min(least, scale);
+                        }
+                    top_scale = max(top_scale, min(least, 0x7800u) & 0x7c00u);
+                } else {
+                    const uint32_t scale = __reduce_max_sync(0xffffffffu, high);
+                    const float own = exponent_of(scale);
+                    top_scale = max(top_scale, min(scale, 0x7800u) & 0x7c00u);
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+                        next[n][0] = fmaxf(lower[n][0], own), next[n][1] = fmaxf(lower[n][1], own);
+                }
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -819,8 +842,8 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                         for (int o_ = 4; o_ < 32; o_ <<= 1)
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o_));
                         const float to = fmaxf(m[n][e], most);
-                        const float f = exp2_approx((m[n][e] - to) + (lower_before - lower));
-                        m[n][e] = to;
+                        const float f = exp2_approx((m[n][e] - to) + (lower[n][e] - next[n][e]));
+                        m[n][e] = to, lower[n][e] = next[n][e];
                         l[n][e] *= f;
 #pragma unroll
                         for (int c = 0; c < NCH; c++) {
@@ -836,7 +859,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        p[h][n][e] = exp2_approx((x[h][n][e] - m[n][e & 1]) - lower);
+                        p[h][n][e] = exp2_approx((x[h][n][e] - m[n][e & 1]) - lower[n][e & 1]);
                     l[n][0] += p[h][n][0] + p[h][n][2];
                     l[n][1] += p[h][n][1] + p[h][n][3];
                 }
@@ -898,7 +921,6 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         }
 
         // ------------------------------------------------ join the warps
-        const float unit_weight = power_of_two(int(lower));  // p back to what is relative to the maximum alone
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -908,7 +930,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                     l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o_);
                 if (g == 0) {
                     stat[warp * ROWS + n * 8 + 2 * t + e] = m[n][e];
-                    stat[(WARPS + warp) * ROWS + n * 8 + 2 * t + e] = l[n][e] * unit_weight;
+                    stat[(WARPS + warp) * ROWS + n * 8 + 2 * t + e] = l[n][e] * power_of_two(int(lower[n][e]));
                 }
             }
         if (!consumers_all<CONSUMERS>(ok))
@@ -927,7 +949,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
 #pragma unroll
                         for (int w = 0; w < WARPS; w++)
                             most = fmaxf(most, stat[w * ROWS + r]);
-                        const float f = exp2_approx(m[n][e] - most) * unit_weight, f1 = f * first, f2 = f * second;
+                        const float f = exp2_approx(m[n][e] - most) * power_of_two(int(lower[n][e])), f1 = f * first, f2 = f * second;
                         float *dst = merge + (warp % S::SLOTS * ROWS + r) * (D + 4) + 4 * g;
 #pragma unroll
                         for (int c = 0; c < NCH; c++) {

@@ -203,3 +203,38 @@ def test_prompt_f16_long_flat_tail(d, heads, peak):
             assert float((got[i, :, e] - want[e]).abs().max()) <= tol + 2.0 ** -11 * abs(float(want[e])), (i, e, got[i, :, e], want[e])
 
 
+# ------------------------------------------------------------ what lies in masked places
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,hq,block", [(64, 2, 64), (128, 4, 32), (128, 12, 128), (256, 4, 32)])
+@pytest.mark.parametrize("scale", [math.inf, math.nan, 65504.0])
+@pytest.mark.parametrize("new,lens,window,at", [([1], [100], 33, 65), ([3], [100], 0, 99), ([2], [70], 20, 48), ([4], [64], 0, 61)])
+def test_kv4_scales_in_masked_places_leave_small_values_exact(dtype, d, hq, block, scale, new, lens, window, at):
+    """A value scale that some rows must not read, far above those that they read, costs them no accuracy."""
+    table, pages = make_table(lens, 16, 1)
+    cache = ctx().kv4_cache(pages, 1, 16, d, block)
+    k, v = randn((lens[0], 1, d), 1), randn((lens[0], 1, d), 2, F32, 2e-4)
+    ctx().kv4_append(cache, k.cuda(), v.cuda(), dev(table), starts(lens), i32(lens))
+    ctx().flush()
+    clean = {w: ref.dequantize(*cache_rows(cache, w)) for w in ("k", "v")}
+    sizes = ref.row_sizes(*cache_rows(cache, "k"))
+    cache.v_scales[int(table[0][at // 16]), 0, at % 16] = scale
+    q = randn((new[0], hq, d), 9, F32, 1.5).to(dtype)
+    got = ctx().attention_kv4(cache, q.cuda(), dev(table), starts(new), i32(lens), max_tokens=new[0], window=window)
+    ctx().flush()
+    got, n, checked = got.cpu(), lens[0], 0
+    p_error, q_error = (2.0 ** -21, 2.0 ** -21) if dtype == F32 else (2.0 ** -11, 0.0)
+    for i in range(new[0]):
+        last = n - new[0] + i
+        first = max(0, last - window + 1) if window else 0
+        if first <= at <= last:
+            continue
+        t = torch.arange(first, last + 1)
+        page = torch.as_tensor(table[0])[t // 16].long()
+        for h in range(hq):
+            want, bound = ref.attend(q[i:i + 1, h].double(), clean["k"][page, 0, t % 16], clean["v"][page, 0, t % 16], d ** -0.5, False, 0,
+                                     p_error, q_error, sizes[page, 0, t % 16])
+            ref.check(got[i:i + 1, h], want, bound, f"row {i} head {h}")
+            checked += 1
+    assert checked
+
+
