@@ -312,7 +312,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
     uint8_t *const qf = reinterpret_cast<uint8_t *>(merge) + S::MERGE;
     float *const q_sum = reinterpret_cast<float *>(qf + S::QF);       // [NCH][ROWS]
     float *const q_factor = q_sum + ROWS * NCH;                       // [ROWS]
-    float *const stat = q_factor + ROWS;                              // [WARPS][ROWS] maxima, then sums
+    float *const stat = q_factor + ROWS;                              // [WARPS][ROWS] references, then sums
     const uint32_t sz = ring + S::RING + warp * S::SZ;
 
     OVK_PDL_LAUNCH_DEPENDENTS();
@@ -623,21 +623,22 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         const uint32_t row_at = ring + 2 * S::CODES + 2 * (S::SCALES + S::ZEROS) + place * 4;
 
         float o[NCH][2][NT][4];
-        // p = 2^(x - m - lower): the maximum and the exponent of the largest scale that the row has read are taken off one
-        // after the other, since beside a large maximum the exponent would be rounded away
-        float m[NT][2], l[NT][2], lower[NT][2];
+        // p = 2^(x - reference): the reference is the maximum m and the exponent, less 21, of the largest scale that the row
+        // has read.  A maximum beyond FAR would round that exponent away, or up to its own last place: there it is m alone, and
+        // no score may be ahead of it (p is then at most 1, which leaves any scale in fp16's range).
+        constexpr float FAR = 0x1p20f, AHEAD = 6.0f;
+        float limit[NT][2], l[NT][2], reference[NT][2];  // limit: m and what a score may be ahead of it
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            m[n][0] = m[n][1] = NONE;
+            limit[n][0] = limit[n][1] = reference[n][0] = reference[n][1] = NONE;
             l[n][0] = l[n][1] = 0.0f;
-            lower[n][0] = lower[n][1] = -21.0f;
 #pragma unroll
             for (int c = 0; c < NCH; c++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     o[c][0][n][e] = o[c][1][n][e] = 0.0f;
         }
-        uint32_t top_scale = 0;  // fp16 bits of the V scale that every row's `lower` allows for
+        uint32_t top_scale = 0;  // fp16 bits of the V scale that every row's reference allows for
         bool ok = true;
         for (int u = 0; u < units_here; u++) {
             ok = wait(&full[stage], phase, dead, a.status, OVK_DEV_TIMEOUT_TMA);
@@ -802,36 +803,35 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    moves |= x[0][n][e] - m[n][e & 1] > 6.0f || x[1][n][e] - m[n][e & 1] > 6.0f;
+                    moves |= x[0][n][e] > limit[n][e & 1] || x[1][n][e] > limit[n][e & 1];
             if (__any_sync(0xffffffffu, moves)) {
-                // Sums and accumulators so far are brought to the new maximum and the new scale's exponent, less 6.  A scale
+                // Sums and accumulators so far are brought to the new maximum and the new scale's exponent.  A scale
                 // counts for the rows that read its token: elsewhere it may be anything, and p would sink below fp16's range.
-                auto exponent_of = [](uint32_t scale) { return float(int(min(scale, 0x7800u) >> 10) - 21); };
-                float next[NT][2];
+                // Tokens that only some rows read are looked through row by row where one has the largest exponent.
+                uint32_t largest = high;  // of the tokens that all rows read
+                bool by_row = false;
                 if (masked) {
-                    const bool there = (present >> lane) & 1u;
                     const int token = token0 + lane;
-                    uint32_t least = 0x7fffu;
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const int p = __shfl_sync(0xffffffffu, pos[n][i & 1], i >> 1);  // column i belongs to lanes of t = i / 2
-                            const bool reads = p < 0 || (there && token <= p && !(window > 0 && token <= p - window));
-                            const uint32_t scale = __reduce_max_sync(0xffffffffu, reads ? high : 0u);
-                            const float own = exponent_of(scale);
-                            if (i >> 1 == t)
-                                next[n][i & 1] = fmaxf(lower[n][i & 1], own);
-                            least = min(least, scale);
-                        }
-                    top_scale = max(top_scale, min(least, 0x7800u) & 0x7c00u);
-                } else {
-                    const uint32_t scale = __reduce_max_sync(0xffffffffu, high);
-                    const float own = exponent_of(scale);
-                    top_scale = max(top_scale, min(scale, 0x7800u) & 0x7c00u);
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-                        next[n][0] = fmaxf(lower[n][0], own), next[n][1] = fmaxf(lower[n][1], own);
+                    const bool there = (present >> lane) & 1u;
+                    const bool by_all = there && token <= pos_first && !(window > 0 && token <= pos_last - window);
+                    const bool by_some = there && token <= pos_last && !(window > 0 && token <= pos_first - window);
+                    largest = by_all ? high : 0u;
+                    by_row = __any_sync(0xffffffffu, by_some && !by_all);
+                    if (by_row)
+                        by_row = __reduce_max_sync(0xffffffffu, by_some ? high : 0u) >> 10 > __reduce_max_sync(0xffffffffu, largest) >> 10;
+                }
+                largest = min(__reduce_max_sync(0xffffffffu, largest) >> 10, 30u);
+                uint32_t exponents = largest * 0x01010101u;  // of this lane's columns, a byte each
+                if (by_row) {
+#pragma unroll 1
+                    for (int i = 0; i < rows; i++) {
+                        const int p = seq.len - seq.n + (row0 + i) / a.group, token = token0 + lane;
+                        const bool reads = ((present >> lane) & 1u) && token <= p && !(window > 0 && token <= p - window);
+                        const uint32_t its = min(__reduce_max_sync(0xffffffffu, reads ? high : 0u) >> 10, 30u);
+                        const int column = (i >> 3) * 2 + (i & 1);
+                        if (((i & 7) >> 1) == t)
+                            exponents = (exponents & ~(255u << (8 * column))) | max(its, largest) << (8 * column);
+                    }
                 }
 #pragma unroll
                 for (int n = 0; n < NT; n++)
@@ -841,9 +841,13 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
 #pragma unroll
                         for (int o_ = 4; o_ < 32; o_ <<= 1)
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o_));
-                        const float to = fmaxf(m[n][e], most);
-                        const float f = exp2_approx((m[n][e] - to) + (lower[n][e] - next[n][e]));
-                        m[n][e] = to, lower[n][e] = next[n][e];
+                        const float m = fabsf(limit[n][e]) > FAR ? limit[n][e] : limit[n][e] - AHEAD;
+                        const float before = m == NONE ? -21.0f : rintf(reference[n][e] - m);
+                        const float to = fmaxf(m, most);
+                        const bool far = fabsf(to) > FAR;
+                        const float next = far ? to : to + fmaxf(before, float(int((exponents >> (16 * n + 8 * e)) & 255u) - 21));
+                        const float f = exp2_approx(reference[n][e] - next);
+                        limit[n][e] = far ? to : to + AHEAD, reference[n][e] = next;
                         l[n][e] *= f;
 #pragma unroll
                         for (int c = 0; c < NCH; c++) {
@@ -851,6 +855,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                             o[c][1][n][e] *= f, o[c][1][n][e + 2] *= f;
                         }
                     }
+                top_scale = max(top_scale, largest << 10);
             }
             float p[2][NT][4];
 #pragma unroll
@@ -859,7 +864,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        p[h][n][e] = exp2_approx((x[h][n][e] - m[n][e & 1]) - lower[n][e & 1]);
+                        p[h][n][e] = exp2_approx(x[h][n][e] - reference[n][e & 1]);
                     l[n][0] += p[h][n][0] + p[h][n][2];
                     l[n][1] += p[h][n][1] + p[h][n][3];
                 }
@@ -929,13 +934,13 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 for (int o_ = 4; o_ < 32; o_ <<= 1)
                     l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o_);
                 if (g == 0) {
-                    stat[warp * ROWS + n * 8 + 2 * t + e] = m[n][e];
-                    stat[(WARPS + warp) * ROWS + n * 8 + 2 * t + e] = l[n][e] * power_of_two(int(lower[n][e]));
+                    stat[warp * ROWS + n * 8 + 2 * t + e] = reference[n][e];
+                    stat[(WARPS + warp) * ROWS + n * 8 + 2 * t + e] = l[n][e];
                 }
             }
         if (!consumers_all<CONSUMERS>(ok))
             return;
-        // groups of SLOTS warps add their sums, relative to the largest maximum of all, one group after the other
+        // groups of SLOTS warps add their sums, relative to the largest reference of all, one group after the other
         constexpr float first = S::SUBNORMAL ? 0x1p24f : 1.0f, second = S::SUBNORMAL ? 0x1p20f : 1.0f;
 #pragma unroll
         for (int round = 0; round < WARPS / S::SLOTS; round++) {
@@ -949,7 +954,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
 #pragma unroll
                         for (int w = 0; w < WARPS; w++)
                             most = fmaxf(most, stat[w * ROWS + r]);
-                        const float f = exp2_approx(m[n][e] - most) * power_of_two(int(lower[n][e])), f1 = f * first, f2 = f * second;
+                        const float f = exp2_approx(reference[n][e] - most), f1 = f * first, f2 = f * second;
                         float *dst = merge + (warp % S::SLOTS * ROWS + r) * (D + 4) + 4 * g;
 #pragma unroll
                         for (int c = 0; c < NCH; c++) {
