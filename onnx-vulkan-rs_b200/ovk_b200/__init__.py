@@ -658,6 +658,8 @@ class Context:
         if (_raw_stream()(self.device) or 1) == self._stream:
             return None
         import torch
+        if self._stream == 1:  # the default stream's handle is not one that torch takes
+            return torch.cuda.default_stream(self.device)
         return torch.cuda.ExternalStream(self._stream, device=torch.device("cuda", self.device))
 
     @staticmethod

@@ -238,3 +238,24 @@ def test_kv4_scales_in_masked_places_leave_small_values_exact(dtype, d, hq, bloc
     assert checked
 
 
+def test_a_context_of_the_default_stream_under_another_current_stream():
+    lens = [70, 5]
+    table, pages = make_table(lens, 16, 1)
+    cos, sin = (torch.rand(100, 64, device="cuda") for _ in range(2))
+    q, k, v = (randn((75, h, 128), s, F16).cuda() for h, s in ((4, 1), (1, 2), (1, 3)))
+    at, cu, n, t = torch.arange(75, device="cuda"), starts(lens), i32(lens), dev(table)
+    c = ctx()
+
+    def layer():
+        x, y = c.rotary(q, cos, sin, at, k=k)
+        cache = c.kv4_cache(pages, 1, 16, 128)
+        c.kv4_append(cache, y, v, t, cu, n)
+        return x, y, c.attention_prompt(x, y, v, cu), c.attention_kv4(cache, x, t, cu, n, max_tokens=70), *cache.tensors
+    want = layer()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = layer()
+        c.flush()
+        assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
