@@ -43,6 +43,10 @@ template <typename... A> static inline cudaError_t ovk_allow_smem(void (*kernel)
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
 }
 
+// Positions are below 2^30: a window of that and more leaves out none, which is what 0 says.  (Beside the largest 64-bit
+// numbers the kernels' differences would wrap.)
+static inline int64_t ovk_window(int64_t window) { return window >= (int64_t(1) << 30) ? 0 : window; }
+
 constexpr int64_t OVK_MAX_HEADS = (1 << 16) - 1;  // heads are a grid dimension
 
 // A [tokens, heads, head_dim] tensor with contiguous heads; `what` names it in the message.  Strides

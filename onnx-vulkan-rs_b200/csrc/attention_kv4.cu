@@ -103,7 +103,7 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
     a.cu = batch->cu_tokens, a.lens = batch->lens, a.table = batch->block_table;
     a.q = q->data, a.out = out->data;
     a.q_token = q->token_stride, a.q_head = q->head_stride, a.o_token = out->token_stride, a.o_head = out->head_stride;
-    a.max_pages = batch->max_pages, a.window = window;
+    a.max_pages = batch->max_pages, a.window = ovk_window(window);
     a.tokens = int(batch->tokens), a.batch = int(batch->batch), a.pages = int(cache->pages), a.kv_heads = int(cache->kv_heads);
     a.group = int(q->heads / cache->kv_heads), a.page_size = int(cache->page_size);
     a.page_shift = -1;

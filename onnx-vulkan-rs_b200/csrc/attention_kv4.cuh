@@ -606,7 +606,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
             }
         const int pos_first = seq.len - seq.n + row0 / a.group;                    // of the tile's first row
         const int pos_last = seq.len - seq.n + (row0 + rows - 1) / a.group;
-        const int window = int(min(a.window, int64_t(1) << 30));  // positions are below 2^30
+        const int window = int(a.window);
         // where the rows that this lane addresses for ldmatrix lie: token lane % 16, and of two neighbouring chunks
         // the one that lanes 16-31 read.  Rows eight apart have the same swizzle.
         uint32_t k_at[NCH / 2];

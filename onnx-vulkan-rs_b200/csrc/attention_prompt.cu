@@ -291,7 +291,8 @@ extern "C" int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p
     a.cu_q = cu_q, a.cu_k = cu_k;
     a.q_tokens = int(p->q_tokens), a.k_tokens = int(p->k_tokens), a.batch = int(p->batch);
     a.heads = int(q->heads), a.group = int(q->heads / k->heads), a.head_dim = int(p->head_dim);
-    a.causal = p->causal != 0, a.window = p->window, a.scale_log2e = p->scale * 1.4426950408889634f;
+    a.causal = p->causal != 0, a.scale_log2e = p->scale * 1.4426950408889634f;
+    a.window = ovk_window(p->window);
     a.max_q = p->max_q;
     a.vec = ovk_rows_aligned(q, elem) && ovk_rows_aligned(k, elem) && ovk_rows_aligned(v, elem);
     a.status = ctx->dev_status;

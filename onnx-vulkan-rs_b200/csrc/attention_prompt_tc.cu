@@ -683,7 +683,7 @@ template <int DP> int32_t launch(ovk_ctx *ctx, const PromptArgs &a, bool *taken)
     p.a = a;
     p.by_heads = C::NS == 2 && a.group % 2 == 0;
     p.pairs = p.by_heads ? a.heads / 2 : a.heads;
-    p.window = a.window >= (int64_t(1) << 30) ? 0 : int(a.window);
+    p.window = int(a.window);
     p.vec_out = aligned_to(a.out, 16) && a.o_token % 8 == 0 && a.o_head % 8 == 0;
     const int64_t rows = C::NS == 2 && !p.by_heads ? 2 * BM : BM;
     const int64_t grid = prompt_tiles(a, rows) * p.pairs;

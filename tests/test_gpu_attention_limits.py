@@ -259,3 +259,20 @@ def test_a_context_of_the_default_stream_under_another_current_stream():
         assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("window", [2 ** 63 - 1, 2 ** 40, 2 ** 31, 2 ** 30])
+def test_windows_of_any_size(dtype, window):
+    """A window longer than any sequence is none, also where there are more new tokens than keys."""
+    cache, table = filled_cache([2, 50], 1, 64, 32, 16, True, 3)
+    q = randn((6, 2, 64), 9, dtype)
+    got = ctx().attention_kv4(cache, q.cuda(), dev(table), starts([5, 1]), i32([2, 50]), max_tokens=5, window=window)
+    ctx().flush()
+    check_kv4(cache, table, q, [5, 1], [2, 50], 64 ** -0.5, 0, got.cpu())
+    q, k, v = randn((140, 2, 64), 1, dtype), randn((12, 1, 64), 2, dtype), randn((12, 1, 64), 3, dtype)
+    for causal in (True, False):
+        got = ctx().attention_prompt(q.cuda(), k.cuda(), v.cuda(), i32([0, 140]), cu_k=i32([0, 12]), causal=causal, window=window)
+        want = ctx().attention_prompt(q.cuda(), k.cuda(), v.cuda(), i32([0, 140]), cu_k=i32([0, 12]), causal=causal)
+        ctx().flush()
+        assert torch.equal(got, want)
+
+
