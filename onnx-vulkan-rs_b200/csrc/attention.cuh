@@ -43,6 +43,9 @@ template <typename... A> static inline cudaError_t ovk_allow_smem(void (*kernel)
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
 }
 
+// The factor that brings scores to powers of two; not finite where the scale, or this product, is not.
+static inline float ovk_scale_log2e(float scale) { return scale * 1.4426950408889634f; }
+
 // Positions are below 2^30: a window of that and more leaves out none, which is what 0 says.  (Beside the largest 64-bit
 // numbers the kernels' differences would wrap.)
 static inline int64_t ovk_window(int64_t window) { return window >= (int64_t(1) << 30) ? 0 : window; }

@@ -88,7 +88,8 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
     OVK_REQUIRE(ctx, batch->tokens * q->heads < (int64_t(1) << 31) - 64, "%s: %lld tokens of %lld heads are too many for one call", op,
                 (long long)batch->tokens, (long long)q->heads);
     OVK_REQUIRE(ctx, window >= 0, "%s: window %lld", op, (long long)window);
-    OVK_REQUIRE(ctx, scale == scale && scale - scale == 0.0f, "%s: scale is not finite", op);
+    const float factor = ovk_scale_log2e(scale);
+    OVK_REQUIRE(ctx, factor - factor == 0.0f, "%s: scale %g is not finite, or not in powers of two", op, double(scale));
     OVK_REQUIRE(ctx, ctx, "%s: null context", op);
     if (batch->tokens == 0 || batch->batch == 0)
         return OVK_OK;
@@ -112,7 +113,7 @@ extern "C" int32_t ovk_attention_kv4(ovk_ctx *ctx, const ovk_kv4_cache *cache, c
             a.page_shift = s;
     a.blocks = int(cache->head_dim / cache->block_size);
     a.chunk_shift = cache->block_size == 32 ? 0 : cache->block_size == 64 ? 1 : 2;
-    a.scale_log2e = scale * 1.4426950408889634f;
+    a.scale_log2e = factor;
     a.status = ctx->dev_status;
 
     const int tiles = tiles_for(max_tokens, a.group);

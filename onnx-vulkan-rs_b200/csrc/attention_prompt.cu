@@ -264,7 +264,8 @@ extern "C" int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p
                 "%s: %lld query and %lld key rows of %lld sequences", op, (long long)p->q_tokens, (long long)p->k_tokens, (long long)p->batch);
     OVK_REQUIRE(ctx, p->max_q >= 0, "%s: max_q %d", op, p->max_q);
     OVK_REQUIRE(ctx, p->window >= 0, "%s: window %lld", op, (long long)p->window);
-    OVK_REQUIRE(ctx, p->scale - p->scale == 0.0f, "%s: scale is not finite", op);
+    const float factor = ovk_scale_log2e(p->scale);
+    OVK_REQUIRE(ctx, factor - factor == 0.0f, "%s: scale %g is not finite, or not in powers of two", op, double(p->scale));
     const size_t elem = ovk_elem_bytes(p->dtype);
     int32_t rc = ovk_check_heads(ctx, op, "q", q, p->q_tokens, p->head_dim, elem, false);
     if (rc == OVK_OK)
@@ -291,7 +292,7 @@ extern "C" int32_t ovk_attention_prompt(ovk_ctx *ctx, const ovk_prompt_params *p
     a.cu_q = cu_q, a.cu_k = cu_k;
     a.q_tokens = int(p->q_tokens), a.k_tokens = int(p->k_tokens), a.batch = int(p->batch);
     a.heads = int(q->heads), a.group = int(q->heads / k->heads), a.head_dim = int(p->head_dim);
-    a.causal = p->causal != 0, a.scale_log2e = p->scale * 1.4426950408889634f;
+    a.causal = p->causal != 0, a.scale_log2e = factor;
     a.window = ovk_window(p->window);
     a.max_q = p->max_q;
     a.vec = ovk_rows_aligned(q, elem) && ovk_rows_aligned(k, elem) && ovk_rows_aligned(v, elem);
