@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 import os
 import struct
 
@@ -102,6 +103,37 @@ def _raw_stream():
 def _capturing():
     import torch
     return torch.cuda.is_current_stream_capturing
+
+
+def _whole(what: str, v, most: int = 2 ** 63 - 1) -> int:
+    """A whole number that a signed field holds whose largest value is `most`."""
+    try:
+        n = operator.index(v)
+    except TypeError:
+        raise OvkError(INVALID_ARGUMENT, f"{what}: a whole number is needed, not {v!r}") from None
+    if not -most - 1 <= n <= most:
+        raise OvkError(INVALID_ARGUMENT, f"{what}: {n} is too large")
+    return n
+
+
+def _scale(what: str, scale) -> float:
+    """A scale as an f32 field takes it (what is not finite is refused behind the C interface)."""
+    try:
+        scale = float(scale)
+    except (TypeError, ValueError, OverflowError):
+        raise OvkError(INVALID_ARGUMENT, f"{what}: scale {scale!r} is no number") from None
+    return scale if abs(scale) <= 3.4028234663852886e38 or scale != scale else float("inf")
+
+
+def _dims(what: str, t, *ranks: int) -> int:
+    """How many dimensions a tensor has, one of `ranks`."""
+    try:
+        n = t.dim()
+    except AttributeError:
+        raise OvkError(INVALID_ARGUMENT, f"{what}: a tensor is needed, not {type(t).__name__}") from None
+    if n not in ranks:
+        raise OvkError(INVALID_ARGUMENT, f"{what}: {' or '.join(map(str, ranks))} dimensions are needed, not {list(t.shape)}")
+    return n
 
 
 class _PackedCalls:
@@ -685,16 +717,31 @@ class Context:
         x = self._activation("Rotary: q", q)
         n, h, d = q.shape
         kind = q.dtype
-        rows, pairs = cos.shape if cos.dim() == 2 else (0, 0)
-        axes = 1 if positions.dim() == 1 else positions.shape[0]
+        try:
+            rows, pairs = cos.shape
+            flat = positions.dim() == 1
+            axes = 1 if flat else positions.shape[0]
+        except (AttributeError, ValueError, IndexError, TypeError):
+            _dims("Rotary: cos", cos, 2)
+            _dims("Rotary: positions", positions, 1, 2)
+            raise
         codes = _activation_codes()
-        at = self._indices("Rotary: positions", positions, (n,) if positions.dim() == 1 else (axes, n), _index_codes())
+        at = self._indices("Rotary: positions", positions, (n,) if flat else (axes, n), _index_codes())
         c = self._indices("Rotary: cos", cos, (rows, pairs), codes)
         s = self._indices("Rotary: sin", sin, (rows, pairs), (cos.dtype,))
         if sections is None:
             sections = (pairs,)
-        if len(sections) != axes or axes > 4:
-            raise OvkError(INVALID_ARGUMENT, f"Rotary: {len(sections)} sections for {axes} axes (1 to 4)")
+        try:
+            if len(sections) != axes or axes > 4:
+                raise OvkError(INVALID_ARGUMENT, f"Rotary: {len(sections)} sections for {axes} axes (1 to 4)")
+            p = _PACK_ROTARY(n, d, 2 * pairs, rows, codes[kind], codes[cos.dtype], _index_codes()[positions.dtype], 1 if interleaved else 0, axes,
+                             *sections, *(0,) * (4 - axes))
+        except (TypeError, struct.error):
+            if not hasattr(sections, "__len__"):
+                raise OvkError(INVALID_ARGUMENT, f"Rotary: sections are pairs per axis, not {sections!r}") from None
+            for v in sections:
+                _whole("Rotary: sections", v, 2 ** 31 - 1)
+            raise
         stream = self._foreign_stream()
         if k is not None:
             x += self._activation("Rotary: k", k, n, None, d, kind)
@@ -709,8 +756,6 @@ class Context:
         else:
             y = self._activation("Rotary: out", out, n, h, d, kind)
         self._keep(stream, q, k, cos, sin, positions, out, k_out)
-        p = _PACK_ROTARY(n, d, 2 * pairs, rows, codes[kind], codes[cos.dtype], _index_codes()[positions.dtype], 1 if interleaved else 0, axes,
-                         *sections, *(0,) * (4 - axes))
         if k is None:
             self.check(self._fast.ovk_rotary(self.h, p, 1, _PACK_HEADS(*x), _PACK_HEADS(*y), at, c, s))
             return out
@@ -720,7 +765,12 @@ class Context:
     def kv4_cache(self, pages, kv_heads, page_size, head_dim, block_size=32, zero_points=True):
         """An empty paged 4-bit cache; with pages = batch and a block table of one column, a [batch, kv_heads, capacity] one."""
         import torch
-        blocks = head_dim // block_size if block_size else 0
+        pages, kv_heads, page_size, head_dim, block_size = (
+            _whole("KV4Cache: " + name, v) for name, v in (("pages", pages), ("kv_heads", kv_heads), ("page_size", page_size), ("head_dim", head_dim),
+                                                          ("block_size", block_size)))
+        if min(pages, kv_heads, page_size, head_dim) < 0 or block_size < 1:
+            raise OvkError(INVALID_ARGUMENT, f"KV4Cache: {pages} pages of {kv_heads} heads x {page_size} places x {head_dim} in blocks of {block_size}")
+        blocks = head_dim // block_size
         zeros = lambda last, dtype: torch.zeros((pages, kv_heads, page_size, last), dtype=dtype, device=torch.device("cuda", self.device))  # noqa: E731
 
         def make():
@@ -737,8 +787,12 @@ class Context:
     def _kv4_batch(self, what, cache, tokens, block_table, cu_tokens, lens):
         if cache.device != self.device:
             raise OvkError(INVALID_ARGUMENT, f"{what}: the cache is on cuda:{cache.device}, the context on cuda:{self.device}")
-        batch = lens.shape[0] if lens.dim() == 1 else -1
-        pages = block_table.shape[1] if block_table.dim() == 2 else -1
+        try:
+            batch, pages = lens.shape[0], block_table.shape[1]
+        except (AttributeError, IndexError):
+            _dims(what + ": lens", lens, 1)
+            _dims(what + ": block_table", block_table, 2)
+            raise
         i32 = _int32()
         return _PACK_BATCH(tokens, batch, pages, self._indices(what + ": cu_tokens", cu_tokens, (batch + 1,), i32),
                            self._indices(what + ": lens", lens, (batch,), i32),
@@ -747,6 +801,8 @@ class Context:
     def kv4_append(self, cache: "KV4Cache", k, v, block_table, cu_tokens, lens):
         """Rounds the new tokens' keys and values [tokens, kv_heads, head_dim] to 4 bits and writes them: sequence b brings rows
         cu_tokens[b] .. cu_tokens[b + 1] - 1, the last of its lens[b] positions; block_table is [batch, max_pages]."""
+        if not isinstance(cache, KV4Cache):
+            raise OvkError(INVALID_ARGUMENT, f"KV4Append: a KV4Cache is needed, not {type(cache).__name__}")
         hk = self._activation("KV4Append: k", k, None, cache.kv_heads, cache.head_dim)
         n = k.shape[0]
         hv = self._activation("KV4Append: v", v, n, cache.kv_heads, cache.head_dim, k.dtype)
@@ -761,9 +817,15 @@ class Context:
         max_tokens: the most new tokens a sequence is expected to bring (it chooses how many rows are computed together;
         results hold for any number); scale: 1 / sqrt(head_dim) unless given; window: positions a token reads, its own
         included (0: all before it)."""
+        if not isinstance(cache, KV4Cache):
+            raise OvkError(INVALID_ARGUMENT, f"AttentionKV4: a KV4Cache is needed, not {type(cache).__name__}")
         hq = self._activation("AttentionKV4: q", q, None, None, cache.head_dim)
         n, h, d = q.shape
         b = self._kv4_batch("AttentionKV4", cache, n, block_table, cu_tokens, lens)
+        # ctypes takes any int for a 64-bit field
+        if not (type(max_tokens) is int is type(window) and 0 <= max_tokens < 1 << 63 and 0 <= window < 1 << 63):
+            max_tokens, window = _whole("AttentionKV4: max_tokens", max_tokens), _whole("AttentionKV4: window", window)
+        scale = d ** -0.5 if scale is None else _scale("AttentionKV4", scale)
         code = _activation_codes()[q.dtype]
         stream = self._foreign_stream()
         if out is None:
@@ -783,7 +845,7 @@ class Context:
             space = torch.empty(need, dtype=torch.uint8, device=q.device)
             space[:4096].zero_()
         self.check(self._fast.ovk_attention_kv4(self.h, cache.packed, b, _PACK_HEADS(*hq), _PACK_HEADS(*ho), code, max_tokens,
-                                                cache.head_dim ** -0.5 if scale is None else scale, window,
+                                                scale, window,
                                                 None if space is None else space.data_ptr(), need))
         return out
 
@@ -797,9 +859,20 @@ class Context:
         kind = q.dtype
         hk = self._activation("AttentionPrompt: k", k, None, None, d, kind)
         hv = self._activation("AttentionPrompt: v", v, k.shape[0], k.shape[1], d, kind)
-        batch = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
+        try:
+            batch = cu_q.shape[0] - 1
+        except (AttributeError, IndexError):
+            _dims("AttentionPrompt: cu_q", cu_q, 1)
+            raise
         pq = self._indices("AttentionPrompt: cu_q", cu_q, (max(batch, 0) + 1,), _int32())
         pk = pq if cu_k is None or cu_k is cu_q else self._indices("AttentionPrompt: cu_k", cu_k, (batch + 1,), _int32())
+        scale = d ** -0.5 if scale is None else _scale("AttentionPrompt", scale)
+        try:
+            p = _PACK_PROMPT(n, k.shape[0], batch, d, _activation_codes()[kind], 1 if causal else 0, window, scale, max_q or 0)
+        except struct.error:
+            _whole("AttentionPrompt: window", window)
+            _whole("AttentionPrompt: max_q", max_q, 2 ** 31 - 1)
+            raise
         stream = self._foreign_stream()
         if out is None:
             out = self._new(q, stream)
@@ -807,8 +880,6 @@ class Context:
         else:
             ho = self._activation("AttentionPrompt: out", out, n, h, d, kind)
         self._keep(stream, q, k, v, cu_q, cu_k, out)
-        p = _PACK_PROMPT(n, k.shape[0], batch, d, _activation_codes()[kind], 1 if causal else 0, window, d ** -0.5 if scale is None else scale,
-                         int(max_q or 0))
         self.check(self._fast.ovk_attention_prompt(self.h, p, _PACK_HEADS(*hq), _PACK_HEADS(*hk), _PACK_HEADS(*hv), pq, pk, _PACK_HEADS(*ho)))
         return out
 
@@ -884,6 +955,9 @@ class KV4Cache:
 
     def __init__(self, k, v, k_scales, v_scales, k_zero_points=None, v_zero_points=None):
         import torch
+        for t in (k, v, k_scales, v_scales, *(t for t in (k_zero_points, v_zero_points) if t is not None)):
+            if not isinstance(t, torch.Tensor):
+                raise OvkError(INVALID_ARGUMENT, f"KV4Cache: tensors are needed, not {type(t).__name__}")
         self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
         self.k_zero_points, self.v_zero_points = k_zero_points, v_zero_points
         self.tensors = tuple(t for t in (k, v, k_scales, v_scales, k_zero_points, v_zero_points) if t is not None)
