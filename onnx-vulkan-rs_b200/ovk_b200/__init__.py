@@ -628,7 +628,9 @@ class Context:
         """interp::gather_block_quantized (interp.rs:2874).  `indices`: a torch CUDA tensor (read on the
         device), or a CPU tensor / numpy array / list (checked on the host first, as the reference does)."""
         import torch
-        rows, half = table.shape
+        if len(table.shape) != 2 and (len(table.shape) < 2 or any(n != 1 for n in table.shape[2:])):
+            raise OvkError(INVALID_ARGUMENT, f"GatherBlockQuantized: a table of [rows, bytes] is needed, not {list(table.shape)}")
+        rows, half = table.shape[:2]
         cols = half * 2
         on_host = not (isinstance(indices, torch.Tensor) and indices.is_cuda)
         if on_host:

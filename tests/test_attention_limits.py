@@ -85,3 +85,8 @@ def test_caches_of_what_is_no_tensor():
     code, scale = torch.zeros((2, 1, 4, 64), dtype=torch.uint8), torch.zeros((2, 1, 4, 4), dtype=torch.float16)
     for args in ((None, code, scale, scale), (code, None, scale, scale), (code, code, [1], scale), (code, code, scale, scale, 3, 3)):
         refused(ovk_b200.KV4Cache, *args, word="tensors")
+
+
+@pytest.mark.parametrize("shape", [(6,), (3, 2, 4), (3, 2, 1, 2)])
+def test_gather_of_a_table_that_is_none(context, shape):
+    refused(context.gather_block_quantized, torch.zeros(shape, dtype=torch.uint8), [0], None, None, 32, word="table")
