@@ -276,3 +276,17 @@ def test_windows_of_any_size(dtype, window):
         assert torch.equal(got, want)
 
 
+def test_fresh_contexts_start_with_cleared_counters():
+    """The first call of a context that was just made, several blocks sharing a sequence."""
+    lens = [6000]
+    cache, table = filled_cache(lens, 1, 128, 32, 64, True, 3)
+    q, t, cu, n = randn((1, 8, 128), 1, F16).cuda(), dev(table), starts([1]), i32(lens)
+    want = ctx().attention_kv4(cache, q, t, cu, n).clone()
+    ctx().flush()
+    for _ in range(20):
+        c = ovk_b200.Context(0)
+        got = torch.empty_like(q)
+        c.attention_kv4(cache, q, t, cu, n, out=got)
+        c.flush()
+        assert torch.equal(got, want)
+        c.close()
