@@ -1,5 +1,6 @@
 """The attention operators at the ends of what their interface allows, against the definitions in 64 bits: widths between the
 16-byte words, bounds that disagree with the call, scores and weights far apart, values in places that are masked."""
+import ctypes as C
 import math
 
 import numpy as np
@@ -289,4 +290,99 @@ def test_fresh_contexts_start_with_cleared_counters():
         c.attention_kv4(cache, q, t, cu, n, out=got)
         c.flush()
         assert torch.equal(got, want)
+        c.close()
+
+
+# --------------------------------------------------------- calls that no other test makes
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,block", [(64, 32), (128, 128), (256, 64)])
+def test_append_of_slices_at_any_alignment(dtype, d, block):
+    """Keys and values as slices of one wide product that starts anywhere: the same codes as from tensors of their own."""
+    wide = randn((21, 4 * d + 3), 1, dtype).cuda()
+    k, v = wide[:, 1:1 + 2 * d].unflatten(1, (2, d)), wide[:, 3 + 2 * d:].unflatten(1, (2, d))
+    lens, caches = [20, 1], []
+    for a, b in ((k, v), (k.contiguous(), v.contiguous())):
+        cache = ctx().kv4_cache(5, 2, 8, d, block)
+        ctx().kv4_append(cache, a, b, i32([[4, 1, 0], [3, -1, -1]]), starts(lens), i32(lens))
+        ctx().flush()
+        caches.append((ctx().last_kernel, cache))
+    assert [c[0] for c in caches] == ["kv4_append_scalar", "kv4_append"]
+    assert all(torch.equal(x, y) for x, y in zip(caches[0][1].tensors, caches[1][1].tensors))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_kv4_sequences_that_share_pages(dtype):
+    """A common beginning of three sequences lies in the cache once."""
+    lens = [48, 61, 70]
+    cache, table = filled_cache([100, 40, 40], 1, 128, 32, 16, True, 5)
+    shared = np.array([[table[0][0], table[0][1], table[0][2], -1, -1], [*table[0][:3], table[1][0], -1], [*table[0][:3], table[2][0], table[2][1]]],
+                      dtype=np.int32)
+    q = randn((3, 8, 128), 9, F32, 1.5).to(dtype)
+    got = ctx().attention_kv4(cache, q.cuda(), dev(shared), starts([1] * 3), i32(lens))
+    ctx().flush()
+    check_kv4(cache, shared, q, [1] * 3, lens, 128 ** -0.5, 0, got.cpu())
+
+
+def test_kv4_workspaces_of_the_caller():
+    """Through the C interface: a workspace of the stated size gives the same bits and is left zeroed; less is refused."""
+    lib, c, lens = ovk_b200.lib(), ctx(), [9000, 3]
+    cache, table = filled_cache(lens, 1, 128, 32, 64, True, 3)
+    q, t, cu, n = randn((2, 8, 128), 1, F16).cuda(), dev(table), starts([1, 1]), i32(lens)
+    want = c.attention_kv4(cache, q, t, cu, n)
+    out = torch.empty_like(q)
+    heads = lambda x: ovk_b200.Heads(x.data_ptr(), 8, 1024, 128)  # noqa: E731
+    batch = ovk_b200.KV4Batch(2, 2, t.shape[1], cu.data_ptr(), n.data_ptr(), t.data_ptr())
+    size = C.c_size_t()
+    assert lib.ovk_attention_kv4_workspace(c.h, cache.params, 8, 1, ovk_b200.FLOAT16, C.byref(size)) == ovk_b200.OK
+    space = torch.full((size.value + 16,), 255, dtype=torch.uint8, device="cuda")
+    space[:4096] = 0
+
+    def call(at, size):
+        return lib.ovk_attention_kv4(c.h, cache.params, batch, heads(q), heads(out), ovk_b200.FLOAT16, 1, 128 ** -0.5, 0, at, size)
+    for _ in range(3):
+        out.zero_()
+        assert call(space.data_ptr(), size.value) == ovk_b200.OK
+        c.flush()
+        assert torch.equal(out, want) and int(space[:4096].sum()) == 0 and bool((space[-16:] == 255).all())
+    assert call(space.data_ptr(), 4096) == ovk_b200.INVALID_ARGUMENT and call(space.data_ptr() + 8, size.value) == ovk_b200.INVALID_ARGUMENT
+    stream = torch.cuda.Stream()
+    own = ovk_b200.Context(0, stream.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):  # the context's own workspace would be shared by all graphs
+        rc = lib.ovk_attention_kv4(own.h, cache.params, batch, heads(q), heads(out), ovk_b200.FLOAT16, 1, 1.0, 0, None, 0)
+        out.zero_()
+    assert rc == ovk_b200.INVALID_ARGUMENT and b"workspace" in lib.ovk_last_error(own.h)
+    del graph
+    own.close()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_every_operator_repeats_itself(dtype):
+    """Results do not depend on timing: the same bits ten times, two contexts at once."""
+    lens = [700, 3, 1500]
+    total = sum(lens)
+    table, pages = make_table(lens, 16, 1)
+    cos, sin = (torch.rand(1500, 64, device="cuda") for _ in range(2))
+    q, k, v = (randn((total, h, 128), s, dtype).cuda() for h, s in ((8, 1), (2, 2), (2, 3)))
+    at = torch.cat([torch.arange(n) for n in lens]).cuda()
+    cu, n, t, last = starts(lens), i32(lens), dev(table), starts([1] * 3)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    contexts = [ovk_b200.Context(0, s.cuda_stream) for s in streams]
+    torch.cuda.synchronize()
+    first = None
+    for _ in range(10):
+        results = []
+        for c, s in zip(contexts, streams):
+            with torch.cuda.stream(s):
+                x, y = c.rotary(q, cos, sin, at, k=k)
+                cache = c.kv4_cache(pages, 2, 16, 128)
+                c.kv4_append(cache, y, v, t, cu, n)
+                results.append((x, y, *cache.tensors, c.attention_prompt(x, y, v, cu), c.attention_kv4(cache, x[:3].contiguous(), t, last, n)))
+        for c in contexts:
+            c.flush()
+        first = first or results[0]
+        for r in results:
+            assert all(torch.equal(a, b) for a, b in zip(r, first))
+    for c in contexts:
         c.close()
