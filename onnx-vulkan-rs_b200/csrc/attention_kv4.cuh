@@ -29,10 +29,12 @@
 //  - V: codes minus zero (exact, so that a value of 0 adds nothing: the zeros as a
 //    product of their own left 2^-17 of them behind) times p * s rounded to fp16.
 //    f32 callers get q and p * s as two fp16 parts, 22 bits.
-//  - The running maximum moves only when a score passes it by 6 (p by 2^6) or a V
-//    scale its own largest by 2^3: p * s starts at 2^6 to 2^7, so it stays below
-//    2^16 and is a normal fp16 number down to 2^-20 of the largest, and a step
-//    needs one vote, not a reduction.
+//  - f16: the running maximum moves only when a score passes it by 6 (p by 2^6) or a
+//    V scale its own largest by 2^3: p * s starts at 2^6 to 2^7, so it stays below
+//    2^16, has all its bits down to 2^-20 of the largest and below that steps of
+//    2^-30; a step needs one vote, not a reduction.  f32: by 3 and 2^2, so that p * s
+//    starts at 2^10 and the steps are 2^-34 (four drafted tokens of six sequences
+//    12.4 us, 12.15 with f16's limits; with 2 and 2^1 12.7).
 //
 // One CTA per SM takes an equal run of units - 32 tokens for each of its consumer
 // warps - of the whole batch (lengths are read on the device).  Four producer
@@ -99,6 +101,10 @@ template <int D_, int NT_, int PARTS_> struct Shape {
     static constexpr int SMEM = 128 + RING + WARPS * SZ + MERGE + QF + ROWS * (NCH + 1) * 4 + 2 * WARPS * ROWS * 4;
     static constexpr bool Q_REGS = PARTS * NT * NCH * 4 <= 16;
     static constexpr bool SUBNORMAL = PARTS == 1;         // how codes enter the products
+    // powers of two that a score may be ahead of its row's maximum, and a V scale of its largest, before they move; and what
+    // an exponent field of the scale is lowered by, so that p * s is at most 2^(AHEAD + SCALE_AHEAD + BASE - 15) = 2^15
+    static constexpr int AHEAD = PARTS == 1 ? 6 : 3, BASE = PARTS == 1 ? 21 : 25;
+    static constexpr uint32_t SCALE_AHEAD = PARTS == 1 ? 3 : 2;
     static constexpr int SLOT = ROWS * (D + 2);           // floats of a partial result
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -623,10 +629,10 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
         const uint32_t row_at = ring + 2 * S::CODES + 2 * (S::SCALES + S::ZEROS) + place * 4;
 
         float o[NCH][2][NT][4];
-        // p = 2^(x - reference): the reference is the maximum m and the exponent, less 21, of the largest scale that the row
+        // p = 2^(x - reference): the reference is the maximum m and the exponent, less BASE, of the largest scale that the row
         // has read.  A maximum beyond FAR would round that exponent away, or up to its own last place: there it is m alone, and
         // no score may be ahead of it (p is then at most 1, which leaves any scale in fp16's range).
-        constexpr float FAR = 0x1p20f, AHEAD = 6.0f;
+        constexpr float FAR = 0x1p20f, AHEAD = S::AHEAD;
         float limit[NT][2], l[NT][2], reference[NT][2];  // limit: m and what a score may be ahead of it
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -715,7 +721,7 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                 else
                     expand(std::integral_constant<int, NCH >= 4 ? 2 : 1>());
             }
-            const bool scale_moves = __any_sync(0xffffffffu, high > top_scale + (3u << 10));
+            const bool scale_moves = __any_sync(0xffffffffu, high > top_scale + (S::SCALE_AHEAD << 10));
             __syncwarp();
 
             // ---------------------------------------------------- scores
@@ -842,10 +848,10 @@ attention_kv4_kernel(const __grid_constant__ Kv4Args a)
                         for (int o_ = 4; o_ < 32; o_ <<= 1)
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o_));
                         const float m = fabsf(limit[n][e]) > FAR ? limit[n][e] : limit[n][e] - AHEAD;
-                        const float before = m == NONE ? -21.0f : rintf(reference[n][e] - m);
+                        const float before = m == NONE ? -S::BASE : rintf(reference[n][e] - m);
                         const float to = fmaxf(m, most);
                         const bool far = fabsf(to) > FAR;
-                        const float next = far ? to : to + fmaxf(before, float(int((exponents >> (16 * n + 8 * e)) & 255u) - 21));
+                        const float next = far ? to : to + fmaxf(before, float(int((exponents >> (16 * n + 8 * e)) & 255u) - S::BASE));
                         const float f = exp2_approx(reference[n][e] - next);
                         limit[n][e] = far ? to : to + AHEAD, reference[n][e] = next;
                         l[n][e] *= f;

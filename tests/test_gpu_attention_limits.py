@@ -386,3 +386,33 @@ def test_every_operator_repeats_itself(dtype):
             assert all(torch.equal(a, b) for a, b in zip(r, first))
     for c in contexts:
         c.close()
+
+
+@pytest.mark.parametrize("dtype,below", [(F16, 24.0), (F32, 24.0), (F32, 33.0)])
+@pytest.mark.parametrize("d,hq", [(64, 2), (128, 12), (256, 4)])
+@pytest.mark.parametrize("n,peak", [(32, 0), (32, 31), (257, 30), (32767, 0), (32767, 32000)])
+def test_kv4_long_flat_tail(dtype, below, d, hq, n, peak):
+    """One token outweighs each of many by 2^below: a weight times its value's scale is off by 2^-11 (f16) or 2^-22 (f32) of
+    itself or by 2^-31 or 2^-35 of the largest weight and scale, whichever is more."""
+    table, pages = make_table([n], 64, 1)
+    cache = ctx().kv4_cache(pages, 1, 64, d, 32)
+    k, v = torch.zeros(n, 1, d), torch.ones(n, 1, d)
+    k[..., 0] = -4.0
+    k[peak, 0, 0], v[peak, 0, :2] = 0.0, 0.0
+    v[:, 0, 1] *= torch.linspace(0, 1, n)
+    ctx().kv4_append(cache, k.cuda(), v.cuda(), dev(table), starts([n]), i32([n]))
+    q = torch.zeros(1, hq, d, dtype=dtype)
+    q[..., 0] = 8.0
+    scale = below / 32.0 * math.log(2)
+    got = ctx().attention_kv4(cache, q.cuda(), dev(table), starts([1]), i32([n]), scale=scale)
+    ctx().flush()
+    at = torch.arange(n)
+    page = torch.as_tensor(table[0])[at // 64].long()
+    rows = {w: ref.dequantize(*cache_rows(cache, w))[page, 0, at % 64] for w in ("k", "v")}
+    p = torch.softmax(rows["k"] @ q[0, 0].double() * scale, 0)
+    itself, floor = (2.0 ** -11, 2.0 ** -31) if dtype == F16 else (2.0 ** -21, 2.0 ** -35)
+    largest = 15 * float(cache.v_scales.max())
+    # a score of -33 powers of two is rounded three times (33 * 3 * 2^-24 of the weight), sums of n weights are off by n 2^-23
+    bound = (p @ rows["v"].abs()) * (itself + 2.0 ** -17 + n * 2.0 ** -23) + n * floor * largest * float(p.max())
+    assert float(p[peak]) > 0.9 and float((p @ rows["v"])[0]) > 1.9 * float(bound[0])  # a tail left out is noticed
+    ref.check(got[0], (p @ rows["v"]).expand(hq, d), bound.expand(hq, d), "tail")
