@@ -110,21 +110,22 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a)
     OVK_PDL_LAUNCH_DEPENDENTS();
     OVK_PDL_WAIT();
     // bounds that leave the tensors: reported here for the whole batch, left out below
-    if (head == 0)
+    if (head == 0 && blockIdx.x <= unsigned(a.batch - 1) / 256)  // few blocks of a large grid
         for (int64_t b = int64_t(blockIdx.x) * 256 + threadIdx.x; b < a.batch; b += int64_t(gridDim.x) * 256)
             if (a.cu[b] < 0 || a.cu[b + 1] < a.cu[b] || a.cu[b + 1] > a.tokens)
                 atomicExch(a.status, OVK_DEV_BAD_SEQUENCE);
     int row = -1;  // rows of the cache are fewer than 2^31
     if (token < a.tokens) {
         const int b = sequence_of(a.cu, a.batch, token, a.tokens);
-        if (b >= 0 && a.cu[b] >= 0 && a.cu[b + 1] <= a.tokens) {
-            const int length = a.lens[b], from_end = a.cu[b + 1] - token;
+        if (b >= 0) {
+            const int length = a.lens[b], first = a.cu[b], end = a.cu[b + 1], from_end = end - token;  // one way to memory
+            const bool inside = first >= 0 && end <= a.tokens;
             const uint32_t position = uint32_t(length) - uint32_t(from_end);
             const uint32_t page = a.page_shift >= 0 ? position >> a.page_shift : position / uint32_t(a.page_size);
-            const int where = length >= from_end && page < a.max_pages ? a.table[b * a.max_pages + page] : -1;
+            const int where = inside && length >= from_end && page < a.max_pages ? a.table[b * a.max_pages + page] : -1;
             if (where >= 0 && where < a.pages)
                 row = (where * a.heads + head) * a.page_size + int(position - page * a.page_size);
-            else if (pair == 0)
+            else if (inside && pair == 0)
                 atomicExch(a.status, OVK_DEV_BAD_PAGE);
         }
     }
