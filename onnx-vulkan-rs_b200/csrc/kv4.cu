@@ -1,10 +1,12 @@
 // The 4-bit key / value cache: argument checks and the write of new tokens.
 //
 // Bytes ought to bound the write: 2 or 4 bytes are read per value and about 0.6
-// stored.  What does is issue: 21784 tokens in f32, one head of 256, keys and values,
-// 50 MB, take some 17.6 us (2.9 TB/s); with eight values a thread 19.6 at 74 % of the
-// issue slots, of which a third went into the values and the rest into places, ranges
-// and scales.
+// stored.  What does is latency: 21784 tokens in f32, one head of 256, keys and values,
+// 50 MB, take 17.3 us from memory (2.9 TB/s), 12.6 from L2, with 53 % of the issue slots
+// and 32 % of the memory's rate in use: 1.2 of 6.7 warps a scheduler can issue, since a
+// row is asked for behind three dependent reads (bounds, length, page).  (With eight
+// values a thread issue did, 74 % of the slots at 19.6 us; asking for rows before the
+// page gained nothing there and was not tried since.)
 // A thread holds sixteen values of a row - two 32-bit words of codes - and the
 // block_size / 16 threads of a block find its range with shuffles; keys and values
 // of a row go through the same thread, so its place in the cache is found once.
