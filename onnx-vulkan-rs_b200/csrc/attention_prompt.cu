@@ -7,10 +7,11 @@
 // holds 64 query rows of one head and walks 64 or 32 keys at a time; a thread
 // computes 8 (256-wide heads: 4) x 4 or 2 scores, then as many rows x head_dim / 16
 // columns of the result.  All of it is f32 arithmetic on the CUDA cores: a step over
-// four d is twelve 16-byte loads of shared memory for 128 multiply-adds, so the
-// adders and not shared memory bound it.  Four chunks of 600 queries after 333 keys, f32,
-// 8 heads of 64: 188 us, 20.9 TFLOP/s counted over the pairs that are read (29 % of the
-// adders' 72; the diagonal's tiles are computed whole and short sequences leave SMs idle).
+// four d is twelve 16-byte loads of shared memory for 128 multiply-adds, and both pipes
+// are busy half of the time (adders 49 %, shared memory 50 %, issue 62 %, 2.2 warps a
+// scheduler).  Four chunks of some 600 queries after 333 keys, f32, 8 heads of 64: 189 us,
+// 20.8 TFLOP/s counted over the pairs that are read (29 % of the adders' 72): the diagonal's
+// tiles are computed whole, and 376 blocks of unequal length are one uneven wave.
 #include "attention_prompt.cuh"
 
 namespace {

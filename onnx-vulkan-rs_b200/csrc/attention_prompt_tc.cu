@@ -24,11 +24,12 @@
 // (The core's queue is short - a warp that issues runs at the core's pace - and a
 // wait costs some 300 cycles even where nothing is to be waited for: one issuer for
 // both tiles took 308 us for 8192 tokens of 16 heads, two 294, with two buffers 280:
-// 982 TFLOP/s (keys with outlier channels; 238 us, 1150, where all are alike).  What is left is the softmax's own latency: 128 rows are four warps,
-// one to a scheduler, and the two tiles run in step.)  256-wide heads fill tensor
+// 980 TFLOP/s, 416000 cycles; replayed for a few milliseconds 239 us, 1150 TFLOP/s.
+// What is left is the softmax's own latency: 128 rows are four warps, one to a
+// scheduler, and the two tiles run in step.)  256-wide heads fill tensor
 // memory with one tile's O, so there one tile has two S buffers of 128 keys, one warp
 // issues Q K^T and the other P V, and the next scores are computed before the last
-// weights are used: 408 us for 8192 tokens of 16 heads, 1350 TFLOP/s.
+// weights are used: 408 us for 8192 tokens of 16 heads so replayed, 1350 TFLOP/s.
 //
 // A block is one query tile (or two) from its first load to its last store, one on
 // an SM at a time: some 15000 cycles pass outside the products (lookup 1200, first
