@@ -592,9 +592,9 @@ OVK_API int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, const o
  * f32; what enters the products is fp16 (the tensor cores take nothing wider): the
  * queries, for OVK_FLOAT as two parts of 22 bits together, and each weight times a
  * value's scale, rounded alike (off by 2^-11 or 2^-22 of itself, or by 2^-31 or 2^-35
- * of the row's largest weight times the largest scale it reads, if more).  Scores of OVK_FLOAT16 queries are good to 2^-17 of the
- * largest product in them.  q and out are [tokens, q_heads, head_dim] of `dtype`,
- * 16-byte aligned rows.
+ * of the row's largest weight times the largest scale it reads, if that is more).
+ * Scores of OVK_FLOAT16 queries are good to 2^-17 of the largest product in them.  q
+ * and out are [tokens, q_heads, head_dim] of `dtype`, 16-byte aligned rows.
  * max_tokens: the most new tokens a sequence is expected to bring (1 in decode); it
  * chooses how many rows are computed together, results hold for any number.
  * workspace: partial results of sequences that several CTAs share, 16-byte
