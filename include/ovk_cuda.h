@@ -594,7 +594,8 @@ OVK_API int32_t ovk_kv4_append(ovk_ctx *ctx, const ovk_kv4_cache *cache, const o
  * value's scale, rounded alike (off by 2^-11 or 2^-22 of itself, or by 2^-31 or 2^-35
  * of the row's largest weight times the largest scale it reads, if that is more).
  * Scores of OVK_FLOAT16 queries are good to 2^-17 of the largest product in them.  q
- * and out are [tokens, q_heads, head_dim] of `dtype`, 16-byte aligned rows.
+ * and out are [tokens, q_heads, head_dim] of `dtype`, 16-byte aligned rows; out may be
+ * q itself.
  * max_tokens: the most new tokens a sequence is expected to bring (1 in decode); it
  * chooses how many rows are computed together, results hold for any number.
  * workspace: partial results of sequences that several CTAs share, 16-byte
@@ -620,7 +621,7 @@ OVK_API int32_t ovk_attention_kv4_workspace(ovk_ctx *ctx, const ovk_kv4_cache *c
  * fp16 (off by 2^-11 of themselves or 2^-32 of the row's largest, if that is more),
  * the sum of them as f32.  head_dim 1 to 256.  The f16 tensor-core
  * kernel takes q, k and v with 16-byte aligned rows of any width; other layouts
- * and f32 run on the CUDA cores. */
+ * and f32 run on the CUDA cores.  out may be q itself. */
 typedef struct ovk_prompt_params {
     int64_t q_tokens, k_tokens, batch, head_dim;
     int32_t dtype, causal;

@@ -416,3 +416,25 @@ def test_kv4_long_flat_tail(dtype, below, d, hq, n, peak):
     bound = (p @ rows["v"].abs()) * (itself + 2.0 ** -17 + n * 2.0 ** -23) + n * floor * largest * float(p.max())
     assert float(p[peak]) > 0.9 and float((p @ rows["v"])[0]) > 1.9 * float(bound[0])  # a tail left out is noticed
     ref.check(got[0], (p @ rows["v"]).expand(hq, d), bound.expand(hq, d), "tail")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,hq,hk", [(64, 3, 3), (128, 8, 2), (256, 4, 1)])
+def test_results_in_the_place_of_the_queries(dtype, d, hq, hk):
+    lens = [1, 700, 0, 129, 2000]
+    n = sum(lens)
+    q, k, v = (randn((n, h, d), s, dtype).cuda() for s, h in ((1, hq), (2, hk), (3, hk)))
+    want = ctx().attention_prompt(q, k, v, starts(lens))
+    x = q.clone()
+    assert ctx().attention_prompt(x, k, v, starts(lens), out=x) is x
+    ctx().flush()
+    assert torch.equal(x, want)
+    cache, table = filled_cache(lens, hk, d, 32, 16, True, 5)
+    new = [1, 40, 0, 3, 1]
+    q, cu, t, total = q[:sum(new)].contiguous(), starts(new), dev(table), i32(lens)
+    want = ctx().attention_kv4(cache, q, t, cu, total, max_tokens=40)
+    for _ in range(5):
+        x = q.clone()
+        ctx().attention_kv4(cache, x, t, cu, total, max_tokens=40, out=x)
+        ctx().flush()
+        assert torch.equal(x, want)
